@@ -58,6 +58,38 @@ int tt_qkv_post_bwd_peer(void* const* dq_ptrs, void* const* dk_ptrs, void* const
                          float* partials, void* dqw, void* dkw, long rows, int heads, long seq_in, long seq_out,
                          long out_offset, long rope_len, float eps, void* stream);
 
+/* ---- rotary positions of queries and keys, alone or behind an RMS norm of every head (rotary.cu) ---- */
+#define TT_BF16 0
+#define TT_FP16 1
+#define TT_FP32 2
+/* [batch, heads, tokens, head_dim] operands with a contiguous last dimension; strides {batch, head, token} in elements.  k_heads 0:
+ * queries only.  The pointer to the arguments is a host pointer, read before the call returns. */
+typedef struct {
+    long struct_size;                   /* sizeof(tt_rotary_args) */
+    long batch, tokens;
+    int q_heads, k_heads, head_dim, pairs;      /* head_dim even, at most 256; 2 * pairs elements are rotated */
+    int dtype, interleaved, transpose, pos_is_64;
+    const void *q, *k;                  /* inputs (tt_rotary with transpose: gradients) */
+    long q_stride[3], k_stride[3];
+    void *out_q, *out_k;
+    long out_q_stride[3], out_k_stride[3];
+    const void* positions;              /* int32, or int64 where pos_is_64; strides {batch, axis, token} */
+    long pos_stride[3];
+    const double* half_turns;           /* [pairs] angle per position, in units of pi */
+    const int* axis;                    /* [pairs] position axis of every pair, or null: axis 0 */
+    float amplitude, eps;
+    const void *q_weight, *k_weight;    /* [head_dim]; norm only */
+    const void *gq, *gk;                /* gradients of the outputs; norm backward only, where out_q, out_k are the inputs' gradients */
+    long gq_stride[3], gk_stride[3];
+    void *dq_weight, *dk_weight;
+    float* partials;                    /* scratch of the backward: partial_floats >= tt_rotary_partial_floats */
+    long partial_floats;
+} tt_rotary_args;
+long tt_rotary_partial_floats(const tt_rotary_args* args);     /* of the norm's backward; touches no device memory */
+int tt_rotary(const tt_rotary_args* args, void* stream);
+int tt_norm_rotary_fwd(const tt_rotary_args* args, void* stream);
+int tt_norm_rotary_bwd(const tt_rotary_args* args, void* stream);
+
 /* ---- activations ---- */
 int tt_gelu_fwd(const void* u, void* y, long n, int kind, void* stream);   /* kind 0 = erf, 1 = tanh */
 int tt_gelu_bwd(const void* dy, const void* u, void* du, long n, int kind, void* stream);

@@ -22,6 +22,7 @@ import torch
 
 from . import reference
 from . import optim  # noqa: F401
+from .rope import Rotary, rotary_frequencies  # noqa: F401
 
 _IMPL = os.environ.get("TELETRON_B200_IMPL", "auto")
 
@@ -69,8 +70,8 @@ def impl(name: str):
         set_impl(prev)
 
 
-def _use_cuda(*tensors: torch.Tensor) -> bool:
-    """True when the sm_100a kernels should run for these operands."""
+def _use_cuda(*tensors: torch.Tensor, dtypes=(torch.bfloat16,)) -> bool:
+    """True when the sm_100a kernels should run for these operands (``dtypes``: the types that the op's kernels take)."""
     if _IMPL == "torch":
         return False
     t0 = tensors[0]
@@ -78,9 +79,10 @@ def _use_cuda(*tensors: torch.Tensor) -> bool:
         if _IMPL == "cuda":
             raise RuntimeError("impl='cuda' requested for a non-CUDA tensor")
         return False
-    if t0.dtype != torch.bfloat16:
+    if t0.dtype not in dtypes:
         if _IMPL == "cuda":
-            raise RuntimeError("the sm_100a kernels take bf16 operands, got %s" % t0.dtype)
+            raise RuntimeError("the sm_100a kernels take %s operands, got %s"
+                               % (" / ".join({"bfloat16": "bf16", "float16": "fp16", "float32": "fp32"}[str(d)[6:]] for d in dtypes), t0.dtype))
         return False
     from . import _lib
     if not _lib.available():
@@ -122,6 +124,41 @@ def rmsnorm(x, weight, eps: float = 1e-6):
 
 def apply_rope(x, cos, sin):
     return reference.apply_rope(x, cos, sin)
+
+
+_ROTARY_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _rotary_kernel_ok(q) -> bool:
+    from . import rope
+    if not _use_cuda(q, dtypes=_ROTARY_DTYPES):
+        return False
+    if rope.supported(q):
+        return True
+    from . import fallback
+    fallback.note("rotary", f"q {tuple(q.shape)} {q.dtype}")
+    return False
+
+
+def rotary(q, k, positions, freqs):
+    """Queries and keys ``[batch, heads, tokens, head_dim]`` (any strides, head counts of their own) rotated by their positions.
+
+    ``positions``: int32 or int64, ``[tokens]`` or ``[batch, tokens]``, with several axes ``[axes, tokens]`` or ``[batch, axes, tokens]``;
+    ``freqs``: what :func:`rotary_frequencies` returns.  ``k`` may be None.  Returns head-major ``(q, k)`` of the same type; the gradients
+    come in the order of the inputs.  bf16, fp16 and fp32."""
+    from . import rope
+    p = rope.check_arguments(q, k, positions, freqs)
+    return rope.rotary(q, k, p, freqs) if _rotary_kernel_ok(q) else reference.rotary(q, k, p, freqs)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps: float = 1e-6):
+    """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``, statistics in fp32), then :func:`rotary`, rounded once."""
+    from . import rope
+    p = rope.check_arguments(q, k, positions, freqs)
+    rope.check_weights(q, k, q_weight, k_weight)
+    if _rotary_kernel_ok(q):
+        return rope.qk_norm_rotary(q, k, q_weight, k_weight, p, freqs, eps)
+    return reference.qk_norm_rotary(q, k, q_weight, k_weight, p, freqs, eps)
 
 
 def linear(x, weight, bias=None, activation=None):

@@ -7,6 +7,7 @@ contiguity, alignment) happens here in :func:`check`; shape arithmetic is re-che
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -60,6 +61,10 @@ def _load() -> Optional[ctypes.CDLL]:
     for name in ("tt_gemm_bf16", "tt_gemm2_bf16"):
         getattr(lib, name).argtypes = [vp] * 5 + [ci] * 3 + [cl] * 3 + [ci] * 3 + [vp] * 2
     lib.tt_gemm2_bf16_splitk.argtypes = [vp] * 5 + [ci] * 3 + [cl] * 3 + [ci] * 4 + [vp] * 3
+    lib.tt_rotary_partial_floats.restype = cl
+    for name in ("tt_rotary", "tt_norm_rotary_fwd", "tt_norm_rotary_bwd"):
+        getattr(lib, name).argtypes = [ctypes.c_char_p, vp]
+    lib.tt_rotary_partial_floats.argtypes = [ctypes.c_char_p]
     lib.tt_gemm2_bf16_two.argtypes = [vp] * 5 + [ci] * 4 + [cl] * 4 + [ci] + [vp] * 3
     _lib = lib
     return lib
@@ -101,6 +106,16 @@ def raw_stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (native calls launch on the current device's current stream)."""
+    if _CUR_DEVICE is not None and t.device.index == _CUR_DEVICE():
+        return _SAME_DEVICE
+    return torch.cuda.device(t.device)
+
+
 def check(t: torch.Tensor, dtype: torch.dtype, name: str, device: Optional[torch.device] = None, align: int = 16) -> torch.Tensor:
     """Validate an operand that will be read through a raw pointer."""
     if not t.is_cuda:
@@ -117,7 +132,7 @@ def check(t: torch.Tensor, dtype: torch.dtype, name: str, device: Optional[torch
 
 
 # kernels launched per native call (for the launch counter the benchmark reports)
-KERNELS_PER_CALL = {"tt_ln_mod_bwd": 2, "tt_adaln_bwd": 2, "tt_gemm2_bf16_splitk": 2, "tt_gate_residual_bwd": 2, "tt_rmsnorm_bwd": 2, "tt_qkv_post_bwd": 2, "tt_attn_bwd": 3, "tt_attn_bwd_fused": 3}
+KERNELS_PER_CALL = {"tt_ln_mod_bwd": 2, "tt_adaln_bwd": 2, "tt_gemm2_bf16_splitk": 2, "tt_gate_residual_bwd": 2, "tt_rmsnorm_bwd": 2, "tt_qkv_post_bwd": 2, "tt_norm_rotary_bwd": 2, "tt_attn_bwd": 3, "tt_attn_bwd_fused": 3}
 LAUNCHES = 0
 
 

@@ -68,6 +68,38 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
     return out.to(x.dtype)
 
 
+def rotary_positions(x: torch.Tensor, positions: torch.Tensor, freqs) -> torch.Tensor:
+    """Rotates ``x [B, h, S, D]`` by the angles of ``positions [1 or B, axes, S]`` (:class:`teletron_b200.ops.Rotary`): angles in
+    64 bits, the rotation in 32 or the wider type of ``x``, rounded once.  Elements behind ``freqs.dim`` pass."""
+    calc = torch.promote_types(x.dtype, torch.float32)
+    pos = positions.double()
+    pos = pos[:, freqs.axis.long()] if freqs.axis is not None else pos.expand(-1, freqs.inv_freq.shape[0], -1)
+    angle = pos.transpose(1, 2) * freqs.inv_freq                                   # [1 or B, S, pairs]
+    cos = (freqs.amplitude * angle.cos()).to(calc)[:, None]
+    sin = (freqs.amplitude * angle.sin()).to(calc)[:, None]
+    head, rest = x[..., :freqs.dim].to(calc), x[..., freqs.dim:]
+    if freqs.interleaved:
+        a, b = head[..., 0::2], head[..., 1::2]
+        y = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+    else:
+        a, b = head.chunk(2, dim=-1)
+        y = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+    return torch.cat([y.to(x.dtype), rest], dim=-1)
+
+
+def rotary(q, k, positions, freqs):
+    return rotary_positions(q, positions, freqs), None if k is None else rotary_positions(k, positions, freqs)
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps: float = 1e-6):
+    """RMS norm of every head in 32 bits (or the wider type), then :func:`rotary_positions`, rounded once."""
+    def one(x, w):
+        xf = x.to(torch.promote_types(x.dtype, torch.float32))
+        y = xf * torch.rsqrt(xf.pow(2).mean(dim=-1, keepdim=True) + eps) * w.to(xf.dtype)
+        return rotary_positions(y, positions, freqs).to(x.dtype)
+    return one(q, q_weight), one(k, k_weight)
+
+
 def _act(x: torch.Tensor, activation: Optional[str]) -> torch.Tensor:
     if activation is None:
         return x
