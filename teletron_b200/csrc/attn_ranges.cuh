@@ -1,0 +1,111 @@
+// Shared by the attention kernels in which every query sees one run of the keys (attn_ranges_*.cu).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "sm100.cuh"
+#include "teletron_b200.h"
+
+namespace ranges {
+
+constexpr int kTile = TT_RANGES_TILE;
+constexpr float kLog2e = 1.4426950408889634f;
+// The bias table lies in shared memory with its end values repeated for kPad entries, so that a tile that is not wholly beyond the
+// largest distance needs no clamp: its distances reach at most 127 + 31 past it.
+constexpr int kPad = 160;
+
+// A plan's parts for one sample.
+struct PlanView {
+    const int4* q_tiles;
+    const uint4* dead;
+    const int2* k_tiles;
+    const int* dirty;
+    const int *first, *behind;
+    int start;
+};
+
+struct PlanPtr {
+    const int* base;
+    tt_ranges_layout at;
+    int q_len, q_tiles, k_tiles;
+    __device__ __forceinline__ PlanView sample(int b) const {
+        PlanView v;
+        v.q_tiles = reinterpret_cast<const int4*>(base + at.q_tiles) + (long)b * q_tiles;
+        v.dead = reinterpret_cast<const uint4*>(base + at.dead) + (long)b * k_tiles;
+        v.k_tiles = reinterpret_cast<const int2*>(base + at.k_tiles) + (long)b * k_tiles;
+        v.dirty = base + at.dirty + (long)b * k_tiles;
+        v.first = base + at.first + (long)b * q_len;
+        v.behind = base + at.behind + (long)b * q_len;
+        v.start = base[at.start + b];
+        return v;
+    }
+};
+
+inline PlanPtr plan_ptr(const tt_ranges_args& a) {
+    PlanPtr p;
+    p.base = a.plan;
+    tt_key_ranges_layout(a.batch, a.q_len, a.kv_len, &p.at);
+    p.q_len = a.q_len;
+    p.q_tiles = (a.q_len + kTile - 1) / kTile;
+    p.k_tiles = (a.kv_len + kTile - 1) / kTile;
+    return p;
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    const __half2 t = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+template <bool BF16> __device__ __forceinline__ float2 unpack2(uint32_t u) {
+    if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+
+// Instruction descriptor of kind::f16 with fp32 accumulation; both operands bf16 or both fp16.
+template <bool BF16> __host__ __device__ constexpr uint32_t idesc(int m, int n, bool a_mn, bool b_mn) {
+    const uint32_t d = sm100::idesc_bf16(m, n, a_mn, b_mn);
+    return BF16 ? d : d & ~((1u << 7) | (1u << 10));
+}
+
+// The wait of a whole warp: all lanes get the same answer, so that none is left behind at a later warp-wide instruction.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, abort_flag));
+}
+
+// Bits [lo, hi) of a 32-bit word, for any lo and hi.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+    const uint32_t below_hi = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u;
+    const uint32_t below_lo = lo >= 32 ? 0xffffffffu : lo <= 0 ? 0u : (1u << lo) - 1u;
+    return below_hi & ~below_lo;
+}
+
+// Clears the rows of a tile (slabs of [128 rows x 128 bytes], as TMA wrote them) whose bit is set; one warp.
+__device__ __forceinline__ void clear_rows(uint32_t tile, int slabs, uint4 bits, int lane) {
+    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (!(w[q] >> lane & 1u)) continue;
+        for (int s = 0; s < slabs; ++s)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + s * (kTile * 128) + (q * 32 + lane) * 128 + c * 16), "r"(0) : "memory");
+    }
+}
+
+// Score of the log2 domain behind the cap: cap tanh(s / cap) log2(e), from tanh x = 1 - 2 / (1 + e^2x), exact to a few roundings of the cap.
+__device__ __forceinline__ float capped(float s, float two_over_cap_log2e, float cap_log2e, float* t_out) {
+    const float t = 1.f - __fdividef(2.f, 1.f + exp2f(s * two_over_cap_log2e));
+    *t_out = t;
+    return cap_log2e * t;
+}
+
+}  // namespace ranges
+
+// [batch, heads, tokens, head_dim] of 16-bit elements with any strides, box [box_rows, 64], 128-byte swizzle: coordinates (element, token, head, batch)
+int tt_make_tmap_bhsd(CUtensorMap* out, const void* base, int batch, int heads, int tokens, int head_dim, const long* stride, int box_rows);
+// validates what every entry point needs; fills in nothing
+int tt_ranges_check(const tt_ranges_args* a);

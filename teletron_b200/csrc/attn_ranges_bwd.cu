@@ -1,0 +1,700 @@
+// Backward of the attention in which every query sees one run of the keys (attn_ranges_fwd.cu has the formulas).
+//
+//   P = exp(s - lse),  dP = dO V^T,  dS = P (dP - delta),  delta = rowsum(dO O)
+//   dbias[h, d] = sum of dS over the diagonals of distance d;   dS' = dS (1 - tanh^2) behind a cap
+//   dQ = scale dS' K,  dK = scale dS'^T Q,  dV = P^T dO
+//
+// Two kernels without atomics, so that results do not depend on the order of anything: one keeps a tile of 128 keys and goes through the
+// queries that see any of them, of all heads of the group (dK and dV accumulate in TMEM; shared key heads need no second sum), the other keeps a
+// tile of 128 queries and goes through its keys (dQ in TMEM).  Seven products per pair of tiles instead of five.
+//
+// Both are one template: stationary operands A1, A2 (K, V or Q, dO) stay in shared memory, streamed operands B1, B2 (Q, dO or K, V) come through
+// rings.  TMEM: T1 = A1 B1^T (scores), T2 = A2 B2^T (dP; overwritten by P and dS as bf16 / fp16 pairs), accumulators from column 256.  Warp
+// 0 loads, warp 1 issues, sixteen warps turn T1, T2 into P and dS (a thread: one stationary row, 32 streamed ones).
+#include <limits.h>
+
+#include "attn_ranges.cuh"
+
+namespace {
+
+using namespace sm100;
+using namespace ranges;
+
+constexpr int kGroups = 4;                                  // warpgroups that share a chunk's columns
+constexpr int kCols = kTile / kGroups;                      // streamed rows of one thread
+constexpr int kThreads = 64 + kGroups * 128;
+constexpr int kSlab = kTile * 128;
+constexpr int kDiagPad = 256;                               // a tile that is not wholly beyond the largest distance reaches at most 254 past it
+
+enum { kPlain = 0, kGeneral = 1, kGeneralDbias = 2 };
+
+struct BwdParams {
+    PlanPtr plan;
+    const float *lse, *delta, *bias;
+    void *out1, *out2;                  // dQ / dV and dK
+    long s1[3], s2[3];                  // their strides
+    float* partials;
+    int q_len, kv_len, q_heads, group, R;
+    float scale, scale_log2, cap_in, cap_out;
+    int* status;
+};
+
+template <int D, bool KVS, int MODE> struct Layout {
+    static constexpr int kSlabs = D / 64;
+    static constexpr int kTileBytes = kSlabs * kSlab;
+    static constexpr int kRing1 = MODE == kGeneralDbias && D == 128 ? 2 : 3, kRing2 = D == 64 ? 3 : 2;
+    static constexpr int kBars = 1 + 3 * kRing1 + 3 * kRing2 + 6;
+    static constexpr int kFixed = (2 + kRing1 + kRing2) * kTileBytes + (kBars + 1) / 2 * 16;
+    static constexpr int smem(int R) { return kFixed + 1024 + (MODE == kGeneralDbias ? (2 * 16 * 64 + 2 * R + 1 + 2 * kDiagPad) * 4 : 0); }
+};
+
+template <int D, bool BF16, bool KVS, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmDO, const BwdParams p) {
+    using L = Layout<D, KVS, MODE>;
+    constexpr int kTileBytes = L::kTileBytes, kRing1 = L::kRing1, kRing2 = L::kRing2;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ volatile int abort_flag;
+    __shared__ uint32_t tmem_base_slot;
+
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sA1 = base, sA2 = base + kTileBytes;
+    const uint32_t sRing1 = base + 2 * kTileBytes, sRing2 = sRing1 + kRing1 * kTileBytes;
+    const uint32_t bars = sRing2 + kRing2 * kTileBytes;
+    float* scratch = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + L::kFixed);      // [2][16 warps][64]: diagonals of a warp's block
+    float* diag = scratch + 2 * 16 * 64;                                                                // [2 R + 1 + 2 kDiagPad]
+    const uint32_t a_full = bars;
+    auto b1_full = [&](int s) { return bars + 8u * (1 + s); };
+    auto b1_empty = [&](int s) { return bars + 8u * (1 + kRing1 + s); };
+    auto b1_clean = [&](int s) { return bars + 8u * (1 + 2 * kRing1 + s); };
+    auto b2_full = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + s); };
+    auto b2_empty = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + kRing2 + s); };
+    auto b2_clean = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + 2 * kRing2 + s); };
+    const uint32_t s_full = bars + 8u * (1 + 3 * kRing1 + 3 * kRing2);      // T1 holds this chunk's scores
+    const uint32_t dp_full = s_full + 8u;                      // T2 holds this chunk's dP
+    const uint32_t p_ready = s_full + 16u;                     // every softmax warp has read the scores
+    const uint32_t ds_ready = s_full + 24u;                    // P and dS have been written over dP
+    const uint32_t acc_final = s_full + 32u;
+    const uint32_t diag_ready = s_full + 40u;                  // every softmax warp has left its diagonals in the scratch
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int b = blockIdx.z;
+    const PlanView plan = p.plan.sample(b);
+    const int tile = KVS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;         // the longest runs of a causal mask first
+    const int r0 = tile * kTile;
+    const int head0 = KVS ? blockIdx.y * p.group : blockIdx.y, kv_head = KVS ? blockIdx.y : blockIdx.y / p.group;
+    int lo = 0, hi = 0;
+    if (KVS) {
+        const int2 k = plan.k_tiles[tile];
+        lo = k.x;
+        hi = k.y;
+    } else {
+        const int4 r = plan.q_tiles[tile];
+        if (r.x < r.y) {
+            lo = r.x / kTile;
+            hi = (r.y + kTile - 1) / kTile;
+        }
+    }
+    const int per_head = max(hi - lo, 0);
+    const int n_chunks = per_head * (KVS ? p.group : 1);
+    struct Chunk {
+        int head, t;
+    };
+    auto chunk_at = [&](int c) {        // KVS: the queries of head after head
+        if (!KVS) return Chunk{head0, lo + c};
+        const int g = c / per_head;
+        return Chunk{head0 + g, lo + c - g * per_head};
+    };
+    // a streamed tile with rows that no run reaches: queries that see nothing, keys that nothing sees
+    auto is_dirty = [&](int c) { return c < n_chunks ? (KVS ? plan.q_tiles[chunk_at(c).t].w == 0 : plan.dirty[lo + c] != 0) : false; };
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        mbar_init(a_full, 1);
+        for (int s = 0; s < kRing1; ++s) {
+            mbar_init(b1_full(s), 1);
+            mbar_init(b1_empty(s), 1);
+            mbar_init(b1_clean(s), 1);
+        }
+        for (int s = 0; s < kRing2; ++s) {
+            mbar_init(b2_full(s), 1);
+            mbar_init(b2_empty(s), 1);
+            mbar_init(b2_clean(s), 1);
+        }
+        mbar_init(s_full, 1);
+        mbar_init(dp_full, 1);
+        mbar_init(p_ready, 4 * kGroups);
+        mbar_init(ds_ready, 4 * kGroups);
+        mbar_init(acc_final, 1);
+        mbar_init(diag_ready, 4 * kGroups);
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_base_slot), 512);
+        tmem_relinquish();
+    }
+    if (MODE == kGeneralDbias)
+        for (int i = threadIdx.x; i < 2 * p.R + 1 + 2 * kDiagPad; i += kThreads) diag[i] = 0.f;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_slot;
+    constexpr uint32_t kT1 = 0, kT2 = 128, kAcc1 = 256, kAcc2 = 256 + D;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ loads
+        const bool lead = elect_one();
+        if (lead && n_chunks > 0) {
+            mbar_arrive_expect_tx(a_full, 2 * kTileBytes);
+#pragma unroll
+            for (int h = 0; h < L::kSlabs; ++h) {
+                tma_load_4d(sA1 + h * kSlab, KVS ? &tmK : &tmQ, a_full, h * 64, r0, KVS ? kv_head : head0, b);
+                tma_load_4d(sA2 + h * kSlab, KVS ? &tmV : &tmDO, a_full, h * 64, r0, KVS ? kv_head : head0, b);
+            }
+        }
+        bool dirty = is_dirty(0);
+        for (int c = 0; c < n_chunks; ++c) {
+            const int s1 = c % kRing1, s2 = c % kRing2;
+            const uint32_t ph1 = (uint32_t)(c / kRing1) & 1u, ph2 = (uint32_t)(c / kRing2) & 1u;
+            const Chunk ch = chunk_at(c);
+            const int row = ch.t * kTile, head = KVS ? ch.head : kv_head;
+            const bool dirty_next = is_dirty(c + 1);
+            const uint32_t d1 = sRing1 + s1 * kTileBytes, d2 = sRing2 + s2 * kTileBytes;
+            if (!warp_wait(b1_empty(s1), ph1 ^ 1u, &abort_flag)) goto done;
+            if (lead) {
+                mbar_arrive_expect_tx(b1_full(s1), kTileBytes);
+#pragma unroll
+                for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d1 + h * kSlab, KVS ? &tmQ : &tmK, b1_full(s1), h * 64, row, head, b);
+            }
+            if (!warp_wait(b2_empty(s2), ph2 ^ 1u, &abort_flag)) goto done;
+            if (lead) {
+                mbar_arrive_expect_tx(b2_full(s2), kTileBytes);
+#pragma unroll
+                for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d2 + h * kSlab, KVS ? &tmDO : &tmV, b2_full(s2), h * 64, row, head, b);
+            }
+            __syncwarp();
+            if (dirty) {        // their P and dS are 0, and 0 times a NaN is a NaN
+                uint4 bits;
+                if (KVS) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int i = row + q * 32 + lane;
+                        w[q] = __ballot_sync(0xffffffffu, i < p.q_len && plan.first[i] >= plan.behind[i]);
+                    }
+                    bits = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    bits = plan.dead[ch.t];
+                }
+                if (!warp_wait(b1_full(s1), ph1, &abort_flag)) goto done;
+                clear_rows(d1, L::kSlabs, bits, lane);
+                if (KVS) {      // V only meets dS through a selection by the mask
+                    if (!warp_wait(b2_full(s2), ph2, &abort_flag)) goto done;
+                    clear_rows(d2, L::kSlabs, bits, lane);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lead) {
+                    mbar_arrive(b1_clean(s1));
+                    if (KVS) mbar_arrive(b2_clean(s2));
+                }
+            }
+            dirty = dirty_next;
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ products
+        if (elect_one()) {
+            constexpr uint32_t idesc_t = idesc<BF16>(kTile, kTile, false, false);   // T = A B^T, both K-major
+            constexpr uint32_t idesc_a = idesc<BF16>(kTile, D, false, true);        // acc += P B, B MN-major
+            auto issue_t = [&](uint32_t t_col, uint32_t sa, uint32_t sb) {
+                const uint64_t a = fresh_desc(smem_desc_sw128(sa, 16, 1024)), k = fresh_desc(smem_desc_sw128(sb, 16, 1024));
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint64_t off = (uint64_t)(((kk >> 2) * kSlab + (kk & 3) * 32) >> 4);
+                    umma_bf16_ss(tmem + t_col, a + off, k + off, idesc_t, kk ? 1u : 0u);
+                }
+            };
+            // acc[128 x D] += A (pairs in tensor memory, 128 stationary x 128 streamed rows) x chunk (MN-major B)
+            auto issue_acc = [&](uint32_t acc_col, uint32_t a_col, uint32_t sb, bool first) {
+                const uint64_t k = fresh_desc(smem_desc_sw128(sb, kSlab, 1024));
+#pragma unroll
+                for (int kk = 0; kk < kTile / 16; ++kk)
+                    umma_bf16_ts(tmem + acc_col, tmem + a_col + (kk >> 1) * kCols + (kk & 1) * 8, k + (uint64_t)(kk * (2048 >> 4)), idesc_a,
+                                 (first && kk == 0) ? 0u : 1u);
+            };
+            uint32_t cleaned1 = 0, cleaned2 = 0;        // bit s: parity of the cleaned uses of slot s
+            auto wait_b1 = [&](int c, bool dirty) {
+                const int s = c % kRing1;
+                if (!dirty) return mbar_wait(b1_full(s), (uint32_t)(c / kRing1) & 1u, &abort_flag);
+                const uint32_t par = cleaned1 >> s & 1u;
+                cleaned1 ^= 1u << s;
+                return mbar_wait(b1_clean(s), par, &abort_flag);
+            };
+            auto wait_b2 = [&](int c, bool dirty) {
+                const int s = c % kRing2;
+                if (!KVS || !dirty) return mbar_wait(b2_full(s), (uint32_t)(c / kRing2) & 1u, &abort_flag);
+                const uint32_t par = cleaned2 >> s & 1u;
+                cleaned2 ^= 1u << s;
+                return mbar_wait(b2_clean(s), par, &abort_flag);
+            };
+            if (n_chunks > 0) {
+                const bool dirty = is_dirty(0);
+                if (!mbar_wait(a_full, 0, &abort_flag)) goto done;
+                if (!wait_b1(0, dirty)) goto done;
+                tc_fence_after();
+                issue_t(kT1, sA1, sRing1);
+                umma_commit(s_full);
+                if (!wait_b2(0, dirty)) goto done;
+                tc_fence_after();
+                issue_t(kT2, sA2, sRing2);
+                umma_commit(dp_full);
+            }
+            for (int c = 0; c < n_chunks; ++c) {
+                const uint32_t par = (uint32_t)c & 1u;
+                const bool more = c + 1 < n_chunks;
+                const bool dirty_next = is_dirty(c + 1);
+                // T1 is free as soon as every softmax warp has read the scores: the next chunk's overlap the dS pass
+                if (!mbar_wait(p_ready, par, &abort_flag)) goto done;
+                tc_fence_after();
+                if (more) {
+                    if (!wait_b1(c + 1, dirty_next)) goto done;
+                    tc_fence_after();
+                    issue_t(kT1, sA1, sRing1 + (c + 1) % kRing1 * kTileBytes);
+                    umma_commit(s_full);
+                }
+                // T2 now holds P (first 16 columns of every 32) and dS (last 16)
+                if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
+                tc_fence_after();
+                issue_acc(KVS ? kAcc2 : kAcc1, kT2 + 16, sRing1 + c % kRing1 * kTileBytes, c == 0);     // dK += dS^T Q  /  dQ += dS K
+                umma_commit(b1_empty(c % kRing1));
+                if (KVS) issue_acc(kAcc1, kT2, sRing2 + c % kRing2 * kTileBytes, c == 0);               // dV += P^T dO
+                umma_commit(b2_empty(c % kRing2));
+                if (more) {
+                    if (!wait_b2(c + 1, dirty_next)) goto done;
+                    tc_fence_after();
+                    issue_t(kT2, sA2, sRing2 + (c + 1) % kRing2 * kTileBytes);
+                    umma_commit(dp_full);
+                }
+            }
+            umma_commit(acc_final);
+        }
+    } else {
+        // ------------------------------------------------------------ P and dS
+        const int part = (warp - 2) >> 2, quad = warp & 3;
+        const int row = r0 + quad * 32 + lane;                  // key (KVS) or query
+        const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+        const uint32_t t1 = tmem + lane_sel + kT1 + part * kCols, t2 = tmem + lane_sel + kT2 + part * kCols;
+        const int pitch = p.plan.q_tiles * kTile;
+        const int start = plan.start;
+        float my_lse = 0.f, my_delta = 0.f;
+        int first = 0, behind = 0;
+        if (!KVS) {
+            const long at = ((long)b * p.q_heads + head0) * pitch + row;
+            my_lse = p.lse[at];             // +inf behind the last query: its P is 0
+            my_delta = p.delta[at];
+            if (row < p.q_len) {
+                first = plan.first[row];
+                behind = plan.behind[row];
+            }
+        }
+        float far_sum = 0.f, near_sum = 0.f;    // of dS beyond the largest distance: ahead of the query, behind it
+        int n_diag = 0;
+        for (int c = 0; c < n_chunks; ++c) {
+            const uint32_t par = (uint32_t)c & 1u;
+            const Chunk ch = chunk_at(c);
+            const int col0 = ch.t * kTile + part * kCols;         // first streamed row of this thread's 32
+            const float4 *lse4 = nullptr, *delta4 = nullptr;
+            uint32_t see = 0xffffffffu;
+            if (KVS) {
+                const long at = ((long)b * p.q_heads + ch.head) * pitch + col0;
+                lse4 = reinterpret_cast<const float4*>(p.lse + at);
+                delta4 = reinterpret_cast<const float4*>(p.delta + at);
+                const int4 r = plan.q_tiles[ch.t];
+                if (r.z > r0 || r.w < min(r0 + kTile, p.kv_len)) {         // some query does not see all of these keys
+                    const int i = col0 + lane, k0 = r0 + quad * 32;
+                    uint32_t mine = 0u;                                    // keys of this warp that query `lane` sees
+                    if (i < p.q_len) mine = bits_between(plan.first[i] - k0, plan.behind[i] - k0);
+                    see = 0u;
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) see |= (__shfl_sync(0xffffffffu, mine, q) >> lane & 1u) << q;
+                }
+            } else {
+                see = bits_between(first - col0, behind - col0);
+            }
+            const bool clean = __all_sync(0xffffffffu, see == 0xffffffffu);
+            // distance of column i: base + i * step
+            const int pos0 = KVS ? row - (start + col0) : col0 - (start + row);
+            bool at_end = false;
+            float end_bias = 0.f;
+            const float* bias_row = nullptr;
+            if (MODE != kPlain && p.R >= 0) {
+                bias_row = p.bias + (long)ch.head * (2 * p.R + 1) + p.R;
+                const int w0 = __shfl_sync(0xffffffffu, pos0, 0), w31 = __shfl_sync(0xffffffffu, pos0, 31);
+                const int least = KVS ? w0 - 31 : w31, most = KVS ? w31 : w0 + 31;
+                at_end = most <= -p.R || least >= p.R;
+                if (at_end) end_bias = bias_row[least >= p.R ? p.R : -p.R] * kLog2e;
+            }
+            uint32_t pk[16], tk[MODE != kPlain ? 16 : 1];
+            if (!warp_wait(s_full, par, &abort_flag)) goto done;
+            tc_fence_after();
+            {
+                uint32_t a[32];
+                tmem_ld_32x32(t1, a);
+                float4 lq[KVS ? 8 : 1];
+                if (KVS) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) lq[i] = __ldg(lse4 + i);
+                }
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float2 l2;
+                    if (KVS) {
+                        const float4 v = lq[i >> 1];
+                        l2 = (i & 1) ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
+                    } else {
+                        l2 = make_float2(my_lse, my_lse);
+                    }
+                    float2 s2 = make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+                    float2 y;
+                    if (MODE == kPlain) {
+                        y = __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), make_float2(-l2.x, -l2.y));
+                    } else {
+                        if (p.cap_in != 0.f) {
+                            float2 t;
+                            s2 = make_float2(capped(s2.x, p.cap_in, p.cap_out, &t.x), capped(s2.y, p.cap_in, p.cap_out, &t.y));
+                            // the cap's slope in fp16: 2^-12 of a factor that is rounded to 16 bits with its dS below
+                            tk[i] = pack2<false>(1.f - t.x * t.x, 1.f - t.y * t.y);
+                        } else {
+                            s2 = make_float2(s2.x * p.scale_log2, s2.y * p.scale_log2);
+                        }
+                        if (p.R >= 0) {
+                            if (at_end) {
+                                s2 = make_float2(s2.x + end_bias, s2.y + end_bias);
+                            } else {
+                                const int d0 = KVS ? pos0 - 2 * i : pos0 + 2 * i, d1 = KVS ? d0 - 1 : d0 + 1;
+                                s2.x += bias_row[max(-p.R, min(p.R, d0))] * kLog2e;
+                                s2.y += bias_row[max(-p.R, min(p.R, d1))] * kLog2e;
+                            }
+                        }
+                        y = make_float2(s2.x - l2.x, s2.y - l2.y);
+                    }
+                    float2 e = make_float2(exp2f(y.x), exp2f(y.y));
+                    if (!clean) {
+                        if (!(see >> (2 * i) & 1u)) e.x = 0.f;
+                        if (!(see >> (2 * i + 1) & 1u)) e.y = 0.f;
+                    }
+                    if (MODE == kGeneralDbias) {        // dS is summed before it is rounded: P stays in 32 bits
+                        a[2 * i] = __float_as_uint(e.x);
+                        a[2 * i + 1] = __float_as_uint(e.y);
+                    } else {
+                        pk[i] = pack2<BF16>(e.x, e.y);
+                    }
+                }
+                // P stays in registers: T1 is released to the next chunk's scores right away
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready);
+
+                if (!warp_wait(dp_full, par, &abort_flag)) goto done;
+                tc_fence_after();
+                uint32_t g[32];
+                tmem_ld_32x32(t2, g);
+                float4 dq4[KVS ? 8 : 1];
+                if (KVS) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dq4[i] = __ldg(delta4 + i);
+                }
+                tmem_ld_wait();
+                uint32_t dk[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float2 d2;
+                    if (KVS) {
+                        const float4 v = dq4[i >> 1];
+                        d2 = (i & 1) ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
+                    } else {
+                        d2 = make_float2(my_delta, my_delta);
+                    }
+                    const float2 pr = MODE == kGeneralDbias ? make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])) : unpack2<BF16>(pk[i]);
+                    float2 ds = __fmul2_rn(pr, make_float2(__uint_as_float(g[2 * i]) - d2.x, __uint_as_float(g[2 * i + 1]) - d2.y));
+                    if (!clean) {           // dP of a key or a query that no run reaches may be anything
+                        if (!(see >> (2 * i) & 1u)) ds.x = 0.f;
+                        if (!(see >> (2 * i + 1) & 1u)) ds.y = 0.f;
+                    }
+                    if (MODE == kGeneralDbias) {
+                        g[2 * i] = __float_as_uint(ds.x);
+                        g[2 * i + 1] = __float_as_uint(ds.y);
+                    }
+                    if (MODE != kPlain && p.cap_in != 0.f) ds = __fmul2_rn(ds, unpack2<false>(tk[i]));
+                    // rounded to the operands' type, as the products take it: half a step of each dS
+                    dk[i] = pack2<BF16>(ds.x, ds.y);
+                }
+                if (KVS) tmem_st_32x16(t2, pk);
+                tmem_st_32x16(t2 + 16, dk);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_ready);
+
+                if (MODE == kGeneralDbias) {
+                    const int corner = ch.t * kTile - (start + r0);         // distance of the tile's first key from its first query
+                    if (corner + kTile - 1 <= -p.R || corner - kTile + 1 >= p.R) {
+                        float s = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s += __uint_as_float(g[i]);
+                        if (corner < 0) near_sum += s;
+                        else far_sum += s;
+                    } else {
+                        // Sums along the diagonals of the warp's 32 x 32 block: a partial sum moves down one row per column.  Slot
+                        // c - row + 31; what leaves the last row at column c is slot c, what is left at the end belongs to slots 62 - row.
+                        float* slots = scratch + ((n_diag & 1) * 16 + part * 4 + quad) * 64;
+                        float acc = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float above = __shfl_up_sync(0xffffffffu, acc, 1);
+                            acc = (lane == 0 ? 0.f : above) + __uint_as_float(g[i]);
+                            if (lane == 31) slots[i] = acc;
+                        }
+                        if (lane < 31) slots[62 - lane] = acc;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(diag_ready);
+                        if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+                        // one diagonal of the tile a thread, its warps' shares in a fixed order
+                        const int x = (int)threadIdx.x - 64;
+                        if (x < 2 * kTile - 1) {
+                            const int d = x - (kTile - 1);
+                            float s = 0.f;
+                            for (int q = 0; q < 4; ++q)
+                                for (int k = 0; k < 4; ++k) {
+                                    const int slot = d - 32 * (k - q) + 31;
+                                    if (slot >= 0 && slot < 63) s += scratch[((n_diag & 1) * 16 + k * 4 + q) * 64 + slot];
+                                }
+                            diag[kDiagPad + p.R + corner + d] += s;
+                        }
+                        ++n_diag;
+                    }
+                }
+            }
+        }
+        if (MODE == kGeneralDbias) {
+            // the sums beyond the largest distance, warp by warp; then this tile's row of the table
+            for (int o = 16; o > 0; o >>= 1) {
+                near_sum += __shfl_xor_sync(0xffffffffu, near_sum, o);
+                far_sum += __shfl_xor_sync(0xffffffffu, far_sum, o);
+            }
+            float* slots = scratch + (n_diag & 1) * 16 * 64;
+            if (lane == 0) {
+                slots[2 * (part * 4 + quad)] = near_sum;
+                slots[2 * (part * 4 + quad) + 1] = far_sum;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(diag_ready);
+            if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+            float* out = p.partials + (((long)b * p.q_heads + head0) * p.plan.q_tiles + tile) * (2 * p.R + 1);
+            for (int e = (int)threadIdx.x - 64; e < 2 * p.R + 1; e += kThreads - 64) {
+                float s = diag[kDiagPad + e];
+                if (e == 0) {
+                    for (int i = 0; i < kDiagPad; ++i) s += diag[i];
+                    for (int i = 0; i < 16; ++i) s += slots[2 * i];
+                }
+                if (e == 2 * p.R) {
+                    for (int i = 0; i < kDiagPad; ++i) s += diag[kDiagPad + 2 * p.R + 1 + i];
+                    for (int i = 0; i < 16; ++i) s += slots[2 * i + 1];
+                }
+                out[e] = s;
+            }
+        }
+        // ------------------------------------------------------------ gradients
+        if (!warp_wait(acc_final, 0, &abort_flag)) goto done;
+        tc_fence_after();
+        const bool store = row < (KVS ? p.kv_len : p.q_len);
+#pragma unroll 1
+        for (int which = 0; which < (KVS ? 2 : 1); ++which) {
+            const long* st = which == 0 ? p.s1 : p.s2;
+            uint16_t* dst = reinterpret_cast<uint16_t*>(which == 0 ? p.out1 : p.out2) + b * st[0] + (KVS ? kv_head : head0) * st[1] + row * st[2];
+            const float mul = n_chunks == 0 ? 0.f : (KVS && which == 0) ? 1.f : p.scale;         // dV is unscaled
+            const uint32_t tacc = tmem + lane_sel + (which == 0 ? kAcc1 : kAcc2);
+#pragma unroll 1
+            for (int cch = part; cch < D / 32; cch += kGroups) {        // the warpgroups share the accumulator's columns
+                uint32_t r[32];
+                tmem_ld_32x32(tacc + cch * 32, r);
+                tmem_ld_wait();
+                if (!store) continue;
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = n_chunks == 0 ? 0.f : __uint_as_float(r[i]) * mul;
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<uint4*>(dst + cch * 32 + g * 8) =
+                        make_uint4(pack2<BF16>(o[g * 8], o[g * 8 + 1]), pack2<BF16>(o[g * 8 + 2], o[g * 8 + 3]), pack2<BF16>(o[g * 8 + 4], o[g * 8 + 5]),
+                                   pack2<BF16>(o[g * 8 + 6], o[g * 8 + 7]));
+            }
+        }
+    }
+
+done:
+    tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {
+        if (threadIdx.x == 0) atomicExch(p.status, TT_ERR_TIMEOUT);
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);         // copies in flight land
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// delta = rowsum(dO O) in fp32; 0 for queries that see nothing (their dO may be anything) and behind the last.  D / 8 lanes a row.
+template <int D, bool BF16, bool WIDE>
+__global__ void __launch_bounds__(256) ranges_delta_kernel(const PlanPtr plan, const uint16_t* __restrict__ dout, const void* __restrict__ out,
+                                                           float* __restrict__ delta, long rows, int q_len, int q_heads) {
+    constexpr int kLanes = D / 8;
+    const int pitch = plan.q_tiles * kTile, l = threadIdx.x % kLanes;
+    for (long w = ((long)blockIdx.x * 256 + threadIdx.x) / kLanes; w < rows; w += (long)gridDim.x * (256 / kLanes)) {
+        // heads of a query are neighbours in memory: w counts [batch, padded queries, heads]
+        const int h = (int)(w % q_heads);
+        const long bi = w / q_heads;
+        const int i = (int)(bi % pitch);
+        const long b = bi / pitch;
+        float s = 0.f;
+        if (i < q_len && plan.base[plan.at.first + b * q_len + i] < plan.base[plan.at.behind + b * q_len + i]) {
+            const long at = ((b * q_len + i) * q_heads + h) * D + l * 8;
+            const uint4 g = *reinterpret_cast<const uint4*>(dout + at);
+            float2 o[4];
+            if (WIDE) {
+                const float4 u = reinterpret_cast<const float4*>((const float*)out + at)[0], v = reinterpret_cast<const float4*>((const float*)out + at)[1];
+                o[0] = make_float2(u.x, u.y);
+                o[1] = make_float2(u.z, u.w);
+                o[2] = make_float2(v.x, v.y);
+                o[3] = make_float2(v.z, v.w);
+            } else {
+                const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*)out + at);
+                o[0] = unpack2<BF16>(u.x);
+                o[1] = unpack2<BF16>(u.y);
+                o[2] = unpack2<BF16>(u.z);
+                o[3] = unpack2<BF16>(u.w);
+            }
+            const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 d = unpack2<BF16>(gw[e]);
+                s += d.x * o[e].x + d.y * o[e].y;
+            }
+        }
+#pragma unroll
+        for (int m = kLanes / 2; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m, kLanes);
+        if (l == 0) delta[(b * q_heads + h) * pitch + i] = s;
+    }
+}
+
+// dbias[h, e]: the tiles' rows of the table, summed in a fixed order.  32 entries a CTA, 32 threads an entry.
+__global__ void __launch_bounds__(1024) ranges_dbias_kernel(const float* __restrict__ partials, float* __restrict__ dbias, int batch, int q_heads,
+                                                            int q_tiles, int entries) {
+    __shared__ float fold[32][33];
+    const int e = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5, h = blockIdx.y;
+    float s = 0.f;
+    if (e < entries)
+        for (int i = g; i < batch * q_tiles; i += 32) {
+            const int b = i / q_tiles, t = i - b * q_tiles;
+            s += partials[(((long)b * q_heads + h) * q_tiles + t) * entries + e];
+        }
+    fold[g][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (g == 0 && e < entries) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += fold[i][threadIdx.x];
+        dbias[(long)h * entries + e] = s;
+    }
+}
+
+struct Maps {
+    CUtensorMap q, k, v, dout;
+};
+
+template <int D, bool BF16, bool KVS, int MODE>
+int launch(const tt_ranges_args& a, const Maps& m, BwdParams p, int dev, cudaStream_t st) {
+    auto kern = ranges_bwd_kernel<D, BF16, KVS, MODE>;
+    using L = Layout<D, KVS, MODE>;
+    static bool configured[64] = {false};         // per device: the attribute belongs to the device's context
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(TT_RANGES_MAX_DISTANCE));
+        if (e != cudaSuccess) return tt_record_cuda(e);
+        configured[dev] = true;
+    }
+    p.out1 = KVS ? a.dv : a.dq;
+    p.out2 = KVS ? a.dk : nullptr;
+    for (int i = 0; i < 3; ++i) {
+        p.s1[i] = KVS ? a.dv_stride[i] : a.dq_stride[i];
+        p.s2[i] = KVS ? a.dk_stride[i] : 0;
+    }
+    const dim3 grid(KVS ? p.plan.k_tiles : p.plan.q_tiles, KVS ? a.k_heads : a.q_heads, a.batch);
+    kern<<<grid, kThreads, L::smem(a.max_distance), st>>>(m.q, m.k, m.v, m.dout, p);
+    TT_CHECK_LAUNCH();
+    return TT_OK;
+}
+
+template <int D, bool BF16>
+int run(const tt_ranges_args& a, const BwdParams& p, int dev, int sms, cudaStream_t st) {
+    Maps m;
+    int rc;
+    const long dout_stride[3] = {(long)a.q_len * a.q_heads * D, D, (long)a.q_heads * D};
+    if ((rc = tt_make_tmap_bhsd(&m.q, a.q, a.batch, a.q_heads, a.q_len, D, a.q_stride, kTile)) != TT_OK) return rc;
+    if ((rc = tt_make_tmap_bhsd(&m.k, a.k, a.batch, a.k_heads, a.kv_len, D, a.k_stride, kTile)) != TT_OK) return rc;
+    if ((rc = tt_make_tmap_bhsd(&m.v, a.v, a.batch, a.k_heads, a.kv_len, D, a.v_stride, kTile)) != TT_OK) return rc;
+    if ((rc = tt_make_tmap_bhsd(&m.dout, a.dout, a.batch, a.q_heads, a.q_len, D, dout_stride, kTile)) != TT_OK) return rc;
+    const long rows = (long)a.batch * a.q_heads * p.plan.q_tiles * kTile, want = (rows * (D / 8) + 255) / 256;
+    const int grid = (int)(want < sms * 16L ? want : sms * 16L);
+    if (a.out32 != nullptr)
+        ranges_delta_kernel<D, BF16, true><<<grid, 256, 0, st>>>(p.plan, (const uint16_t*)a.dout, a.out32, a.delta, rows, a.q_len, a.q_heads);
+    else
+        ranges_delta_kernel<D, BF16, false><<<grid, 256, 0, st>>>(p.plan, (const uint16_t*)a.dout, a.out, a.delta, rows, a.q_len, a.q_heads);
+    TT_CHECK_LAUNCH();
+    const bool gen = a.softcap > 0.f || a.max_distance >= 0;
+    rc = gen ? launch<D, BF16, true, kGeneral>(a, m, p, dev, st) : launch<D, BF16, true, kPlain>(a, m, p, dev, st);
+    if (rc != TT_OK) return rc;
+    if (a.dbias == nullptr) return gen ? launch<D, BF16, false, kGeneral>(a, m, p, dev, st) : launch<D, BF16, false, kPlain>(a, m, p, dev, st);
+    if ((rc = launch<D, BF16, false, kGeneralDbias>(a, m, p, dev, st)) != TT_OK) return rc;
+    const int entries = 2 * a.max_distance + 1;
+    ranges_dbias_kernel<<<dim3((entries + 31) / 32, a.q_heads), 1024, 0, st>>>(a.partials, a.dbias, a.batch, a.q_heads, p.plan.q_tiles, entries);
+    TT_CHECK_LAUNCH();
+    return TT_OK;
+}
+
+}  // namespace
+
+extern "C" int tt_attn_ranges_bwd(const tt_ranges_args* a, void* stream) {
+    int rc = tt_ranges_check(a);
+    if (rc != TT_OK) return rc;
+    if (a->dout == nullptr || a->delta == nullptr || a->dq == nullptr || a->dk == nullptr || a->dv == nullptr) return TT_ERR_ARG;
+    for (const void* x : {a->dout, (const void*)a->lse, (const void*)a->delta, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+        if ((uintptr_t)x & 15) return TT_ERR_ARG;
+    for (const long* s : {a->dq_stride, a->dk_stride, a->dv_stride})
+        if (s[0] % 8 || s[1] % 8 || s[2] % 8) return TT_ERR_ARG;
+    if (a->dbias != nullptr && (a->partials == nullptr || a->max_distance < 0)) return TT_ERR_ARG;
+    const tt_device_info dev = tt_device();
+    BwdParams p;
+    p.plan = plan_ptr(*a);
+    p.lse = a->lse;
+    p.delta = a->delta;
+    p.bias = a->bias;
+    p.partials = a->partials;
+    p.q_len = a->q_len;
+    p.kv_len = a->kv_len;
+    p.q_heads = a->q_heads;
+    p.group = a->q_heads / a->k_heads;
+    p.R = a->max_distance;
+    p.scale = a->scale;
+    p.scale_log2 = a->scale * kLog2e;
+    p.cap_in = a->softcap > 0.f ? 2.f * a->scale / a->softcap * kLog2e : 0.f;
+    p.cap_out = a->softcap * kLog2e;
+    p.status = a->status;
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool bf = a->dtype == TT_BF16;
+    if (a->head_dim == 128) return bf ? run<128, true>(*a, p, dev.dev, dev.sms, st) : run<128, false>(*a, p, dev.dev, dev.sms, st);
+    return bf ? run<64, true>(*a, p, dev.dev, dev.sms, st) : run<64, false>(*a, p, dev.dev, dev.sms, st);
+}

@@ -161,6 +161,47 @@ int tt_attn_bwd_fused(const void* q, const void* k, const void* v, const void* o
 /* the kernel that route 0 takes on a device of `sms` SMs (1: CTA pairs); touches no device */
 int tt_attn_bwd_uses_pairs(int heads, int S, int sms);
 
+/* ---- attention in which every query sees one run of the keys (attn_ranges*.cu) ---- */
+#define TT_RANGES_TILE 128          /* rows of a tile of queries and of a tile of keys */
+#define TT_RANGES_MAX_DISTANCE 1024
+/* Offsets, in ints, of the parts of a plan for `batch` samples; the whole takes tt_key_ranges_ints. */
+typedef struct {
+    long q_tiles;       /* [batch, tiles of queries, 4]: first key any of them sees, behind the last, first key all see, behind the last */
+    long dead;          /* [batch, tiles of keys, 4]: bit j: key j of the tile is seen by no query */
+    long k_tiles;       /* [batch, tiles of keys, 2]: first tile of queries that sees any of them, behind the last */
+    long dirty;         /* [batch, tiles of keys]: dead has a bit set */
+    long first, behind; /* [batch, queries]: the keys that a query sees; 0, 0 where there is none */
+    long start;         /* [batch]: position of the first query */
+    long ints;
+} tt_ranges_layout;
+void tt_key_ranges_layout(int batch, int q_len, int kv_len, tt_ranges_layout* out);
+/* documents: offsets [batch or 1, n + 1] (document_stride 0: shared) or null; prefix: [batch or 1, n or 1] or null (then prefix_len
+ * holds for all); kv_valid_len, query_start: [batch] or null */
+int tt_key_ranges(int* plan, int batch, int q_len, int kv_len, int causal, const int* documents, int n_documents, long document_stride,
+                  const int* prefix, long prefix_stride, int prefix_per_document, int prefix_len, const int* kv_valid_len, const int* query_start,
+                  void* stream);
+typedef struct {
+    long struct_size;                   /* sizeof(tt_ranges_args) */
+    int batch, q_heads, k_heads, q_len, kv_len, head_dim, dtype, max_distance;      /* max_distance -1: no bias */
+    const void *q, *k, *v;              /* [batch, heads, tokens, head_dim], strides {batch, head, token} in elements, multiples of 8 */
+    long q_stride[3], k_stride[3], v_stride[3];
+    void* out;                          /* [batch, q_len, q_heads * head_dim] */
+    float* out32;                       /* the same before rounding, or null */
+    float* lse;                         /* [batch, q_heads, q_len rounded up to 128], log2 of the sums; +inf where a query sees nothing */
+    const int* plan;                    /* tt_key_ranges */
+    const float* bias;                  /* [q_heads, 2 * max_distance + 1] */
+    float scale, softcap;               /* softcap 0: none */
+    const void* dout;                   /* backward: [batch, q_len, q_heads * head_dim] */
+    float* delta;                       /* scratch like lse */
+    void *dq, *dk, *dv;
+    long dq_stride[3], dk_stride[3], dv_stride[3];
+    float* dbias;                       /* [q_heads, 2 * max_distance + 1] or null */
+    float* partials;                    /* scratch [batch, q_heads, tiles of queries, 2 * max_distance + 1] where dbias is wanted */
+    int* status;
+} tt_ranges_args;
+int tt_attn_ranges_fwd(const tt_ranges_args* args, void* stream);
+int tt_attn_ranges_bwd(const tt_ranges_args* args, void* stream);
+
 /* ---- symmetric heap + in-kernel collectives over IPC-mapped peer memory (comm.cu) ---- */
 int tt_symm_alloc(size_t bytes, void** out);                 /* cudaMalloc + zero */
 int tt_symm_free(void* p);

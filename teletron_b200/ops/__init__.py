@@ -22,6 +22,7 @@ import torch
 
 from . import reference
 from . import optim  # noqa: F401
+from .attn_ranges import KeyRanges, key_ranges  # noqa: F401
 from .rope import Rotary, rotary_frequencies  # noqa: F401
 
 _IMPL = os.environ.get("TELETRON_B200_IMPL", "auto")
@@ -182,6 +183,26 @@ def attention(q, k, v, kv_valid_len=None, scale=None, mask_range=None):
         from . import cuda_ops
         return cuda_ops.attention(q, k, v, kv_valid_len, scale, mask_range)
     return reference.attention(q, k, v, kv_valid_len, scale, mask_range)
+
+
+def masked_attention(q, k, v, ranges, scale=None, softcap=None, distance_bias=None):
+    """Softmax attention in which every query sees one run of the keys: causal, prefix and document masks, padded batches, caches.
+
+    ``q [batch, heads, queries, head_dim]``, ``k``, ``v`` ``[batch, key heads, keys, head_dim]`` (any strides; the heads are a multiple of the key
+    heads); ``ranges``: what :func:`key_ranges` returns.  ``scale`` defaults to ``head_dim ** -0.5``; ``softcap`` caps the scaled scores as
+    ``softcap * tanh(s / softcap)``; ``distance_bias [heads, 2 R + 1]`` (fp32) is added for the distance key position - query position, distances
+    beyond R taking the ends' values.  Returns token-major ``[batch, queries, heads * head_dim]``, 0 for queries that see nothing.
+
+    Keys, values, queries and output gradients that no run reaches (padding) may hold anything; those that some query sees have to be finite,
+    as a query's weights of 0 still multiply what its neighbours see.  Kernels: bf16 and fp16, head_dim 64 and 128, R up to 1024."""
+    from . import attn_ranges
+    attn_ranges.check_arguments(q, k, v, ranges, scale, softcap, distance_bias)
+    if _use_cuda(q, dtypes=(torch.bfloat16, torch.float16)):
+        if attn_ranges.supported(q, k, v, ranges, distance_bias):
+            return attn_ranges.masked_attention(q, k, v, ranges, scale, softcap, distance_bias)
+        from . import fallback
+        fallback.note("masked_attention", f"q {tuple(q.shape)} {q.dtype}")
+    return reference.masked_attention(q, k, v, ranges, scale, softcap, distance_bias)
 
 
 def qkv_projection(x, weight, bias, q_norm_weight, k_norm_weight, cos, sin, num_heads,

@@ -62,7 +62,7 @@ def _load() -> Optional[ctypes.CDLL]:
         getattr(lib, name).argtypes = [vp] * 5 + [ci] * 3 + [cl] * 3 + [ci] * 3 + [vp] * 2
     lib.tt_gemm2_bf16_splitk.argtypes = [vp] * 5 + [ci] * 3 + [cl] * 3 + [ci] * 4 + [vp] * 3
     lib.tt_rotary_partial_floats.restype = cl
-    for name in ("tt_rotary", "tt_norm_rotary_fwd", "tt_norm_rotary_bwd"):
+    for name in ("tt_rotary", "tt_norm_rotary_fwd", "tt_norm_rotary_bwd", "tt_attn_ranges_fwd", "tt_attn_ranges_bwd"):
         getattr(lib, name).argtypes = [ctypes.c_char_p, vp]
     lib.tt_rotary_partial_floats.argtypes = [ctypes.c_char_p]
     lib.tt_gemm2_bf16_two.argtypes = [vp] * 5 + [ci] * 4 + [cl] * 4 + [ci] + [vp] * 3
@@ -132,7 +132,7 @@ def check(t: torch.Tensor, dtype: torch.dtype, name: str, device: Optional[torch
 
 
 # kernels launched per native call (for the launch counter the benchmark reports)
-KERNELS_PER_CALL = {"tt_ln_mod_bwd": 2, "tt_adaln_bwd": 2, "tt_gemm2_bf16_splitk": 2, "tt_gate_residual_bwd": 2, "tt_rmsnorm_bwd": 2, "tt_qkv_post_bwd": 2, "tt_norm_rotary_bwd": 2, "tt_attn_bwd": 3, "tt_attn_bwd_fused": 3}
+KERNELS_PER_CALL = {"tt_ln_mod_bwd": 2, "tt_adaln_bwd": 2, "tt_gemm2_bf16_splitk": 2, "tt_gate_residual_bwd": 2, "tt_rmsnorm_bwd": 2, "tt_qkv_post_bwd": 2, "tt_norm_rotary_bwd": 2, "tt_key_ranges": 2, "tt_attn_ranges_bwd": 3, "tt_attn_bwd": 3, "tt_attn_bwd_fused": 3}
 LAUNCHES = 0
 
 

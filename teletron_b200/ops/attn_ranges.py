@@ -1,0 +1,271 @@
+"""Attention in which every query sees one run of the keys (``csrc/attn_ranges_*.cu``).
+
+Causal, prefix and document masks, padded batches and caches in use up to a length all let a query see one run of keys.  A
+:class:`KeyRanges` holds the runs and what the kernels need to skip and to mask by tiles; it is made once for a batch and shared by its
+layers.  The reference passes no mask to its attention at all (``teletron/models/dit/dit_attention.py:311-313``) and leaves
+the text encoders' masks and biases to their package (``teletron/models/hunyuanvideo/text_encoder.py``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+import math
+import struct
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import c_int, c_long, call, on_device, ptr, stream
+from .gemm_tcgen05 import status_tensor
+
+TILE = 128
+MAX_DISTANCE = 1024
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+@dataclasses.dataclass(frozen=True, eq=False)
+class KeyRanges:
+    """Runs of keys ``[first, behind)`` that the queries of a batch see (int32 ``[batch, q_len]`` both; 0, 0: none).
+
+    Made by :func:`key_ranges`; its tensors are not to be written to."""
+    batch: int
+    q_len: int
+    kv_len: int
+    first: torch.Tensor
+    behind: torch.Tensor
+    query_start: Optional[torch.Tensor]
+    plan: Optional[torch.Tensor]
+
+    @property
+    def device(self):
+        return self.first.device
+
+
+def _lengths(value, name: str, batch: int, device, per_document: Optional[int] = None):
+    """An int, or per-sample integers, as ``(int or None, int32 tensor or None)``."""
+    if value is None or isinstance(value, int):
+        return value, None
+    t = value if isinstance(value, torch.Tensor) else torch.tensor(value)
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: expected integers, got {t.dtype}")
+    shapes = [(batch,)] + ([(batch, per_document)] if per_document is not None else [])
+    if tuple(t.shape) not in shapes:
+        raise ValueError(f"{name}: expected an int or one of the shapes {shapes}, got {tuple(t.shape)}")
+    return None, t.to(device=device, dtype=torch.int32).contiguous()
+
+
+def _runs(q_len, kv_len, batch, causal, documents, prefix_len, prefix, kv_valid_len, query_start, device):
+    """The runs in torch operations: the definition, and the path without the native library's device."""
+    i = torch.arange(q_len, device=device).expand(batch, q_len)
+    at = i if query_start is None else i + query_start.long()[:, None]
+    lo, hi, start, doc = torch.zeros_like(i), torch.full_like(i, kv_len), torch.zeros_like(i), None
+    if kv_valid_len is not None:
+        hi = torch.minimum(hi, kv_valid_len.long()[:, None].expand_as(hi))
+    if documents is not None:
+        off = documents.long().expand(batch, -1).contiguous()
+        n = off.shape[1] - 1
+        place = torch.searchsorted(off, i.contiguous(), right=True)
+        inside = (place > 0) & (place <= n)
+        doc = (place - 1).clamp(0, n - 1)
+        start = off.gather(1, doc).clamp_min(0)
+        lo = start
+        hi = torch.where(inside, torch.minimum(hi, off.gather(1, doc + 1)), torch.zeros_like(hi))
+    if causal:
+        p = prefix_len or 0
+        if prefix is not None:
+            p = prefix.long()[:, None] if prefix.dim() == 1 else prefix.long().gather(1, doc)
+            p = p.clamp_min(0)
+        hi = torch.minimum(hi, torch.maximum(at + 1, start + p))
+    none = lo >= hi
+    return lo.masked_fill(none, 0).to(torch.int32), hi.masked_fill(none, 0).to(torch.int32)
+
+
+def key_ranges(q_len: int, kv_len: Optional[int] = None, *, batch: int = 1, causal: bool = False, documents=None, prefix_len=None,
+               kv_valid_len=None, query_start=None, device=None) -> KeyRanges:
+    """The runs of keys that ``q_len`` queries of ``batch`` samples see among ``kv_len`` keys (default: as many as queries).
+
+    * ``causal``: a query sees keys up to its own position, ``query_start`` (int or ``[batch]``, default 0) plus its index.
+    * ``documents``: offsets of documents that are packed one after another, integers ``[n + 1]`` or ``[batch, n + 1]`` that do not
+      decrease; a query sees its own document only, and nothing behind the last or ahead of the first.  A batch padded to the right is one
+      document per sample, ``[[0, length], ...]``.  Needs ``q_len == kv_len`` and no ``query_start``.
+    * ``prefix_len`` (int, ``[batch]`` or, with documents, ``[batch, n]``): that many first keys of the sample, or of each document, are
+      seen by all of its queries.  Needs ``causal``.
+    * ``kv_valid_len`` (int or ``[batch]``): keys from there on are seen by nobody (a cache that is not full).
+
+    With ``causal`` and another number of keys than queries the positions have to be said, by ``query_start``."""
+    q_len, kv_len, batch = int(q_len), int(q_len if kv_len is None else kv_len), int(batch)
+    if q_len < 0 or kv_len < 0 or batch < 0:
+        raise ValueError(f"key_ranges: negative sizes ({q_len} queries, {kv_len} keys, {batch} samples)")
+    for v in (documents, prefix_len, kv_valid_len, query_start):
+        if device is None and isinstance(v, torch.Tensor):
+            device = v.device
+    device = torch.device("cpu" if device is None else device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    if prefix_len is not None and not causal:
+        raise ValueError("key_ranges: a prefix needs causal=True")
+    if causal and q_len != kv_len and query_start is None:
+        raise ValueError(f"key_ranges: {q_len} queries and {kv_len} keys: causal runs need query_start")
+    n = None
+    if documents is not None:
+        if q_len != kv_len or query_start is not None:
+            raise ValueError("key_ranges: documents need as many queries as keys and no query_start")
+        documents = documents if isinstance(documents, torch.Tensor) else torch.tensor(documents)
+        if documents.dtype not in (torch.int32, torch.int64) or documents.dim() not in (1, 2) or documents.shape[-1] < 2 \
+                or (documents.dim() == 2 and documents.shape[0] != batch):
+            raise ValueError(f"documents: expected integer offsets [n + 1] or [{batch}, n + 1], got {documents.dtype} {tuple(documents.shape)}")
+        documents = documents.to(device=device, dtype=torch.int32).contiguous()
+        documents = documents[None] if documents.dim() == 1 else documents
+        n = documents.shape[1] - 1
+    prefix_len, prefix = _lengths(prefix_len, "prefix_len", batch, device, n)
+    kv_valid_int, kv_valid = _lengths(kv_valid_len, "kv_valid_len", batch, device)
+    start_int, start = _lengths(query_start, "query_start", batch, device)
+    if prefix_len is not None and prefix_len < 0:
+        raise ValueError(f"prefix_len: {prefix_len} is negative")
+    if kv_valid_int is not None:
+        kv_valid = torch.full((batch,), min(max(kv_valid_int, 0), kv_len), dtype=torch.int32, device=device)
+    if start_int:
+        start = torch.full((batch,), start_int, dtype=torch.int32, device=device)
+    if device.type != "cuda" or not _lib.available() or min(q_len, kv_len, batch) == 0:
+        first, behind = _runs(q_len, kv_len, batch, causal, documents, prefix_len, prefix, kv_valid, start, device)
+        return KeyRanges(batch, q_len, kv_len, first, behind, start, None)
+    at = _layout(batch, q_len, kv_len)
+    with torch.cuda.device(device):
+        plan = torch.empty(at.ints, dtype=torch.int32, device=device)
+        call("tt_key_ranges", ptr(plan), c_int(batch), c_int(q_len), c_int(kv_len), c_int(causal), ptr(documents), c_int(n or 0),
+             c_long(0 if documents is None or documents.shape[0] == 1 else documents.shape[1]), ptr(prefix),
+             c_long(0 if prefix is None else prefix.stride(0)), c_int(prefix is not None and prefix.dim() == 2), c_int(prefix_len or 0),
+             ptr(kv_valid), ptr(start), stream())
+    rows = batch * q_len
+    return KeyRanges(batch, q_len, kv_len, plan[at.first:at.first + rows].view(batch, q_len), plan[at.behind:at.behind + rows].view(batch, q_len),
+                     start, plan)
+
+
+class _Layout(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_long) for n in ("q_tiles", "dead", "k_tiles", "dirty", "first", "behind", "start", "ints")]
+
+
+def _layout(batch, q_len, kv_len):
+    at = _Layout()
+    _lib.lib().tt_key_ranges_layout(c_int(batch), c_int(q_len), c_int(kv_len), ctypes.byref(at))
+    return at
+
+
+def check_arguments(q, k, v, ranges, scale, softcap, distance_bias) -> None:
+    """Raises ``ValueError`` where the operands do not belong together."""
+    if not isinstance(ranges, KeyRanges):
+        raise ValueError("masked_attention: expected the runs that key_ranges returns")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"expected [batch, heads, tokens, head_dim], got q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    B, hq, n, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.shape[1] == 0 or hq % k.shape[1]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if not q.dtype.is_floating_point or k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError(f"q {q.dtype} on {q.device}, k {k.dtype} on {k.device}, v {v.dtype} on {v.device} do not belong together")
+    if (ranges.batch, ranges.q_len, ranges.kv_len) != (B, n, k.shape[2]):
+        raise ValueError(f"runs of {ranges.batch} x {ranges.q_len} queries and {ranges.kv_len} keys for {B} x {n} queries and {k.shape[2]} keys")
+    if ranges.device != q.device:
+        raise ValueError(f"runs on {ranges.device}, queries on {q.device}")
+    if scale is not None and not math.isfinite(scale):
+        raise ValueError(f"scale: {scale} is not finite")
+    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+        raise ValueError(f"softcap: expected a positive number or None, got {softcap}")
+    if distance_bias is not None:
+        if distance_bias.dim() != 2 or distance_bias.shape[0] != hq or distance_bias.shape[1] % 2 == 0:
+            raise ValueError(f"distance_bias: expected [{hq}, 2 R + 1], got {tuple(distance_bias.shape)}")
+        if distance_bias.dtype != torch.float32 or distance_bias.device != q.device:
+            raise ValueError(f"distance_bias: expected float32 on {q.device}, got {distance_bias.dtype} on {distance_bias.device}")
+
+
+def supported(q, k, v, ranges, distance_bias) -> bool:
+    return (_lib.available() and q.is_cuda and q.dtype in _DTYPES and q.shape[3] in (64, 128) and ranges.plan is not None
+            and q.numel() > 0 and k.numel() > 0 and q.shape[0] <= 65535 and q.shape[1] <= 65535
+            and (distance_bias is None or distance_bias.shape[1] <= 2 * MAX_DISTANCE + 1))
+
+
+# ------------------------------------------------------------------------------------------------ native calls
+
+_ARGS = struct.Struct("@l iiii iiii PPP 9l PPP PP ff PP PPP 9l PP P")
+_NONE9 = (0,) * 9
+
+
+def _rows(t):
+    """Operand that the copies can address: contiguous rows at 16-byte boundaries, steps of any size above 0."""
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _like(x):
+    """A gradient in ``x``'s order of heads and tokens."""
+    B, H, S, D = x.shape
+    if x.stride(1) < x.stride(2):
+        return torch.empty(B, S, H, D, dtype=x.dtype, device=x.device).transpose(1, 2)
+    return torch.empty(B, H, S, D, dtype=x.dtype, device=x.device)
+
+
+def _native(fn, q, k, v, ranges, out, out32, lse, scale, softcap, bias, grads=None):
+    """``grads``: ``(dout, delta, dq, dk, dv, dbias, partials)``."""
+    B, hq, n, D = q.shape
+    dout, delta, dq, dk, dv, dbias, partials = grads or (None,) * 7
+    address = lambda t: 0 if t is None else t.data_ptr()
+    packed = _ARGS.pack(_ARGS.size, B, hq, k.shape[1], n, k.shape[2], D, _DTYPES[q.dtype], -1 if bias is None else (bias.shape[1] - 1) // 2,
+                        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                        out.data_ptr(), address(out32), lse.data_ptr(), ranges.plan.data_ptr(), address(bias),
+                        scale, softcap, address(dout), address(delta), address(dq), address(dk), address(dv),
+                        *(_NONE9 if grads is None else (*dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3])),
+                        address(dbias), address(partials), status_tensor(q.device).data_ptr())
+    call(fn, packed, stream())
+
+
+def _forward(q, k, v, ranges, scale, softcap, bias, wide):
+    B, hq, n, D = q.shape
+    out = torch.empty(B, n, hq * D, dtype=q.dtype, device=q.device)
+    out32 = torch.empty(B, n, hq * D, dtype=torch.float32, device=q.device) if wide else None
+    lse = torch.empty(B, hq, (n + TILE - 1) // TILE * TILE, dtype=torch.float32, device=q.device)
+    _native("tt_attn_ranges_fwd", q, k, v, ranges, out, out32, lse, scale, softcap, bias)
+    return out, out32, lse
+
+
+class _MaskedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, ranges, scale, softcap):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        bias = None if bias is None else bias.contiguous()
+        # a bias that is trained needs the output before rounding, to more than P's 16 bits (4 bytes an element, kept for the backward)
+        wide = bias is not None and ctx.needs_input_grad[3]
+        out, out32, lse = _forward(q, k, v, ranges, scale, softcap, bias, wide)
+        ctx.save_for_backward(q, k, v, bias, out32 if wide else out, lse, ranges.plan)
+        ctx.ranges, ctx.scale, ctx.softcap, ctx.wide = ranges, scale, softcap, wide
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, bias, out, lse, _ = ctx.saved_tensors
+        B, hq, n, D = q.shape
+        with on_device(q):
+            dout = dout.contiguous()
+            if dout.data_ptr() % 16:
+                dout = dout.clone()
+            dq, dk, dv = _like(q), _like(k), _like(v)
+            dbias = partials = None
+            if ctx.wide:
+                dbias = torch.empty_like(bias)
+                partials = torch.empty(B * hq * (lse.shape[2] // TILE) * bias.shape[1], dtype=torch.float32, device=q.device)
+            _native("tt_attn_ranges_bwd", q, k, v, ctx.ranges, out, out if ctx.wide else None, lse, ctx.scale, ctx.softcap, bias,
+                    (dout, torch.empty_like(lse), dq, dk, dv, dbias, partials))
+        return tuple(t if need else None for t, need in zip((dq, dk, dv, dbias), ctx.needs_input_grad)) + (None, None, None)
+
+
+def masked_attention(q, k, v, ranges, scale, softcap, distance_bias):
+    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    softcap = 0.0 if softcap is None else float(softcap)
+    with on_device(q):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, distance_bias)):
+            return _MaskedAttention.apply(q, k, v, distance_bias, ranges, scale, softcap)
+        bias = None if distance_bias is None else distance_bias.contiguous()
+        return _forward(_rows(q), _rows(k), _rows(v), ranges, scale, softcap, bias, False)[0]

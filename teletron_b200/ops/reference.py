@@ -150,6 +150,34 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return o.transpose(1, 2).reshape(B, S, h * D)
 
 
+def masked_attention(q, k, v, ranges, scale: Optional[float] = None, softcap: Optional[float] = None, distance_bias=None) -> torch.Tensor:
+    """Softmax attention in which query ``i`` sees the keys ``[first, behind)`` of ``ranges`` (:class:`teletron_b200.ops.KeyRanges`), from
+    plain products in 32 bits (or the wider type of ``q``).  Queries that see nothing get 0."""
+    B, h, S, D = q.shape
+    n, group = k.shape[2], h // k.shape[1]
+    calc = torch.promote_types(q.dtype, torch.float32)
+    kf, vf = (t.to(calc).repeat_interleave(group, dim=1) for t in (k, v))
+    s = (q.to(calc) @ kf.transpose(-1, -2)) * (D ** -0.5 if scale is None else scale)
+    if softcap is not None:
+        s = softcap * torch.tanh(s / softcap)
+    j = torch.arange(n, device=q.device)
+    if distance_bias is not None:
+        R = (distance_bias.shape[1] - 1) // 2
+        i = torch.arange(S, device=q.device)[None] + (0 if ranges.query_start is None else ranges.query_start.long()[:, None])
+        far = (j - i[..., None]).clamp(-R, R) + R                                      # [1 or B, S, n]
+        s = s + distance_bias.to(calc)[:, far].transpose(0, 1)
+    see = (j >= ranges.first[..., None]) & (j < ranges.behind[..., None])              # [B, S, n]
+    s = s.masked_fill(~see[:, None], float("-inf"))
+    top = s.amax(dim=-1, keepdim=True).detach() if n else s.new_zeros(B, h, S, 1)
+    p = torch.exp(s - top.masked_fill(top == float("-inf"), 0.0))
+    total = p.sum(dim=-1, keepdim=True)
+    p = p / total.masked_fill(total == 0, 1.0)
+    # values that no query sees may hold anything: 0 times a NaN is a NaN
+    used = see.any(dim=1)[:, None, :, None]
+    o = p @ vf.masked_fill(~used, 0.0)
+    return o.to(q.dtype).transpose(1, 2).reshape(B, S, h * D)
+
+
 def qkv_projection(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
                    q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor,
                    cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
