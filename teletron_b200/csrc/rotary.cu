@@ -8,9 +8,10 @@
 // dw = sum over rows of g' x^, dx = r (g' w - x^ mean(g' w x^)).
 //
 // No table is read: the angle of a (token, pair) is shared by all heads, so a warp forms it once per token, in 64 bits (a
-// position of 10^5 times a frequency near 1 leaves 2^-7 of a turn's fraction in 32 bits), reduced to a part of a turn, and keeps cos and sin
-// in registers over the token's heads.  The kernels are bound by memory: 2 passes over q and k forward, 3 for the norm's backward.
+// position of 10^5 times a frequency near 1 leaves 2^-7 of a turn's fraction in 32 bits), reduced to a part of a turn and spread over
+// the lanes while the first heads' elements are being loaded.  The kernels are bound by memory: 2 passes over q and k forward, 3 for the norm's backward.
 #include <cuda_fp16.h>
+#include <limits.h>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -45,223 +46,354 @@ template <typename T, int V> struct Pack {
     __device__ __forceinline__ Pack() : raw() {}
     __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const R*>(p); }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<R*>(p) = raw; }
-    __device__ __forceinline__ void get(float* f) const {
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = to_f(v[i]);
-    }
-    __device__ __forceinline__ void set(const float* f) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = from_f<T>(f[i]);
-    }
 };
 
-// A lane's share of a head: NV chunks of V pairs, each as two vectors of V elements at off0 and off1.
+// Packed arithmetic on neighbours of an array: half the instructions, which are what the kernels spend next to their loads.
+template <int V, typename F2, typename F1> __device__ __forceinline__ void pairwise(F2&& two, F1&& one) {
+    if (V % 2 == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) two(e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) one(e);
+    }
+}
+__device__ __forceinline__ float2 at2(const float* f, int e) { return make_float2(f[e], f[e + 1]); }
+__device__ __forceinline__ void put2(float* f, int e, float2 v) {
+    f[e] = v.x;
+    f[e + 1] = v.y;
+}
+// x *= y;  x += y z
+template <int V> __device__ __forceinline__ void mul(float* x, const float* y) {
+    pairwise<V>([&](int e) { put2(x, e, __fmul2_rn(at2(x, e), at2(y, e))); }, [&](int e) { x[e] *= y[e]; });
+}
+template <int V> __device__ __forceinline__ void scale(float* x, float y) {
+    pairwise<V>([&](int e) { put2(x, e, __fmul2_rn(at2(x, e), make_float2(y, y))); }, [&](int e) { x[e] *= y; });
+}
+template <int V> __device__ __forceinline__ void add_product(float* x, const float* y, const float* z) {
+    pairwise<V>([&](int e) { put2(x, e, __ffma2_rn(at2(y, e), at2(z, e), at2(x, e))); }, [&](int e) { x[e] += y[e] * z[e]; });
+}
+
+// A lane's share of a head: NV chunks of V pairs, each as two vectors of V elements at off0 and off1.  In the half layout the vectors hold the
+// pairs' first and second elements; in the interleaved one V / 2 whole pairs each, and full-width vectors lie one lane apart, so that a
+// group of lanes reads neighbouring addresses.  Chunks behind the rotated elements pass.
 template <int V, int NV, bool INTER> struct Geometry {
+    static constexpr bool kWhole = INTER && V > 1;         // vectors of whole pairs
     int off0[NV], off1[NV];
-    bool in0[NV], in1[NV], rot0[NV], rot1[NV];
-    __device__ __forceinline__ Geometry(int l, int log_l, int D, int P) {
+    __device__ __forceinline__ Geometry(int l, int log_l, int P) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = l + (i << log_l);
-            if (INTER && V > 1) {
-                off0[i] = c * 2 * V;
-                off1[i] = off0[i] + V;
-                rot0[i] = off0[i] < 2 * P;
-                rot1[i] = off1[i] < 2 * P;
+            if (kWhole) {
+                off0[i] = NV == 1 ? c * V : c * 2 * V;
+                off1[i] = NV == 1 ? off0[i] + (V << log_l) : off0[i] + V;
             } else if (c * V < P) {
                 off0[i] = INTER ? 2 * c : c * V;
                 off1[i] = INTER ? 2 * c + 1 : P + c * V;
-                rot0[i] = rot1[i] = true;
             } else {
                 off0[i] = 2 * P + (c - P / V) * 2 * V;
                 off1[i] = off0[i] + V;
-                rot0[i] = rot1[i] = false;
             }
-            in0[i] = off0[i] < D;
-            in1[i] = off1[i] < D;
         }
     }
-    // the pair whose angle entry e of chunk i belongs to
-    __device__ __forceinline__ int pair(int i, int e, int l, int log_l) const {
-        if (INTER && V > 1) return e < V / 2 ? off0[i] / 2 + e : off1[i] / 2 + e - V / 2;
-        return (l + (i << log_l)) * V + e;
+    // Where pair p's cos and sin lie.  A lane of the half layout takes eight neighbours: their two 16-byte halves are kept apart, so that
+    // neighbouring lanes read neighbouring banks.
+    __device__ __forceinline__ static int place(int p, int P) {
+        return V == 8 && !INTER ? (p % 8 / 4) * ((P + 7) / 8 * 4) + p / 8 * 4 + p % 4 : p;
     }
+    // cos or sin of chunk i's pairs, read from shared memory where they are used: kept in registers they cost 16 a thread, and with them a
+    // third of the warps that hide the loads
+    __device__ __forceinline__ void angles(uint32_t table, int i, int l, int log_l, int P, float* f) const {
+        const int c = l + (i << log_l);
+        if (V == 8) {
+            const int second = INTER ? 1 << log_l : (P + 7) / 8;
+            quad(table + 16 * c, f);
+            quad(table + 16 * (c + second), f + 4);
+        } else if (V == 4 && INTER) {
+            two(table + 8 * c, f);
+            two(table + 8 * (c + (1 << log_l)), f + 2);
+        } else if (V == 4) {
+            quad(table + 16 * c, f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[e]) : "r"(table + 4 * min(c * V + e, kMaxD / 2 - 1)));
+        }
+    }
+    __device__ __forceinline__ static void quad(uint32_t at, float* f) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(at));
+    }
+    __device__ __forceinline__ static void two(uint32_t at, float* f) { asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f[0]), "=f"(f[1]) : "r"(at)); }
 };
 
-template <int V, bool INTER>
-__device__ __forceinline__ void rotate(float* u, float* v, const float* c, const float* s, bool rot0, bool rot1) {
-    if (INTER && V > 1) {
+// The pairs' first and second elements of two vectors, and back
+template <typename T, int V, bool WHOLE> __device__ __forceinline__ void unpack(const Pack<T, V>& p0, const Pack<T, V>& p1, float* a, float* b) {
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e) {
-            const float a0 = u[2 * e], a1 = u[2 * e + 1], b0 = v[2 * e], b1 = v[2 * e + 1];
-            if (rot0) {
-                u[2 * e] = a0 * c[e] - a1 * s[e];
-                u[2 * e + 1] = a1 * c[e] + a0 * s[e];
-            }
-            if (rot1) {
-                v[2 * e] = b0 * c[V / 2 + e] - b1 * s[V / 2 + e];
-                v[2 * e + 1] = b1 * c[V / 2 + e] + b0 * s[V / 2 + e];
-            }
+    for (int e = 0; e < V; ++e) {
+        if (!WHOLE) {
+            a[e] = to_f(p0.v[e]);
+            b[e] = to_f(p1.v[e]);
+        } else {
+            const Pack<T, V>& p = e < V / 2 ? p0 : p1;
+            a[e] = to_f(p.v[2 * e % V]);
+            b[e] = to_f(p.v[(2 * e + 1) % V]);
         }
-    } else if (rot0) {
+    }
+}
+template <typename T, int V, bool WHOLE> __device__ __forceinline__ void pack(const float* a, const float* b, Pack<T, V>& p0, Pack<T, V>& p1) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float a = u[e], b = v[e];
-            u[e] = a * c[e] - b * s[e];
-            v[e] = b * c[e] + a * s[e];
+    for (int e = 0; e < V; ++e) {
+        if (!WHOLE) {
+            p0.v[e] = from_f<T>(a[e]);
+            p1.v[e] = from_f<T>(b[e]);
+        } else {
+            Pack<T, V>& p = e < V / 2 ? p0 : p1;
+            p.v[2 * e % V] = from_f<T>(a[e]);
+            p.v[(2 * e + 1) % V] = from_f<T>(b[e]);
         }
+    }
+}
+
+// (a, b) -> (a c - b s, b c + a s) for the pairs that are rotated; the second half of a chunk of whole pairs has a flag of its own
+template <int V, bool WHOLE> __device__ __forceinline__ void rotate(float* a, float* b, const float* c, const float* s, bool rot0, bool rot1) {
+    float y[V], z[V];
+    pairwise<V>(
+        [&](int e) {
+            const float2 a2 = at2(a, e), b2 = at2(b, e), c2 = at2(c, e), s2 = at2(s, e), n2 = make_float2(-s2.x, -s2.y);
+            put2(y, e, __ffma2_rn(a2, c2, __fmul2_rn(b2, n2)));
+            put2(z, e, __ffma2_rn(b2, c2, __fmul2_rn(a2, s2)));
+        },
+        [&](int e) {
+            y[e] = a[e] * c[e] - b[e] * s[e];
+            z[e] = b[e] * c[e] + a[e] * s[e];
+        });
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const bool rot = WHOLE && e >= V / 2 ? rot1 : rot0;
+        a[e] = rot ? y[e] : a[e];
+        b[e] = rot ? z[e] : b[e];
     }
 }
 
 enum { kRotate = 0, kNorm = 1, kNormBwd = 2 };
 
-// A group of 2^log_l lanes holds one head of one token; a warp's groups take consecutive heads of the same token, U rows per group at a
-// time so that 2 U (backward 4 U) loads are in flight.  A unit is one token with heads_per_unit heads; consecutive warps take
-// consecutive tokens, whose rows are neighbours in the head-major output.  CTAs below ctas_q work on q, the others on k.
-template <typename T, int V, int NV, bool INTER, int MODE>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const tt_rotary_args a, const int log_l, const int ctas_q, const int hpu_q, const int hpu_k) {
-    constexpr int U = MODE == kNormBwd ? (NV * V >= 8 ? 1 : 2) : (NV * V >= 4 ? 4 : 4);
+// Queries or keys.  Read from the constant bank where it is used (the index is the same for a whole CTA).
+struct Side {
+    const void *x, *g, *w;
+    void* y;
+    long xs[3], gs[3], ys[3];
+    int heads, hpu, parts;         // heads, heads per unit, units per token
+};
+struct Params {
+    Side side[2];
+    const void* positions;
+    const double* half_turns;
+    const int* axis;
+    float* partials;
+    long pos_stride[3], batch_tokens;
+    int tokens, D, P, pos_is_64, whole, ctas_q;
+    float amplitude, sin_amplitude, eps, inv_D;
+};
+
+// A group of 2^log_l lanes holds one head of one token; a warp's groups take consecutive heads.  A unit is a token with all heads of q and k
+// (`whole`), or with `hpu` heads of one of them; consecutive warps take consecutive tokens, whose rows are neighbours in the head-major
+// output.  The norm's backward keeps q and k apart, since a CTA sums one weight's gradient: CTAs below ctas_q work on q, the others on k.
+// The next row's loads are under way behind a row's arithmetic, and registers are held down for more warps: rotating 24 + 24 heads of 32400
+// tokens there and back took 367 us without the loads ahead, 331 with them and three CTAs an SM, 288 with four (5.5 TB/s; the norm's
+// forward 211 with two and 175 with three).
+template <typename T, int V, int NV, bool INTER, int MODE, int LOGL>
+__global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm ? 3 : 2) rotary_kernel(const __grid_constant__ Params a, const int any_log_l) {
+    constexpr bool WHOLE = Geometry<V, NV, INTER>::kWhole;
+    __shared__ alignas(16) float angle[kWarps][2][kMaxD / 2];         // cos, sin
     __shared__ float fold[MODE == kNormBwd ? kWarps : 1][MODE == kNormBwd ? kMaxD : 1];
-    const int which = (int)blockIdx.x >= ctas_q;
-    const long cta = which ? (long)blockIdx.x - ctas_q : blockIdx.x, n_ctas = which ? (long)gridDim.x - ctas_q : ctas_q;
-    const int heads = which ? a.k_heads : a.q_heads, hpu = which ? hpu_k : hpu_q;
-    const T* __restrict__ x = (const T*)(which ? a.k : a.q);
-    const T* __restrict__ g = (const T*)(which ? a.gk : a.gq);
-    const T* __restrict__ w = (const T*)(which ? a.k_weight : a.q_weight);
-    T* __restrict__ y = (T*)(which ? a.out_k : a.out_q);
-    const long *xs = which ? a.k_stride : a.q_stride, *gs = which ? a.gk_stride : a.gq_stride, *ys = which ? a.out_k_stride : a.out_q_stride;
-    const long xb = xs[0], xh = xs[1], xt = xs[2], gb = gs[0], gh = gs[1], gt = gs[2], yb = ys[0], yh = ys[1], yt = ys[2];
+    const int log_l = LOGL >= 0 ? LOGL : any_log_l;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int l = lane & ((1 << log_l) - 1), sub = lane >> log_l, rows = 32 >> log_l;
-    const int D = a.head_dim, P = a.pairs;
-    const Geometry<V, NV, INTER> geo(l, log_l, D, P);
-    const long tokens = (long)a.batch * a.tokens;
-    const int parts = (heads + hpu - 1) / hpu;
-    const long units = tokens * parts;
-
-    float w0[NV][V], w1[NV][V], acc0[NV][V], acc1[NV][V];
-    if (MODE != kRotate) {
+    const int D = a.D, P = a.P;
+    const Geometry<V, NV, INTER> geo(l, log_l, P);
+    bool in0[NV], in1[NV], rot0[NV], rot1[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            Pack<T, V> p0, p1;
-            if (geo.in0[i]) p0.load(w + geo.off0[i]);
-            if (geo.in1[i]) p1.load(w + geo.off1[i]);
-            p0.get(w0[i]);
-            p1.get(w1[i]);
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc0[i][e] = acc1[i][e] = 0.f;
-        }
+    for (int i = 0; i < NV; ++i) {
+        in0[i] = geo.off0[i] < D;
+        in1[i] = geo.off1[i] < D;
+        rot0[i] = WHOLE ? geo.off0[i] < 2 * P : (l + (i << log_l)) * V < P;
+        rot1[i] = geo.off1[i] < 2 * P;
     }
+    const uint32_t cos_table = sm100::smem_u32(&angle[warp][0][0]);
+    const int only = MODE != kNormBwd ? -1 : (int)blockIdx.x >= a.ctas_q ? 1 : 0;
+    const int cta = (int)blockIdx.x - (only == 1 ? a.ctas_q : 0), n_ctas = only < 0 ? (int)gridDim.x : only ? (int)gridDim.x - a.ctas_q : a.ctas_q;
+    const int parts = only >= 0 ? a.side[only].parts : a.whole ? 1 : a.side[0].parts + a.side[1].parts;
+    const long units = a.batch_tokens * parts;
+
+    float acc0[NV][V], acc1[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc0[i][e] = acc1[i][e] = 0.f;
     auto group_sum = [&](float v) {
-        for (int o = 1 << log_l >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            if (o < 1 << log_l) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     };
 
-    for (long unit = cta * kWarps + warp; unit < units; unit += n_ctas * kWarps) {
-        const int part = parts == 1 ? 0 : (int)(unit / tokens);
-        const long token = parts == 1 ? unit : unit - (long)part * tokens;
-        const long b = token / a.tokens, t = token - b * a.tokens;
-        const int h_end = min(heads, (part + 1) * hpu);
-        float cs[NV][V], sn[NV][V];
-        {
-            const long at = b * a.pos_stride[0] + t * a.pos_stride[2];
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const int p = geo.pair(i, e, l, log_l);
-                    cs[i][e] = 1.f;
-                    sn[i][e] = 0.f;
-                    if (p < P) {
-                        const long q = at + (a.axis != nullptr ? a.axis[p] * a.pos_stride[1] : 0L);
-                        const double pos = a.pos_is_64 ? (double)((const long long*)a.positions)[q] : (double)((const int*)a.positions)[q];
-                        const double h = pos * a.half_turns[p];                // angle / pi
-                        sincospif((float)(h - 2.0 * rint(0.5 * h)), &sn[i][e], &cs[i][e]);
-                        cs[i][e] *= a.amplitude;
-                        sn[i][e] *= MODE == kNormBwd || a.transpose ? -a.amplitude : a.amplitude;
-                    }
-                }
+    for (long unit = (long)cta * kWarps + warp; unit < units; unit += (long)n_ctas * kWarps) {
+        int part = 0;
+        long token = unit;
+        if (parts > 1) {
+            part = (int)(unit / a.batch_tokens);
+            token = unit - (long)part * a.batch_tokens;
         }
-        const T* xp = x + b * xb + t * xt;
-        const T* gp = g + b * gb + t * gt;
-        T* yp = y + b * yb + t * yt;
-        for (int h0 = part * hpu + sub; h0 - sub < h_end; h0 += rows * U) {
-            Pack<T, V> px0[U][NV], px1[U][NV], pg0[U][NV], pg1[U][NV];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int h = h0 + u * rows;
-                if (h < h_end) {
-#pragma unroll
-                    for (int i = 0; i < NV; ++i) {
-                        if (geo.in0[i]) px0[u][i].load(xp + h * xh + geo.off0[i]);
-                        if (geo.in1[i]) px1[u][i].load(xp + h * xh + geo.off1[i]);
-                        if (MODE == kNormBwd) {
-                            if (geo.in0[i]) pg0[u][i].load(gp + h * gh + geo.off0[i]);
-                            if (geo.in1[i]) pg1[u][i].load(gp + h * gh + geo.off1[i]);
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int h = h0 + u * rows;
-                float f0[NV][V], f1[NV][V];
+        long b = 0;
+        int t = (int)token;
+        if (a.batch_tokens > a.tokens) {
+            b = a.batch_tokens <= INT_MAX ? (int)token / a.tokens : token / a.tokens;
+            t = (int)(token - b * a.tokens);
+        }
+        int which = only >= 0 ? only : !a.whole && part >= a.side[0].parts ? 1 : 0;
+        if (only < 0 && which) part -= a.side[0].parts;
+        const int last = only < 0 && a.whole ? 2 : which + 1;
+        bool angles_done = false;
+        for (; which < last; ++which) {
+            const Side& side = a.side[which];
+            const int h_end = min(side.heads, (part + 1) * side.hpu);
+            int h0 = part * side.hpu + sub;
+            if (h0 - sub >= h_end) continue;        // no heads
+            const T* xr = (const T*)side.x + b * side.xs[0] + t * side.xs[2] + h0 * side.xs[1];
+            const T* gr = (const T*)side.g + b * side.gs[0] + t * side.gs[2] + h0 * side.gs[1];
+            T* yr = (T*)side.y + b * side.ys[0] + t * side.ys[2] + h0 * side.ys[1];
+            Pack<T, V> nx0[NV], nx1[NV], ng0[NV], ng1[NV], pw0[NV], pw1[NV];
+            auto load = [&] {           // rows behind the last head are 0: they count for nothing in the weights' gradient
+                const bool ok = h0 < h_end;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    px0[u][i].get(f0[i]);
-                    px1[u][i].get(f1[i]);
-                }
-                if (MODE != kRotate) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int i = 0; i < NV; ++i)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) ss += f0[i][e] * f0[i][e] + f1[i][e] * f1[i][e];
-                    const float r = rsqrtf(group_sum(ss) / (float)D + a.eps);
-#pragma unroll
-                    for (int i = 0; i < NV; ++i)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            f0[i][e] *= MODE == kNorm ? r * w0[i][e] : r;
-                            f1[i][e] *= MODE == kNorm ? r * w1[i][e] : r;
-                        }
+                    nx0[i] = nx1[i] = Pack<T, V>();
+                    if (ok && in0[i]) nx0[i].load(xr + geo.off0[i]);
+                    if (ok && in1[i]) nx1[i].load(xr + geo.off1[i]);
                     if (MODE == kNormBwd) {
-                        float g0[NV][V], g1[NV][V], dot = 0.f;
-#pragma unroll
-                        for (int i = 0; i < NV; ++i) {
-                            pg0[u][i].get(g0[i]);
-                            pg1[u][i].get(g1[i]);
-                            rotate<V, INTER>(g0[i], g1[i], cs[i], sn[i], geo.rot0[i], geo.rot1[i]);
-#pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                acc0[i][e] += g0[i][e] * f0[i][e];
-                                acc1[i][e] += g1[i][e] * f1[i][e];
-                                g0[i][e] *= w0[i][e];
-                                g1[i][e] *= w1[i][e];
-                                dot += g0[i][e] * f0[i][e] + g1[i][e] * f1[i][e];
-                            }
-                        }
-                        dot = group_sum(dot) / (float)D;
-#pragma unroll
-                        for (int i = 0; i < NV; ++i)
-#pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                f0[i][e] = r * (g0[i][e] - f0[i][e] * dot);
-                                f1[i][e] = r * (g1[i][e] - f1[i][e] * dot);
-                            }
+                        ng0[i] = ng1[i] = Pack<T, V>();
+                        if (ok && in0[i]) ng0[i].load(gr + geo.off0[i]);
+                        if (ok && in1[i]) ng1[i].load(gr + geo.off1[i]);
                     }
                 }
-                if (h < h_end) {
+            };
+            load();         // under way while the angles are formed
+            if (MODE != kRotate) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    if (in0[i]) pw0[i].load((const T*)side.w + geo.off0[i]);
+                    if (in1[i]) pw1[i].load((const T*)side.w + geo.off1[i]);
+                }
+            }
+            if (!angles_done) {     // every pair's angle once per warp, spread over the lanes
+                const long at = b * a.pos_stride[0] + t * a.pos_stride[2];
+                __syncwarp();
+                for (int p = lane; p < P; p += 32) {
+                    const long q = at + (a.axis != nullptr ? a.axis[p] * a.pos_stride[1] : 0L);
+                    const double pos = a.pos_is_64 ? (double)((const long long*)a.positions)[q] : (double)((const int*)a.positions)[q];
+                    const double h = pos * a.half_turns[p];                // angle / pi
+                    float c, s;
+                    sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
+                    const int place = Geometry<V, NV, INTER>::place(p, P);
+                    angle[warp][0][place] = c * a.amplitude;
+                    angle[warp][1][place] = s * a.sin_amplitude;
+                }
+                __syncwarp();
+                angles_done = true;
+            }
+            while (true) {
+                Pack<T, V> px0[NV], px1[NV], pg0[NV], pg1[NV];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    px0[i] = nx0[i];
+                    px1[i] = nx1[i];
+                    if (MODE == kNormBwd) {
+                        pg0[i] = ng0[i];
+                        pg1[i] = ng1[i];
+                    }
+                }
+                const bool mine = h0 < h_end;
+                T* out = yr;
+                h0 += rows;
+                const bool more = h0 - sub < h_end;
+                if (more) {         // the next row's loads are under way behind this one's arithmetic
+                    xr += rows * side.xs[1];
+                    gr += rows * side.gs[1];
+                    yr += rows * side.ys[1];
+                    load();
+                }
+                float f0[NV][V], f1[NV][V];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) unpack<T, V, WHOLE>(px0[i], px1[i], f0[i], f1[i]);
+                if (MODE != kRotate) {
+                    float sq[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) sq[e] = 0.f;
 #pragma unroll
                     for (int i = 0; i < NV; ++i) {
-                        if (MODE != kNormBwd) rotate<V, INTER>(f0[i], f1[i], cs[i], sn[i], geo.rot0[i], geo.rot1[i]);
-                        Pack<T, V> o0, o1;
-                        o0.set(f0[i]);
-                        o1.set(f1[i]);
-                        if (geo.in0[i]) o0.store(yp + h * yh + geo.off0[i]);
-                        if (geo.in1[i]) o1.store(yp + h * yh + geo.off1[i]);
+                        add_product<V>(sq, f0[i], f0[i]);
+                        add_product<V>(sq, f1[i], f1[i]);
+                    }
+                    float ss = sq[0];
+#pragma unroll
+                    for (int e = 1; e < V; ++e) ss += sq[e];
+                    const float r = rsqrtf(group_sum(ss) * a.inv_D + a.eps);
+                    float g0[NV][V], g1[NV][V], dots[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) dots[e] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        float w0[V], w1[V];
+                        unpack<T, V, WHOLE>(pw0[i], pw1[i], w0, w1);
+                        scale<V>(f0[i], r);
+                        scale<V>(f1[i], r);
+                        if (MODE == kNorm) {
+                            mul<V>(f0[i], w0);
+                            mul<V>(f1[i], w1);
+                        } else {
+                            float cs[V], sn[V];
+                            geo.angles(cos_table, i, l, log_l, P, cs);
+                            geo.angles(cos_table + 4 * (kMaxD / 2), i, l, log_l, P, sn);
+                            unpack<T, V, WHOLE>(pg0[i], pg1[i], g0[i], g1[i]);
+                            rotate<V, WHOLE>(g0[i], g1[i], cs, sn, rot0[i], rot1[i]);
+                            add_product<V>(acc0[i], g0[i], f0[i]);
+                            add_product<V>(acc1[i], g1[i], f1[i]);
+                            mul<V>(g0[i], w0);
+                            mul<V>(g1[i], w1);
+                            add_product<V>(dots, g0[i], f0[i]);
+                            add_product<V>(dots, g1[i], f1[i]);
+                        }
+                    }
+                    if (MODE == kNormBwd) {
+                        float dot = dots[0];
+#pragma unroll
+                        for (int e = 1; e < V; ++e) dot += dots[e];
+                        dot = -group_sum(dot) * a.inv_D;
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) {
+                            scale<V>(f0[i], dot);
+                            scale<V>(f1[i], dot);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) {
+                                f0[i][e] = r * (g0[i][e] + f0[i][e]);
+                                f1[i][e] = r * (g1[i][e] + f1[i][e]);
+                            }
+                        }
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    if (MODE != kNormBwd) {
+                        float cs[V], sn[V];
+                        geo.angles(cos_table, i, l, log_l, P, cs);
+                        geo.angles(cos_table + 4 * (kMaxD / 2), i, l, log_l, P, sn);
+                        rotate<V, WHOLE>(f0[i], f1[i], cs, sn, rot0[i], rot1[i]);
+                    }
+                    Pack<T, V> o0, o1;
+                    pack<T, V, WHOLE>(f0[i], f1[i], o0, o1);
+                    if (mine && in0[i]) o0.store(out + geo.off0[i]);
+                    if (mine && in1[i]) o1.store(out + geo.off1[i]);
+                }
+                if (!more) break;
             }
         }
     }
@@ -278,9 +410,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const tt_rotary_args a
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if (geo.in0[i]) fold[warp][geo.off0[i] + e] = acc0[i][e];
-                    if (geo.in1[i]) fold[warp][geo.off1[i] + e] = acc1[i][e];
+                for (int e = 0; e < V; ++e) {       // where unpack took entry e from
+                    const bool second = WHOLE && e >= V / 2;
+                    const int at0 = !WHOLE ? geo.off0[i] + e : (second ? geo.off1[i] : geo.off0[i]) + 2 * e % V;
+                    const int at1 = !WHOLE ? geo.off1[i] + e : at0 + 1;
+                    if (at0 < D) fold[warp][at0] = acc0[i][e];
+                    if (at1 < D) fold[warp][at1] = acc1[i][e];
                 }
         }
         __syncthreads();
@@ -316,7 +451,7 @@ __global__ void __launch_bounds__(kFinCols * kFinRows) rotary_weight_kernel(cons
 }
 
 struct Plan {
-    int width, log_l, ctas_q, ctas_k, hpu_q, hpu_k;
+    int width, log_l, whole, ctas_q, ctas_k, hpu_q, hpu_k;      // forward: ctas_q for both
 };
 
 int elem_size(int dtype) { return dtype == TT_FP32 ? 4 : 2; }
@@ -343,15 +478,16 @@ int vector_width(const tt_rotary_args& a) {
     return 1;
 }
 
-Plan plan(const tt_rotary_args& a, int sms) {
+Plan plan(const tt_rotary_args& a, int sms, int mode) {
     Plan p;
     p.width = vector_width(a);
     const int chunks = (a.head_dim + 2 * p.width - 1) / (2 * p.width);
     p.log_l = 0;
     while ((1 << p.log_l) < chunks && p.log_l < 5) ++p.log_l;
     const int rows = 32 >> p.log_l;
-    const long tokens = (long)a.batch * a.tokens;
+    const long tokens = a.batch * a.tokens;
     // All heads of a token in one unit share its angles.  With few tokens a unit takes fewer heads, so that the units cover the device.
+    p.whole = tokens >= (long)sms * kWarps;
     auto heads_per_unit = [&](int heads) {
         int per = (heads + rows - 1) / rows;
         while (per > 1 && tokens * ((heads + rows * per - 1) / (rows * per)) < (long)sms * kWarps) per = (per + 1) / 2;
@@ -360,39 +496,75 @@ Plan plan(const tt_rotary_args& a, int sms) {
     p.hpu_q = heads_per_unit(a.q_heads);
     p.hpu_k = heads_per_unit(a.k_heads);
     const long cap = (long)sms * 8;
-    auto ctas = [&](int heads, int hpu) {
-        if (heads == 0) return 0L;
-        const long units = tokens * ((heads + hpu - 1) / hpu), want = (units + kWarps - 1) / kWarps;
-        const long most = (cap * heads + a.q_heads + a.k_heads - 1) / (a.q_heads + a.k_heads);
-        return want < most ? want : most;
+    auto ctas = [&](long parts, long most) {
+        const long want = (tokens * parts + kWarps - 1) / kWarps;
+        return (int)(want < most ? want : most);
     };
-    p.ctas_q = (int)ctas(a.q_heads, p.hpu_q);
-    p.ctas_k = (int)ctas(a.k_heads, p.hpu_k);
+    const long parts_q = (a.q_heads + p.hpu_q - 1) / p.hpu_q, parts_k = (a.k_heads + p.hpu_k - 1) / p.hpu_k;
+    if (mode != kNormBwd) {
+        p.ctas_q = ctas(p.whole ? 1 : parts_q + parts_k, INT_MAX);
+        p.ctas_k = 0;
+    } else {
+        p.ctas_q = ctas(parts_q, (cap * a.q_heads + a.q_heads + a.k_heads - 1) / (a.q_heads + a.k_heads));
+        p.ctas_k = ctas(parts_k, (cap * a.k_heads + a.q_heads + a.k_heads - 1) / (a.q_heads + a.k_heads));
+    }
     return p;
 }
 
-template <typename T, int V, int NV, bool INTER>
-void launch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
-    const int grid = p.ctas_q + p.ctas_k;
-    if (mode == kRotate) rotary_kernel<T, V, NV, INTER, kRotate><<<grid, kThreads, 0, st>>>(a, p.log_l, p.ctas_q, p.hpu_q, p.hpu_k);
-    else if (mode == kNorm) rotary_kernel<T, V, NV, INTER, kNorm><<<grid, kThreads, 0, st>>>(a, p.log_l, p.ctas_q, p.hpu_q, p.hpu_k);
-    else rotary_kernel<T, V, NV, INTER, kNormBwd><<<grid, kThreads, 0, st>>>(a, p.log_l, p.ctas_q, p.hpu_q, p.hpu_k);
+Params params(const tt_rotary_args& a, const Plan& p, int mode) {
+    Params k;
+    k.side[0] = {a.q, a.gq, a.q_weight, a.out_q, {}, {}, {}, a.q_heads, p.hpu_q, (a.q_heads + p.hpu_q - 1) / p.hpu_q};
+    k.side[1] = {a.k, a.gk, a.k_weight, a.out_k, {}, {}, {}, a.k_heads, p.hpu_k, (a.k_heads + p.hpu_k - 1) / p.hpu_k};
+    for (int i = 0; i < 3; ++i) {
+        k.side[0].xs[i] = a.q_stride[i];
+        k.side[0].gs[i] = a.gq_stride[i];
+        k.side[0].ys[i] = a.out_q_stride[i];
+        k.side[1].xs[i] = a.k_stride[i];
+        k.side[1].gs[i] = a.gk_stride[i];
+        k.side[1].ys[i] = a.out_k_stride[i];
+        k.pos_stride[i] = a.pos_stride[i];
+    }
+    k.positions = a.positions;
+    k.half_turns = a.half_turns;
+    k.axis = a.axis;
+    k.partials = a.partials;
+    k.batch_tokens = a.batch * a.tokens;
+    k.tokens = (int)a.tokens;
+    k.D = a.head_dim;
+    k.P = a.pairs;
+    k.pos_is_64 = a.pos_is_64;
+    k.whole = p.whole;
+    k.ctas_q = p.ctas_q;
+    k.amplitude = a.amplitude;
+    k.sin_amplitude = mode == kNormBwd || a.transpose ? -a.amplitude : a.amplitude;
+    k.eps = a.eps;
+    k.inv_D = 1.f / (float)a.head_dim;
+    return k;
 }
 
+template <typename T, int V, int NV, bool INTER, int LOGL = -1>
+void launch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
+    const int grid = p.ctas_q + p.ctas_k;
+    const Params k = params(a, p, mode);
+    if (mode == kRotate) rotary_kernel<T, V, NV, INTER, kRotate, LOGL><<<grid, kThreads, 0, st>>>(k, p.log_l);
+    else if (mode == kNorm) rotary_kernel<T, V, NV, INTER, kNorm, LOGL><<<grid, kThreads, 0, st>>>(k, p.log_l);
+    else rotary_kernel<T, V, NV, INTER, kNormBwd, LOGL><<<grid, kThreads, 0, st>>>(k, p.log_l);
+}
+
+// Full-width vectors of 16-bit heads of 64 and 128 (four and eight lanes) have the lanes of a head compiled in.
 template <typename T>
 void dispatch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
-    constexpr int W = 16 / sizeof(T);
-    if (p.width == W && a.interleaved) launch<T, W, 1, true>(a, p, mode, st);
-    else if (p.width == W) launch<T, W, 1, false>(a, p, mode, st);
-    else if (p.width == 2 && a.interleaved) launch<T, 2, 2, true>(a, p, mode, st);
-    else if (p.width == 2) launch<T, 2, 2, false>(a, p, mode, st);
-    else if (a.interleaved) launch<T, 1, 4, true>(a, p, mode, st);
-    else launch<T, 1, 4, false>(a, p, mode, st);
+    constexpr int W = 16 / sizeof(T), A = W == 8 ? 3 : -1, B = W == 8 ? 2 : -1;
+    if (p.width == W && W == 8 && p.log_l == 3) a.interleaved ? launch<T, W, 1, true, A>(a, p, mode, st) : launch<T, W, 1, false, A>(a, p, mode, st);
+    else if (p.width == W && W == 8 && p.log_l == 2) a.interleaved ? launch<T, W, 1, true, B>(a, p, mode, st) : launch<T, W, 1, false, B>(a, p, mode, st);
+    else if (p.width == W) a.interleaved ? launch<T, W, 1, true>(a, p, mode, st) : launch<T, W, 1, false>(a, p, mode, st);
+    else if (p.width == 2) a.interleaved ? launch<T, 2, 2, true>(a, p, mode, st) : launch<T, 2, 2, false>(a, p, mode, st);
+    else a.interleaved ? launch<T, 1, 4, true>(a, p, mode, st) : launch<T, 1, 4, false>(a, p, mode, st);
 }
 
 int check(const tt_rotary_args* a) {
     if (a == nullptr || a->struct_size != (long)sizeof(tt_rotary_args)) return TT_ERR_ARG;
-    if (a->batch <= 0 || a->tokens <= 0 || a->q_heads < 0 || a->k_heads < 0 || a->q_heads + a->k_heads == 0) return TT_ERR_ARG;
+    if (a->batch <= 0 || a->tokens <= 0 || a->tokens > INT_MAX || a->batch > INT_MAX || a->q_heads < 0 || a->k_heads < 0 || a->q_heads + a->k_heads == 0) return TT_ERR_ARG;
     if (a->head_dim <= 0 || a->head_dim % 2 || a->pairs <= 0 || 2 * a->pairs > a->head_dim) return TT_ERR_ARG;
     if (a->head_dim > kMaxD) return TT_ERR_LIMIT;
     if (a->dtype != TT_BF16 && a->dtype != TT_FP16 && a->dtype != TT_FP32) return TT_ERR_ARG;
@@ -409,7 +581,7 @@ int run(const tt_rotary_args* a, int mode, void* stream) {
     if (mode == kNormBwd && (a->partials == nullptr || (a->q_heads > 0 && (a->gq == nullptr || a->dq_weight == nullptr)) ||
                              (a->k_heads > 0 && (a->gk == nullptr || a->dk_weight == nullptr))))
         return TT_ERR_ARG;
-    const Plan p = plan(*a, tt_device().sms);
+    const Plan p = plan(*a, tt_device().sms, mode);
     if (mode == kNormBwd && a->partial_floats < (long)(p.ctas_q + p.ctas_k) * a->head_dim) return TT_ERR_ARG;
     cudaStream_t st = (cudaStream_t)stream;
     if (a->dtype == TT_BF16) dispatch<__nv_bfloat16>(*a, p, mode, st);
@@ -436,7 +608,7 @@ int run(const tt_rotary_args* a, int mode, void* stream) {
 
 extern "C" long tt_rotary_partial_floats(const tt_rotary_args* a) {
     if (check(a) != TT_OK) return -1;
-    const Plan p = plan(*a, tt_device().sms);
+    const Plan p = plan(*a, tt_device().sms, kNormBwd);
     return (long)(p.ctas_q + p.ctas_k) * a->head_dim;
 }
 extern "C" int tt_rotary(const tt_rotary_args* a, void* stream) { return run(a, kRotate, stream); }
