@@ -96,11 +96,41 @@ __device__ __forceinline__ void clear_rows(uint32_t tile, int slabs, uint4 bits,
     }
 }
 
-// Score of the log2 domain behind the cap: cap tanh(s / cap) log2(e), from tanh x = 1 - 2 / (1 + e^2x), exact to a few roundings of the cap.
-__device__ __forceinline__ float capped(float s, float two_over_cap_log2e, float cap_log2e, float* t_out) {
-    const float t = 1.f - __fdividef(2.f, 1.f + exp2f(s * two_over_cap_log2e));
-    *t_out = t;
-    return cap_log2e * t;
+// cap tanh(scale z / cap) log2(e) of raw scores z, in the log2 domain.  Where all of a warp's scores are small against the cap the odd Taylor
+// series up to the ninth power (|u| <= 0.3: the next term is below 2^-24 of the value) takes six packed multiply-adds a pair; else
+// tanh u = 1 - 2 / (1 + e^2u), two special functions a score, exact to a few roundings of the cap.
+struct Cap {
+    float two_u, out, inv_out;      // 2 / cap * scale * log2(e); cap * log2(e), and its inverse; two_u and out 0: no cap
+    float small;                    // largest |z| of the series
+    float c[5];                     // its coefficients times scale * log2(e)
+};
+inline Cap make_cap(float scale, float softcap) {
+    Cap k = {};
+    if (!(softcap > 0.f)) return k;
+    const double u = (double)scale / softcap, t[5] = {1.0, -1.0 / 3, 2.0 / 15, -17.0 / 315, 62.0 / 2835};
+    double power = (double)scale * kLog2e;
+    for (int i = 0; i < 5; ++i, power *= u * u) k.c[i] = (float)(t[i] * power);
+    k.two_u = (float)(2.0 * u * kLog2e);
+    k.out = softcap * kLog2e;
+    k.inv_out = 1.f / k.out;
+    k.small = scale != 0.f ? (float)fmin(0.3 / fabs(u), 3e38) : 3e38f;
+    return k;
+}
+__device__ __forceinline__ float2 cap_small(const Cap& k, float2 z) {
+    const float2 zz = __fmul2_rn(z, z);
+    float2 q = __ffma2_rn(zz, make_float2(k.c[4], k.c[4]), make_float2(k.c[3], k.c[3]));
+    q = __ffma2_rn(q, zz, make_float2(k.c[2], k.c[2]));
+    q = __ffma2_rn(q, zz, make_float2(k.c[1], k.c[1]));
+    q = __ffma2_rn(q, zz, make_float2(k.c[0], k.c[0]));
+    return __fmul2_rn(z, q);
+}
+__device__ __forceinline__ float cap_any(const Cap& k, float z) { return k.out * (1.f - __fdividef(2.f, 1.f + exp2f(z * k.two_u))); }
+// whether the largest magnitude of N scores of every lane is one of the series
+template <int N> __device__ __forceinline__ bool all_small(const Cap& k, const uint32_t* z) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(__uint_as_float(z[i])));
+    return __all_sync(0xffffffffu, m <= k.small);
 }
 
 }  // namespace ranges

@@ -9,7 +9,9 @@
 // tile of 128 queries and goes through its keys (dQ in TMEM).  Seven products per pair of tiles instead of five.
 //
 // Both are one template: stationary operands A1, A2 (K, V or Q, dO) stay in shared memory, streamed operands B1, B2 (Q, dO or K, V) come through
-// rings.  TMEM: T1 = A1 B1^T (scores), T2 = A2 B2^T (dP; overwritten by P and dS as bf16 / fp16 pairs), accumulators from column 256.  Warp
+// rings.  TMEM: T1 = A1 B1^T (scores), T2 = A2 B2^T (dP), accumulators from column 256.  The order of the products keeps both sides busy: with
+// stationary keys P overwrites the scores and dV takes it while dS is formed over dP; with stationary queries the next chunk's scores and
+// dP (in a second buffer) are formed behind this chunk's dS.  Warp
 // 0 loads, warp 1 issues, sixteen warps turn T1, T2 into P and dS (a thread: one stationary row, 32 streamed ones).
 #include <limits.h>
 
@@ -35,7 +37,8 @@ struct BwdParams {
     long s1[3], s2[3];                  // their strides
     float* partials;
     int q_len, kv_len, q_heads, group, R;
-    float scale, scale_log2, cap_in, cap_out;
+    float scale, scale_log2;
+    Cap cap;
     int* status;
 };
 
@@ -43,10 +46,13 @@ template <int D, bool KVS, int MODE> struct Layout {
     static constexpr int kSlabs = D / 64;
     static constexpr int kTileBytes = kSlabs * kSlab;
     static constexpr int kRing1 = MODE == kGeneralDbias && D == 128 ? 2 : 3, kRing2 = D == 64 ? 3 : 2;
-    static constexpr int kBars = 1 + 3 * kRing1 + 3 * kRing2 + 6;
-    static constexpr int kFixed = (2 + kRing1 + kRing2) * kTileBytes + (kBars + 1) / 2 * 16;
-    static constexpr int smem(int R) { return kFixed + 1024 + (MODE == kGeneralDbias ? (2 * 16 * 64 + 2 * R + 1 + 2 * kDiagPad) * 4 : 0); }
+    static constexpr int kStats = KVS ? (kRing1 + kRing2) * kTile * 4 : 0;      // lse with every slot of Q, delta with every slot of dO
+    static constexpr int kBars = 1 + 3 * kRing1 + 3 * kRing2 + 7;
+    static constexpr int kFixed = (2 + kRing1 + kRing2) * kTileBytes + kStats + (kBars + 1) / 2 * 16 + 16;      // barriers, the abort flag and the tensor memory's address
+    // dynamic shared memory is declared to start at a 1024-byte boundary, and there is no static one ahead of it
+    static constexpr int smem(int R) { return kFixed + (MODE == kGeneralDbias ? (2 * 16 * 64 + 2 * R + 1 + 2 * kDiagPad) * 4 : 0); }
 };
+static_assert(Layout<128, true, kPlain>::smem(0) <= 232448, "shared memory of an SM");
 
 template <int D, bool BF16, bool KVS, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -54,15 +60,20 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                   const __grid_constant__ CUtensorMap tmDO, const BwdParams p) {
     using L = Layout<D, KVS, MODE>;
     constexpr int kTileBytes = L::kTileBytes, kRing1 = L::kRing1, kRing2 = L::kRing2;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ volatile int abort_flag;
-    __shared__ uint32_t tmem_base_slot;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem_raw + L::kFixed - 16);
+    uint32_t& tmem_base_slot = *reinterpret_cast<uint32_t*>(smem_raw + L::kFixed - 8);
 
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t base = smem_u32(smem_raw);
+    if (base & 1023u) {                 // the swizzled tiles would be read wrongly
+        if (threadIdx.x == 0) atomicExch(p.status, TT_ERR_ARG);
+        return;
+    }
     const uint32_t sA1 = base, sA2 = base + kTileBytes;
     const uint32_t sRing1 = base + 2 * kTileBytes, sRing2 = sRing1 + kRing1 * kTileBytes;
-    const uint32_t bars = sRing2 + kRing2 * kTileBytes;
-    float* scratch = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + L::kFixed);      // [2][16 warps][64]: diagonals of a warp's block
+    const uint32_t sLse = sRing2 + kRing2 * kTileBytes, sDelta = sLse + kRing1 * kTile * 4;     // KVS
+    const uint32_t bars = sRing2 + kRing2 * kTileBytes + L::kStats;
+    float* scratch = reinterpret_cast<float*>(smem_raw + L::kFixed);      // [2][16 warps][64]: diagonals of a warp's block
     float* diag = scratch + 2 * 16 * 64;                                                                // [2 R + 1 + 2 kDiagPad]
     const uint32_t a_full = bars;
     auto b1_full = [&](int s) { return bars + 8u * (1 + s); };
@@ -72,7 +83,7 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     auto b2_empty = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + kRing2 + s); };
     auto b2_clean = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + 2 * kRing2 + s); };
     const uint32_t s_full = bars + 8u * (1 + 3 * kRing1 + 3 * kRing2);      // T1 holds this chunk's scores
-    const uint32_t dp_full = s_full + 8u;                      // T2 holds this chunk's dP
+    auto dp_full = [&](int c) { return s_full + 8u + (KVS ? 0u : 40u * (uint32_t)(c & 1)); };      // the chunk's dP is there (dQ: two buffers)
     const uint32_t p_ready = s_full + 16u;                     // every softmax warp has read the scores
     const uint32_t ds_ready = s_full + 24u;                    // P and dS have been written over dP
     const uint32_t acc_final = s_full + 32u;
@@ -106,6 +117,7 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int g = c / per_head;
         return Chunk{head0 + g, lo + c - g * per_head};
     };
+    auto lds4 = [](uint32_t at, float4& v) { asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at)); };
     // a streamed tile with rows that no run reaches: queries that see nothing, keys that nothing sees
     auto is_dirty = [&](int c) { return c < n_chunks ? (KVS ? plan.q_tiles[chunk_at(c).t].w == 0 : plan.dirty[lo + c] != 0) : false; };
 
@@ -123,7 +135,8 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             mbar_init(b2_clean(s), 1);
         }
         mbar_init(s_full, 1);
-        mbar_init(dp_full, 1);
+        mbar_init(dp_full(0), 1);
+        if (!KVS) mbar_init(dp_full(1), 1);
         mbar_init(p_ready, 4 * kGroups);
         mbar_init(ds_ready, 4 * kGroups);
         mbar_init(acc_final, 1);
@@ -141,7 +154,7 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_slot;
-    constexpr uint32_t kT1 = 0, kT2 = 128, kAcc1 = 256, kAcc2 = 256 + D;
+    constexpr uint32_t kT1 = 0, kT2 = 128, kAcc1 = 256, kAcc2 = 256 + D, kT3 = 384;       // kT3: the second dP of the dQ kernel, which has no kAcc2
 
     if (warp == 0) {
         // ------------------------------------------------------------ loads
@@ -164,13 +177,15 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint32_t d1 = sRing1 + s1 * kTileBytes, d2 = sRing2 + s2 * kTileBytes;
             if (!warp_wait(b1_empty(s1), ph1 ^ 1u, &abort_flag)) goto done;
             if (lead) {
-                mbar_arrive_expect_tx(b1_full(s1), kTileBytes);
+                mbar_arrive_expect_tx(b1_full(s1), kTileBytes + (KVS ? kTile * 4 : 0));
+                if (KVS) bulk_load_1d(sLse + s1 * kTile * 4, p.lse + (((long)b * p.q_heads + head) * p.plan.q_tiles + ch.t) * kTile, kTile * 4, b1_full(s1));
 #pragma unroll
                 for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d1 + h * kSlab, KVS ? &tmQ : &tmK, b1_full(s1), h * 64, row, head, b);
             }
             if (!warp_wait(b2_empty(s2), ph2 ^ 1u, &abort_flag)) goto done;
             if (lead) {
-                mbar_arrive_expect_tx(b2_full(s2), kTileBytes);
+                mbar_arrive_expect_tx(b2_full(s2), kTileBytes + (KVS ? kTile * 4 : 0));
+                if (KVS) bulk_load_1d(sDelta + s2 * kTile * 4, p.delta + (((long)b * p.q_heads + head) * p.plan.q_tiles + ch.t) * kTile, kTile * 4, b2_full(s2));
 #pragma unroll
                 for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d2 + h * kSlab, KVS ? &tmDO : &tmV, b2_full(s2), h * 64, row, head, b);
             }
@@ -249,33 +264,53 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (!wait_b2(0, dirty)) goto done;
                 tc_fence_after();
                 issue_t(kT2, sA2, sRing2);
-                umma_commit(dp_full);
+                umma_commit(dp_full(0));
+                if (!KVS) umma_commit(b2_empty(0));
             }
             for (int c = 0; c < n_chunks; ++c) {
                 const uint32_t par = (uint32_t)c & 1u;
                 const bool more = c + 1 < n_chunks;
                 const bool dirty_next = is_dirty(c + 1);
-                // T1 is free as soon as every softmax warp has read the scores: the next chunk's overlap the dS pass
+                const uint32_t next1 = sRing1 + (c + 1) % kRing1 * kTileBytes, next2 = sRing2 + (c + 1) % kRing2 * kTileBytes;
                 if (!mbar_wait(p_ready, par, &abort_flag)) goto done;
                 tc_fence_after();
-                if (more) {
-                    if (!wait_b1(c + 1, dirty_next)) goto done;
+                if (KVS) {
+                    // T1 holds P: dV takes it while dS is formed, then the next chunk's scores take T1
+                    issue_acc(kAcc1, kT1, sRing2 + c % kRing2 * kTileBytes, c == 0);                    // dV += P^T dO
+                    if (more) {
+                        if (!wait_b1(c + 1, dirty_next)) goto done;
+                        tc_fence_after();
+                        issue_t(kT1, sA1, next1);
+                        umma_commit(s_full);
+                    }
+                    if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
                     tc_fence_after();
-                    issue_t(kT1, sA1, sRing1 + (c + 1) % kRing1 * kTileBytes);
-                    umma_commit(s_full);
-                }
-                // T2 now holds P (first 16 columns of every 32) and dS (last 16)
-                if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
-                tc_fence_after();
-                issue_acc(KVS ? kAcc2 : kAcc1, kT2 + 16, sRing1 + c % kRing1 * kTileBytes, c == 0);     // dK += dS^T Q  /  dQ += dS K
-                umma_commit(b1_empty(c % kRing1));
-                if (KVS) issue_acc(kAcc1, kT2, sRing2 + c % kRing2 * kTileBytes, c == 0);               // dV += P^T dO
-                umma_commit(b2_empty(c % kRing2));
-                if (more) {
-                    if (!wait_b2(c + 1, dirty_next)) goto done;
+                    issue_acc(kAcc2, kT2, sRing1 + c % kRing1 * kTileBytes, c == 0);                    // dK += dS^T Q
+                    umma_commit(b1_empty(c % kRing1));
+                    umma_commit(b2_empty(c % kRing2));         // not behind dV: delta lies in the slot until dS is formed
+                    if (more) {
+                        if (!wait_b2(c + 1, dirty_next)) goto done;
+                        tc_fence_after();
+                        issue_t(kT2, sA2, next2);
+                        umma_commit(dp_full(c + 1));
+                    }
+                } else {
+                    // the scores have been read: the next chunk's, and its dP in the other buffer, overlap this chunk's dS
+                    if (more) {
+                        if (!wait_b1(c + 1, dirty_next)) goto done;
+                        tc_fence_after();
+                        issue_t(kT1, sA1, next1);
+                        umma_commit(s_full);
+                        if (!wait_b2(c + 1, dirty_next)) goto done;
+                        tc_fence_after();
+                        issue_t(c & 1 ? kT2 : kT3, sA2, next2);
+                        umma_commit(dp_full(c + 1));
+                        umma_commit(b2_empty((c + 1) % kRing2));
+                    }
+                    if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
                     tc_fence_after();
-                    issue_t(kT2, sA2, sRing2 + (c + 1) % kRing2 * kTileBytes);
-                    umma_commit(dp_full);
+                    issue_acc(kAcc1, c & 1 ? kT3 : kT2, sRing1 + c % kRing1 * kTileBytes, c == 0);      // dQ += dS K
+                    umma_commit(b1_empty(c % kRing1));
                 }
             }
             umma_commit(acc_final);
@@ -286,12 +321,11 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int row = r0 + quad * 32 + lane;                  // key (KVS) or query
         const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
         const uint32_t t1 = tmem + lane_sel + kT1 + part * kCols, t2 = tmem + lane_sel + kT2 + part * kCols;
-        const int pitch = p.plan.q_tiles * kTile;
         const int start = plan.start;
         float my_lse = 0.f, my_delta = 0.f;
         int first = 0, behind = 0;
         if (!KVS) {
-            const long at = ((long)b * p.q_heads + head0) * pitch + row;
+            const long at = ((long)b * p.q_heads + head0) * p.plan.q_tiles * kTile + row;
             my_lse = p.lse[at];             // +inf behind the last query: its P is 0
             my_delta = p.delta[at];
             if (row < p.q_len) {
@@ -305,12 +339,8 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint32_t par = (uint32_t)c & 1u;
             const Chunk ch = chunk_at(c);
             const int col0 = ch.t * kTile + part * kCols;         // first streamed row of this thread's 32
-            const float4 *lse4 = nullptr, *delta4 = nullptr;
             uint32_t see = 0xffffffffu;
             if (KVS) {
-                const long at = ((long)b * p.q_heads + ch.head) * pitch + col0;
-                lse4 = reinterpret_cast<const float4*>(p.lse + at);
-                delta4 = reinterpret_cast<const float4*>(p.delta + at);
                 const int4 r = plan.q_tiles[ch.t];
                 if (r.z > r0 || r.w < min(r0 + kTile, p.kv_len)) {         // some query does not see all of these keys
                     const int i = col0 + lane, k0 = r0 + quad * 32;
@@ -336,146 +366,145 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 at_end = most <= -p.R || least >= p.R;
                 if (at_end) end_bias = bias_row[least >= p.R ? p.R : -p.R] * kLog2e;
             }
-            uint32_t pk[16], tk[MODE != kPlain ? 16 : 1];
+            uint32_t tk[MODE != kPlain ? 16 : 1], a[32];
             if (!warp_wait(s_full, par, &abort_flag)) goto done;
             tc_fence_after();
-            {
-                uint32_t a[32];
-                tmem_ld_32x32(t1, a);
-                float4 lq[KVS ? 8 : 1];
-                if (KVS) {
+            tmem_ld_32x32(t1, a);
+            tmem_ld_wait();
+            if (MODE != kPlain) {           // raw scores to the log2 domain
+                if (p.cap.out != 0.f) {
+                    const bool small = all_small<32>(p.cap, a);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) lq[i] = __ldg(lse4 + i);
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 z = make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+                        const float2 y = small ? cap_small(p.cap, z) : make_float2(cap_any(p.cap, z.x), cap_any(p.cap, z.y));
+                        const float2 t = __fmul2_rn(y, make_float2(p.cap.inv_out, p.cap.inv_out));
+                        const float2 slope = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
+                        // the cap's slope in fp16: 2^-11 of a factor that is rounded to 16 bits with its dS below
+                        tk[i] = pack2<false>(slope.x, slope.y);
+                        a[2 * i] = __float_as_uint(y.x);
+                        a[2 * i + 1] = __float_as_uint(y.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * p.scale_log2);
                 }
-                tmem_ld_wait();
+                if (p.R >= 0) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float2 l2;
-                    if (KVS) {
-                        const float4 v = lq[i >> 1];
-                        l2 = (i & 1) ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
-                    } else {
-                        l2 = make_float2(my_lse, my_lse);
-                    }
-                    float2 s2 = make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
-                    float2 y;
-                    if (MODE == kPlain) {
-                        y = __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), make_float2(-l2.x, -l2.y));
-                    } else {
-                        if (p.cap_in != 0.f) {
-                            float2 t;
-                            s2 = make_float2(capped(s2.x, p.cap_in, p.cap_out, &t.x), capped(s2.y, p.cap_in, p.cap_out, &t.y));
-                            // the cap's slope in fp16: 2^-12 of a factor that is rounded to 16 bits with its dS below
-                            tk[i] = pack2<false>(1.f - t.x * t.x, 1.f - t.y * t.y);
-                        } else {
-                            s2 = make_float2(s2.x * p.scale_log2, s2.y * p.scale_log2);
-                        }
-                        if (p.R >= 0) {
-                            if (at_end) {
-                                s2 = make_float2(s2.x + end_bias, s2.y + end_bias);
-                            } else {
-                                const int d0 = KVS ? pos0 - 2 * i : pos0 + 2 * i, d1 = KVS ? d0 - 1 : d0 + 1;
-                                s2.x += bias_row[max(-p.R, min(p.R, d0))] * kLog2e;
-                                s2.y += bias_row[max(-p.R, min(p.R, d1))] * kLog2e;
-                            }
-                        }
-                        y = make_float2(s2.x - l2.x, s2.y - l2.y);
-                    }
-                    float2 e = make_float2(exp2f(y.x), exp2f(y.y));
-                    if (!clean) {
-                        if (!(see >> (2 * i) & 1u)) e.x = 0.f;
-                        if (!(see >> (2 * i + 1) & 1u)) e.y = 0.f;
-                    }
-                    if (MODE == kGeneralDbias) {        // dS is summed before it is rounded: P stays in 32 bits
-                        a[2 * i] = __float_as_uint(e.x);
-                        a[2 * i + 1] = __float_as_uint(e.y);
-                    } else {
-                        pk[i] = pack2<BF16>(e.x, e.y);
+                    for (int i = 0; i < 32; ++i) {
+                        const int d = KVS ? pos0 - i : pos0 + i;
+                        const float add = at_end ? end_bias : bias_row[max(-p.R, min(p.R, d))] * kLog2e;
+                        a[i] = __float_as_uint(__uint_as_float(a[i]) + add);
                     }
                 }
-                // P stays in registers: T1 is released to the next chunk's scores right away
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready);
-
-                if (!warp_wait(dp_full, par, &abort_flag)) goto done;
-                tc_fence_after();
-                uint32_t g[32];
-                tmem_ld_32x32(t2, g);
-                float4 dq4[KVS ? 8 : 1];
-                if (KVS) {
+            }
+            // P in 32 bits over the scores
+            if (KVS && !warp_wait(b1_full(c % kRing1), (uint32_t)(c / kRing1) & 1u, &abort_flag)) goto done;       // has the copied lse: long complete
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dq4[i] = __ldg(delta4 + i);
-                }
-                tmem_ld_wait();
-                uint32_t dk[16];
+            for (int q = 0; q < 8; ++q) {
+                float4 l4 = make_float4(my_lse, my_lse, my_lse, my_lse);
+                if (KVS) lds4(sLse + ((c % kRing1) * kTile + part * kCols + 4 * q) * 4, l4);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float2 d2;
-                    if (KVS) {
-                        const float4 v = dq4[i >> 1];
-                        d2 = (i & 1) ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
-                    } else {
-                        d2 = make_float2(my_delta, my_delta);
-                    }
-                    const float2 pr = MODE == kGeneralDbias ? make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1])) : unpack2<BF16>(pk[i]);
-                    float2 ds = __fmul2_rn(pr, make_float2(__uint_as_float(g[2 * i]) - d2.x, __uint_as_float(g[2 * i + 1]) - d2.y));
-                    if (!clean) {           // dP of a key or a query that no run reaches may be anything
-                        if (!(see >> (2 * i) & 1u)) ds.x = 0.f;
-                        if (!(see >> (2 * i + 1) & 1u)) ds.y = 0.f;
-                    }
-                    if (MODE == kGeneralDbias) {
-                        g[2 * i] = __float_as_uint(ds.x);
-                        g[2 * i + 1] = __float_as_uint(ds.y);
-                    }
-                    if (MODE != kPlain && p.cap_in != 0.f) ds = __fmul2_rn(ds, unpack2<false>(tk[i]));
-                    // rounded to the operands' type, as the products take it: half a step of each dS
-                    dk[i] = pack2<BF16>(ds.x, ds.y);
+                for (int h = 0; h < 2; ++h) {
+                    const int i = 4 * q + 2 * h;
+                    const float2 s2 = make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+                    const float2 n2 = h ? make_float2(-l4.z, -l4.w) : make_float2(-l4.x, -l4.y);
+                    const float2 y = MODE == kPlain ? __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), n2) : __fadd2_rn(s2, n2);
+                    a[i] = __float_as_uint(exp2f(y.x));
+                    a[i + 1] = __float_as_uint(exp2f(y.y));
                 }
-                if (KVS) tmem_st_32x16(t2, pk);
-                tmem_st_32x16(t2 + 16, dk);
+            }
+            if (!clean) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (!(see >> i & 1u)) a[i] = 0u;
+            }
+            if (KVS) {          // rounded for the product only: half a step of the operands' type
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pk[i] = pack2<BF16>(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+                tmem_st_32x16(t1, pk);
                 tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ds_ready);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready);
 
-                if (MODE == kGeneralDbias) {
-                    const int corner = ch.t * kTile - (start + r0);         // distance of the tile's first key from its first query
-                    if (corner + kTile - 1 <= -p.R || corner - kTile + 1 >= p.R) {
-                        float s = 0.f;
+            const uint32_t t2c = KVS || !(c & 1) ? t2 : t2 + (kT3 - kT2);
+            if (!warp_wait(dp_full(c), KVS ? par : (uint32_t)(c >> 1) & 1u, &abort_flag)) goto done;
+            tc_fence_after();
+            if (KVS && !warp_wait(b2_full(c % kRing2), (uint32_t)(c / kRing2) & 1u, &abort_flag)) goto done;       // and delta
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s += __uint_as_float(g[i]);
-                        if (corner < 0) near_sum += s;
-                        else far_sum += s;
-                    } else {
-                        // Sums along the diagonals of the warp's 32 x 32 block: a partial sum moves down one row per column.  Slot
-                        // c - row + 31; what leaves the last row at column c is slot c, what is left at the end belongs to slots 62 - row.
-                        float* slots = scratch + ((n_diag & 1) * 16 + part * 4 + quad) * 64;
-                        float acc = 0.f;
+            for (int half = 0; half < 2; ++half) {
+                uint32_t g[16], dk[8];
+                tmem_ld_32x16(t2c + 16 * half, g);
+                tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float above = __shfl_up_sync(0xffffffffu, acc, 1);
-                            acc = (lane == 0 ? 0.f : above) + __uint_as_float(g[i]);
-                            if (lane == 31) slots[i] = acc;
+                for (int q = 0; q < 4; ++q) {
+                    float4 d4 = make_float4(my_delta, my_delta, my_delta, my_delta);
+                    if (KVS) lds4(sDelta + ((c % kRing2) * kTile + part * kCols + 16 * half + 4 * q) * 4, d4);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int i = 4 * q + 2 * h, k = 16 * half + i;
+                        const float2 n2 = h ? make_float2(-d4.z, -d4.w) : make_float2(-d4.x, -d4.y);
+                        float2 ds = __fmul2_rn(make_float2(__uint_as_float(a[k]), __uint_as_float(a[k + 1])),
+                                               __fadd2_rn(make_float2(__uint_as_float(g[i]), __uint_as_float(g[i + 1])), n2));
+                        if (!clean) {           // dP of a key or a query that no run reaches may be anything
+                            if (!(see >> k & 1u)) ds.x = 0.f;
+                            if (!(see >> (k + 1) & 1u)) ds.y = 0.f;
                         }
-                        if (lane < 31) slots[62 - lane] = acc;
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(diag_ready);
-                        if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
-                        // one diagonal of the tile a thread, its warps' shares in a fixed order
-                        const int x = (int)threadIdx.x - 64;
-                        if (x < 2 * kTile - 1) {
-                            const int d = x - (kTile - 1);
-                            float s = 0.f;
-                            for (int q = 0; q < 4; ++q)
-                                for (int k = 0; k < 4; ++k) {
-                                    const int slot = d - 32 * (k - q) + 31;
-                                    if (slot >= 0 && slot < 63) s += scratch[((n_diag & 1) * 16 + k * 4 + q) * 64 + slot];
-                                }
-                            diag[kDiagPad + p.R + corner + d] += s;
+                        if (MODE == kGeneralDbias) {
+                            a[k] = __float_as_uint(ds.x);
+                            a[k + 1] = __float_as_uint(ds.y);
                         }
-                        ++n_diag;
+                        if (MODE != kPlain && p.cap.out != 0.f) ds = __fmul2_rn(ds, unpack2<false>(tk[k >> 1]));
+                        // rounded to the operands' type, as the products take it: half a step of each dS
+                        dk[i >> 1] = pack2<BF16>(ds.x, ds.y);
                     }
+                }
+                tmem_st_32x8(t2c + 8 * half, dk);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_ready);
+
+            if (MODE == kGeneralDbias) {
+                const int corner = ch.t * kTile - (start + r0);         // distance of the tile's first key from its first query
+                if (corner + kTile - 1 <= -p.R || corner - kTile + 1 >= p.R) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s += __uint_as_float(a[i]);
+                    if (corner < 0) near_sum += s;
+                    else far_sum += s;
+                } else {
+                    // Sums along the diagonals of the warp's 32 x 32 block: a partial sum moves down one row per column.  Slot
+                    // c - row + 31; what leaves the last row at column c is slot c, what is left at the end belongs to slots 62 - row.
+                    float* slots = scratch + ((n_diag & 1) * 16 + part * 4 + quad) * 64;
+                    float acc = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float above = __shfl_up_sync(0xffffffffu, acc, 1);
+                        acc = (lane == 0 ? 0.f : above) + __uint_as_float(a[i]);
+                        if (lane == 31) slots[i] = acc;
+                    }
+                    if (lane < 31) slots[62 - lane] = acc;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(diag_ready);
+                    if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+                    // one diagonal of the tile a thread, its warps' shares in a fixed order
+                    const int x = (int)threadIdx.x - 64;
+                    if (x < 2 * kTile - 1) {
+                        const int d = x - (kTile - 1);
+                        float s = 0.f;
+                        for (int q = 0; q < 4; ++q)
+                            for (int k = 0; k < 4; ++k) {
+                                const int slot = d - 32 * (k - q) + 31;
+                                if (slot >= 0 && slot < 63) s += scratch[((n_diag & 1) * 16 + k * 4 + q) * 64 + slot];
+                            }
+                        diag[kDiagPad + p.R + corner + d] += s;
+                    }
+                    ++n_diag;
                 }
             }
         }
@@ -690,8 +719,7 @@ extern "C" int tt_attn_ranges_bwd(const tt_ranges_args* a, void* stream) {
     p.R = a->max_distance;
     p.scale = a->scale;
     p.scale_log2 = a->scale * kLog2e;
-    p.cap_in = a->softcap > 0.f ? 2.f * a->scale / a->softcap * kLog2e : 0.f;
-    p.cap_out = a->softcap * kLog2e;
+    p.cap = make_cap(a->scale, a->softcap);
     p.status = a->status;
     cudaStream_t st = (cudaStream_t)stream;
     const bool bf = a->dtype == TT_BF16;

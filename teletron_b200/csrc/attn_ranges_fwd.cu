@@ -35,7 +35,8 @@ struct FwdParams {
     float *out32, *lse;
     const float* bias;
     int q_len, q_heads, group, pair_heads, R;
-    float scale_log2, cap_in, cap_out;      // cap_in = 2 scale / cap * log2(e), cap_out = cap * log2(e); 0: no cap
+    float scale_log2;
+    Cap cap;
     int* status;
 };
 
@@ -295,11 +296,17 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             for (int c = 0; c < kTile / 32; ++c) tmem_ld_32x32(tS + c * 32, r + c * 32);
             tmem_ld_wait();
             if (GEN) {
-                if (p.cap_in != 0.f) {
+                if (p.cap.out != 0.f) {
+                    if (all_small<kTile>(p.cap, r)) {
 #pragma unroll
-                    for (int i = 0; i < kTile; ++i) {
-                        float unused;
-                        r[i] = __float_as_uint(capped(__uint_as_float(r[i]), p.cap_in, p.cap_out, &unused));
+                        for (int i = 0; i < kTile; i += 2) {
+                            const float2 y = cap_small(p.cap, make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+                            r[i] = __float_as_uint(y.x);
+                            r[i + 1] = __float_as_uint(y.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i) r[i] = __float_as_uint(cap_any(p.cap, __uint_as_float(r[i])));
                     }
                 } else {
 #pragma unroll
@@ -483,8 +490,7 @@ extern "C" int tt_attn_ranges_fwd(const tt_ranges_args* a, void* stream) {
     p.pair_heads = p.group % 2 == 0;
     p.R = a->max_distance;
     p.scale_log2 = a->scale * kLog2e;
-    p.cap_in = a->softcap > 0.f ? 2.f * a->scale / a->softcap * kLog2e : 0.f;
-    p.cap_out = a->softcap * kLog2e;
+    p.cap = make_cap(a->scale, a->softcap);
     p.status = a->status;
     cudaStream_t st = (cudaStream_t)stream;
     const bool gen = a->softcap > 0.f || a->max_distance >= 0 || !(a->scale > 0.f) || a->out32 != nullptr;
