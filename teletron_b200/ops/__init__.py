@@ -21,6 +21,8 @@ import os
 import torch
 
 from . import reference
+from . import attn_ranges
+from . import rope
 from . import optim  # noqa: F401
 from .attn_ranges import KeyRanges, key_ranges  # noqa: F401
 from .rope import Rotary, rotary_frequencies  # noqa: F401
@@ -131,7 +133,6 @@ _ROTARY_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _rotary_kernel_ok(q) -> bool:
-    from . import rope
     if not _use_cuda(q, dtypes=_ROTARY_DTYPES):
         return False
     if rope.supported(q):
@@ -147,19 +148,19 @@ def rotary(q, k, positions, freqs):
     ``positions``: int32 or int64, ``[tokens]`` or ``[batch, tokens]``, with several axes ``[axes, tokens]`` or ``[batch, axes, tokens]``;
     ``freqs``: what :func:`rotary_frequencies` returns.  ``k`` may be None.  Returns head-major ``(q, k)`` of the same type; the gradients
     come in the order of the inputs.  bf16, fp16 and fp32."""
-    from . import rope
-    p = rope.check_arguments(q, k, positions, freqs)
-    return rope.rotary(q, k, p, freqs) if _rotary_kernel_ok(q) else reference.rotary(q, k, p, freqs)
+    stride = rope.check_arguments(q, k, positions, freqs)
+    if _rotary_kernel_ok(q):
+        return rope.rotary(q, k, positions, stride, freqs)
+    return reference.rotary(q, k, rope.by_axis(positions, freqs.num_axes), freqs)
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps: float = 1e-6):
     """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``, statistics in fp32), then :func:`rotary`, rounded once."""
-    from . import rope
-    p = rope.check_arguments(q, k, positions, freqs)
+    stride = rope.check_arguments(q, k, positions, freqs)
     rope.check_weights(q, k, q_weight, k_weight)
     if _rotary_kernel_ok(q):
-        return rope.qk_norm_rotary(q, k, q_weight, k_weight, p, freqs, eps)
-    return reference.qk_norm_rotary(q, k, q_weight, k_weight, p, freqs, eps)
+        return rope.qk_norm_rotary(q, k, q_weight, k_weight, positions, stride, freqs, eps)
+    return reference.qk_norm_rotary(q, k, q_weight, k_weight, rope.by_axis(positions, freqs.num_axes), freqs, eps)
 
 
 def linear(x, weight, bias=None, activation=None):
@@ -195,7 +196,6 @@ def masked_attention(q, k, v, ranges, scale=None, softcap=None, distance_bias=No
 
     Keys, values, queries and output gradients that no run reaches (padding) may hold anything; those that some query sees have to be finite,
     as a query's weights of 0 still multiply what its neighbours see.  Kernels: bf16 and fp16, head_dim 64 and 128, R up to 1024."""
-    from . import attn_ranges
     attn_ranges.check_arguments(q, k, v, ranges, scale, softcap, distance_bias)
     if _use_cuda(q, dtypes=(torch.bfloat16, torch.float16)):
         if attn_ranges.supported(q, k, v, ranges, distance_bias):

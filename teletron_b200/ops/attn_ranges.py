@@ -161,13 +161,15 @@ def check_arguments(q, k, v, ranges, scale, softcap, distance_bias) -> None:
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"expected [batch, heads, tokens, head_dim], got q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     B, hq, n, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.shape[1] == 0 or hq % k.shape[1]:
+    Bk, hk, m, Dk = k.shape
+    dtype, device = q.dtype, q.get_device()
+    if k.shape != v.shape or Bk != B or Dk != D or hk == 0 or hq % hk:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    if not q.dtype.is_floating_point or k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+    if not dtype.is_floating_point or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != device or v.get_device() != device:
         raise ValueError(f"q {q.dtype} on {q.device}, k {k.dtype} on {k.device}, v {v.dtype} on {v.device} do not belong together")
-    if (ranges.batch, ranges.q_len, ranges.kv_len) != (B, n, k.shape[2]):
-        raise ValueError(f"runs of {ranges.batch} x {ranges.q_len} queries and {ranges.kv_len} keys for {B} x {n} queries and {k.shape[2]} keys")
-    if ranges.device != q.device:
+    if ranges.batch != B or ranges.q_len != n or ranges.kv_len != m:
+        raise ValueError(f"runs of {ranges.batch} x {ranges.q_len} queries and {ranges.kv_len} keys for {B} x {n} queries and {m} keys")
+    if ranges.first.get_device() != device:
         raise ValueError(f"runs on {ranges.device}, queries on {q.device}")
     if scale is not None and not math.isfinite(scale):
         raise ValueError(f"scale: {scale} is not finite")
@@ -176,7 +178,7 @@ def check_arguments(q, k, v, ranges, scale, softcap, distance_bias) -> None:
     if distance_bias is not None:
         if distance_bias.dim() != 2 or distance_bias.shape[0] != hq or distance_bias.shape[1] % 2 == 0:
             raise ValueError(f"distance_bias: expected [{hq}, 2 R + 1], got {tuple(distance_bias.shape)}")
-        if distance_bias.dtype != torch.float32 or distance_bias.device != q.device:
+        if distance_bias.dtype is not torch.float32 or distance_bias.get_device() != device:
             raise ValueError(f"distance_bias: expected float32 on {q.device}, got {distance_bias.dtype} on {distance_bias.device}")
 
 
@@ -188,13 +190,20 @@ def supported(q, k, v, ranges, distance_bias) -> bool:
 
 # ------------------------------------------------------------------------------------------------ native calls
 
+_HEAD = struct.Struct("@l iiii iiii PPP 9l PPP PP ff")           # everything that the forward kernel reads but the status word
+_TAIL = struct.Struct("@PP PPP 9l PP P")
 _ARGS = struct.Struct("@l iiii iiii PPP 9l PPP PP ff PP PPP 9l PP P")
-_NONE9 = (0,) * 9
+_NO_BACKWARD = bytes(_TAIL.size - 8)
+_STATUS = struct.Struct("@P")
 
 
 def _rows(t):
     """Operand that the copies can address: contiguous rows at 16-byte boundaries, steps of any size above 0."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
+    sb, sh, st, sd = t.stride()
+    if sd == 1 and not t.data_ptr() & 15 and not (sb | sh | st) & 7 and sb > 0 and sh > 0 and st > 0:
+        return t
+    B, H, S, _ = t.shape        # a dimension of one is never stepped over
+    if sd == 1 and not t.data_ptr() & 15 and all(n == 1 or (s > 0 and not s & 7) for n, s in ((B, sb), (H, sh), (S, st))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -202,32 +211,49 @@ def _rows(t):
 def _like(x):
     """A gradient in ``x``'s order of heads and tokens."""
     B, H, S, D = x.shape
-    if x.stride(1) < x.stride(2):
-        return torch.empty(B, S, H, D, dtype=x.dtype, device=x.device).transpose(1, 2)
-    return torch.empty(B, H, S, D, dtype=x.dtype, device=x.device)
+    return x.new_empty((B, S, H, D)).transpose(1, 2) if x.stride(1) < x.stride(2) else x.new_empty((B, H, S, D))
 
 
-def _native(fn, q, k, v, ranges, out, out32, lse, scale, softcap, bias, grads=None):
-    """``grads``: ``(dout, delta, dq, dk, dv, dbias, partials)``."""
+def _pack(q, k, v, ranges, out, out32, lse, scale, softcap, bias):
     B, hq, n, D = q.shape
-    dout, delta, dq, dk, dv, dbias, partials = grads or (None,) * 7
-    address = lambda t: 0 if t is None else t.data_ptr()
-    packed = _ARGS.pack(_ARGS.size, B, hq, k.shape[1], n, k.shape[2], D, _DTYPES[q.dtype], -1 if bias is None else (bias.shape[1] - 1) // 2,
-                        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                        out.data_ptr(), address(out32), lse.data_ptr(), ranges.plan.data_ptr(), address(bias),
-                        scale, softcap, address(dout), address(delta), address(dq), address(dk), address(dv),
-                        *(_NONE9 if grads is None else (*dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3])),
-                        address(dbias), address(partials), status_tensor(q.device).data_ptr())
-    call(fn, packed, stream())
+    return _HEAD.pack(_ARGS.size, B, hq, k.shape[1], n, k.shape[2], D, _DTYPES[q.dtype], -1 if bias is None else bias.shape[1] >> 1,
+                      q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                      out.data_ptr(), 0 if out32 is None else out32.data_ptr(), lse.data_ptr(), ranges.plan.data_ptr(),
+                      0 if bias is None else bias.data_ptr(), scale, softcap)
 
 
 def _forward(q, k, v, ranges, scale, softcap, bias, wide):
     B, hq, n, D = q.shape
-    out = torch.empty(B, n, hq * D, dtype=q.dtype, device=q.device)
-    out32 = torch.empty(B, n, hq * D, dtype=torch.float32, device=q.device) if wide else None
-    lse = torch.empty(B, hq, (n + TILE - 1) // TILE * TILE, dtype=torch.float32, device=q.device)
-    _native("tt_attn_ranges_fwd", q, k, v, ranges, out, out32, lse, scale, softcap, bias)
+    out = q.new_empty((B, n, hq * D))
+    out32 = q.new_empty((B, n, hq * D), dtype=torch.float32) if wide else None
+    lse = q.new_empty((B, hq, (n + TILE - 1) // TILE * TILE), dtype=torch.float32)
+    call("tt_attn_ranges_fwd", _pack(q, k, v, ranges, out, out32, lse, scale, softcap, bias) + _NO_BACKWARD + _STATUS.pack(status_tensor(q.device).data_ptr()),
+         stream())
     return out, out32, lse
+
+
+def _backward(ctx, dout):
+    q, k, v, bias, out, lse, _ = ctx.saved_tensors
+    B, hq, n, D = q.shape
+    with on_device(q):
+        dout = dout.contiguous()
+        if dout.data_ptr() & 15:
+            dout = dout.clone()
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        delta = lse.new_empty(lse.shape)
+        dbias = partials = None
+        if ctx.wide:
+            dbias = bias.new_empty(bias.shape)
+            partials = lse.new_empty((B * hq * (lse.shape[2] // TILE) * bias.shape[1],))
+        call("tt_attn_ranges_bwd", _pack(q, k, v, ctx.ranges, out, out if ctx.wide else None, lse, ctx.scale, ctx.softcap, bias)
+             + _TAIL.pack(dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dq.stride()[:3], *dk.stride()[:3],
+                          *dv.stride()[:3], 0 if dbias is None else dbias.data_ptr(), 0 if partials is None else partials.data_ptr(),
+                          status_tensor(q.device).data_ptr()), stream())
+    a, b, c, d = ctx.needs_input_grad[:4]
+    return dq if a else None, dk if b else None, dv if c else None, dbias if d else None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _MaskedAttention(torch.autograd.Function):
@@ -243,22 +269,9 @@ class _MaskedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, bias, out, lse, _ = ctx.saved_tensors
-        B, hq, n, D = q.shape
-        with on_device(q):
-            dout = dout.contiguous()
-            if dout.data_ptr() % 16:
-                dout = dout.clone()
-            dq, dk, dv = _like(q), _like(k), _like(v)
-            dbias = partials = None
-            if ctx.wide:
-                dbias = torch.empty_like(bias)
-                partials = torch.empty(B * hq * (lse.shape[2] // TILE) * bias.shape[1], dtype=torch.float32, device=q.device)
-            _native("tt_attn_ranges_bwd", q, k, v, ctx.ranges, out, out if ctx.wide else None, lse, ctx.scale, ctx.softcap, bias,
-                    (dout, torch.empty_like(lse), dq, dk, dv, dbias, partials))
-        return tuple(t if need else None for t, need in zip((dq, dk, dv, dbias), ctx.needs_input_grad)) + (None, None, None)
+        # the wrapper, which a second derivative would need to fail in, costs the host 5 us of a first one
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dout)
 
 
 def masked_attention(q, k, v, ranges, scale, softcap, distance_bias):

@@ -37,11 +37,10 @@ class Rotary:
     num_axes: int
     amplitude: float
     interleaved: bool
+    dim: int = dataclasses.field(init=False)        # elements of a head that are rotated
 
-    @property
-    def dim(self) -> int:
-        """Elements of a head that are rotated."""
-        return 2 * self.inv_freq.shape[0]
+    def __post_init__(self):
+        object.__setattr__(self, "dim", 2 * self.inv_freq.shape[0])
 
     def to(self, device) -> "Rotary":
         move = lambda t: None if t is None else t.to(device)
@@ -117,40 +116,53 @@ def rotary_frequencies(dim: int, theta: float = 10000.0, *, axes: Optional[Seque
     return rot if device is None else rot.to(device)
 
 
-def check_arguments(q, k, positions, rotary: Rotary) -> torch.Tensor:
-    """Raises ``ValueError`` where the operands do not belong together; returns the positions as ``[1 or batch, axes, tokens]``."""
+def check_arguments(q, k, positions, rotary: Rotary) -> Tuple[int, int, int]:
+    """Raises ``ValueError`` where the operands do not belong together; returns the positions' strides over samples, axes and tokens.
+    (A call for a few tokens takes the host longer than the device, so what is right is found to be so with few look-ups.)"""
     if not isinstance(rotary, Rotary):
         raise ValueError("rotary: expected the frequencies that rotary_frequencies returns")
-    for t, n in ((q, "q"), (k, "k")):
-        if t is None and n == "k":
-            continue
-        if t.dim() != 4:
-            raise ValueError(f"{n}: expected [batch, heads, tokens, head_dim], got {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.device != q.device or (t.shape[0], t.shape[2], t.shape[3]) != (q.shape[0], q.shape[2], q.shape[3]):
-            raise ValueError(f"q {tuple(q.shape)} {q.dtype} on {q.device} and k {tuple(t.shape)} {t.dtype} on {t.device} do not belong together")
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f"expected [batch, heads, tokens, head_dim], got q {tuple(q.shape)}" + ("" if k is None else f", k {tuple(k.shape)}"))
+    B, _, S, D = q.shape
+    device = q.get_device()
+    if k is not None:
+        Bk, _, Sk, Dk = k.shape
+        if Bk != B or Sk != S or Dk != D or k.dtype is not q.dtype or k.get_device() != device:
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} on {q.device} and k {tuple(k.shape)} {k.dtype} on {k.device} do not belong together")
     if not q.dtype.is_floating_point:
         raise ValueError(f"q: expected a floating type, got {q.dtype}")
-    if rotary.dim > q.shape[3]:
-        raise ValueError(f"{rotary.dim} elements to rotate in heads of {q.shape[3]}")
-    if rotary.inv_freq.device != q.device:
+    if rotary.dim > D:
+        raise ValueError(f"{rotary.dim} elements to rotate in heads of {D}")
+    if rotary.inv_freq.get_device() != device:
         raise ValueError(f"rotary frequencies on {rotary.inv_freq.device}, queries on {q.device}")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+    if (positions.dtype is not torch.int32 and positions.dtype is not torch.int64) or positions.get_device() != device:
         raise ValueError(f"positions: expected int32 or int64 on {q.device}, got {positions.dtype} on {positions.device}")
-    B, S, A = q.shape[0], q.shape[2], rotary.num_axes
-    p = positions
-    if A == 1 and p.dim() in (1, 2):
-        p = p.view(1, 1, -1) if p.dim() == 1 else p[:, None]
-    elif A > 1 and p.dim() == 2:
-        p = p[None]
-    if p.dim() != 3 or p.shape[0] not in (1, B) or p.shape[1:] != (A, S):
-        want = "[tokens] or [batch, tokens]" if A == 1 else f"[{A}, tokens] or [batch, {A}, tokens]"
-        raise ValueError(f"positions: expected {want} for {S} tokens of {B} samples, got {tuple(positions.shape)}")
-    return p
+    A, shape, stride = rotary.num_axes, tuple(positions.shape), positions.stride()
+    if A == 1:
+        if shape == (S,):
+            return 0, 0, stride[0]
+        if shape == (B, S) or shape == (1, S):
+            return (stride[0] if shape[0] > 1 else 0), 0, stride[1]
+    if shape == (A, S):
+        return 0, stride[0], stride[1]
+    if shape == (B, A, S) or shape == (1, A, S):
+        return (stride[0] if shape[0] > 1 else 0), stride[1], stride[2]
+    want = "[tokens] or [batch, tokens]" if A == 1 else f"[{A}, tokens] or [batch, {A}, tokens]"
+    raise ValueError(f"positions: expected {want} for {S} tokens of {B} samples, got {shape}")
+
+
+def by_axis(positions, num_axes: int):
+    """Positions that :func:`check_arguments` has taken as ``[1 or batch, axes, tokens]``, for the plain path."""
+    if positions.dim() == 3:
+        return positions
+    if num_axes > 1:
+        return positions[None]
+    return positions[None, None] if positions.dim() == 1 else positions[:, None]
 
 
 def check_weights(q, k, q_weight, k_weight) -> None:
     for x, w, n in ((q, q_weight, "q_weight"), (k, k_weight, "k_weight")):
-        if w.shape != (x.shape[3],) or w.dtype != x.dtype or w.device != x.device:
+        if w.dim() != 1 or w.shape[0] != x.shape[3] or w.dtype is not x.dtype or w.get_device() != x.get_device():
             raise ValueError(f"{n}: expected [{x.shape[3]}] {x.dtype} on {x.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")
 
 
@@ -160,8 +172,9 @@ def supported(q) -> bool:
 
 # ------------------------------------------------------------------------------------------------ native calls
 
+_HEAD = struct.Struct("@lll iiii iiii PP 6l PP 6l P 3l PP ff PP")        # everything that the forward kernels read
 _ARGS = struct.Struct("@lll iiii iiii PP 6l PP 6l P 3l PP ff PP PP 6l PP P l")
-_NONE3 = (0, 0, 0)
+_NO_BACKWARD = bytes(_ARGS.size - _HEAD.size)
 
 
 def _rows(t):
@@ -169,124 +182,137 @@ def _rows(t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
-def _strides(t):
-    return _NONE3 if t is None else t.stride()[:3]
+def _pack(q, k, out_q, out_k, positions, pos_stride, rotary, transpose, eps, q_weight, k_weight):
+    """The arguments that the forward kernels read; ``q`` or ``k`` may be None."""
+    some = k if q is None else q
+    B, _, S, D = some.shape
+    hq = hk = 0
+    pq = pk = oq = ok = 0
+    sq = sk = tq = tk = (0, 0, 0, 0)
+    if q is not None:
+        hq, pq, oq, sq, tq = q.shape[1], q.data_ptr(), out_q.data_ptr(), q.stride(), out_q.stride()
+    if k is not None:
+        hk, pk, ok, sk, tk = k.shape[1], k.data_ptr(), out_k.data_ptr(), k.stride(), out_k.stride()
+    return _HEAD.pack(_ARGS.size, B, S, hq, hk, D, rotary.dim >> 1, _DTYPES[some.dtype], rotary.interleaved, transpose, positions.dtype is torch.int64,
+                      pq, pk, sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], oq, ok, tq[0], tq[1], tq[2], tk[0], tk[1], tk[2], positions.data_ptr(),
+                      *pos_stride, rotary.half_turns.data_ptr(), 0 if rotary.axis is None else rotary.axis.data_ptr(), rotary.amplitude, eps,
+                      0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr())
 
 
-def _address(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _native(fn, q, k, out_q, out_k, positions, rotary, *, transpose=False, eps=0.0, weights=(None, None), grads=(None, None), dweights=(None, None),
-            partials=None):
-    B, _, S, D = q.shape if q is not None else k.shape
-    dtype = (q if q is not None else k).dtype
-    packed = _ARGS.pack(
-        _ARGS.size, B, S, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], D, rotary.dim // 2,
-        _DTYPES[dtype], rotary.interleaved, transpose, positions.dtype == torch.int64,
-        _address(q), _address(k), *_strides(q), *_strides(k), _address(out_q), _address(out_k), *_strides(out_q), *_strides(out_k),
-        positions.data_ptr(), 0 if positions.shape[0] == 1 else positions.stride(0), positions.stride(1), positions.stride(2),
-        rotary.half_turns.data_ptr(), _address(rotary.axis), rotary.amplitude, eps, _address(weights[0]), _address(weights[1]),
-        _address(grads[0]), _address(grads[1]), *_strides(grads[0]), *_strides(grads[1]), _address(dweights[0]), _address(dweights[1]),
-        _address(partials), 0 if partials is None else partials.numel())
-    if fn is None:
-        return packed
-    call(fn, packed, stream())
-
-
-def _head_major(t):
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def _like(x):
-    """An output in ``x``'s order of heads and tokens, so that the gradient of a token-major projection needs no transposition."""
+def _ordered(x, token_major: bool):
+    """An empty tensor of ``x``'s shape in the given order of heads and tokens: the gradient of a token-major projection's view then needs
+    no transposition."""
     B, H, S, D = x.shape
-    if x.stride(1) < x.stride(2):
-        return torch.empty(B, S, H, D, dtype=x.dtype, device=x.device).transpose(1, 2)
-    return torch.empty(B, H, S, D, dtype=x.dtype, device=x.device)
+    return x.new_empty((B, S, H, D)).transpose(1, 2) if token_major else x.new_empty((B, H, S, D))
 
 
-def _rotate(q, k, positions, rotary, transpose, make):
-    """``k`` None: queries only."""
-    ins = [None if t is None else _rows(t) for t in (q, k)]
-    outs = [None if t is None else make(t) for t in (q, k)]
-    if any(t is not None and t.numel() for t in ins):
-        _native("tt_rotary", *[t if t is not None and t.numel() else None for t in ins], *outs, positions, rotary, transpose=transpose)
-    return outs
+def _token_major(x) -> bool:
+    return x.stride(1) < x.stride(2)
+
+
+def _forward(q, k, positions, pos_stride, freqs):
+    q = _rows(q)
+    out_q, out_k = q.new_empty(q.shape), None
+    if k is not None:
+        k = _rows(k)
+        out_k = k.new_empty(k.shape)
+    some_q, some_k = q.numel() > 0, k is not None and k.numel() > 0
+    if some_q or some_k:
+        call("tt_rotary", _pack(q if some_q else None, k if some_k else None, out_q, out_k, positions, pos_stride, freqs, False, 0.0, None, None)
+             + _NO_BACKWARD, stream())
+    return out_q, out_k
+
+
+def _rotary_backward(ctx, gq, gk=None):
+    positions, = ctx.saved_tensors
+    grads = []
+    for g, need, order in zip((gq, gk), ctx.needs_input_grad, ctx.token_major):
+        grads.append((_rows(g), _ordered(g, order)) if need and g is not None else (None, None))
+    (gq, dq), (gk, dk) = grads
+    some_q, some_k = gq is not None and gq.numel() > 0, gk is not None and gk.numel() > 0
+    if some_q or some_k:
+        with on_device(positions):
+            call("tt_rotary", _pack(gq if some_q else None, gk if some_k else None, dq, dk, positions, ctx.pos_stride, ctx.freqs, True, 0.0, None, None)
+                 + _NO_BACKWARD, stream())
+    return dq, dk, None, None, None
+
+
+_rotary_backward_once = once_differentiable(_rotary_backward)
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, rotary):
-        ctx.rotary = rotary
+    def forward(ctx, q, k, positions, pos_stride, freqs):
+        ctx.freqs, ctx.pos_stride = freqs, pos_stride
         ctx.save_for_backward(positions)
-        ctx.token_major = [t is not None and t.stride(1) < t.stride(2) for t in (q, k)]
-        out = _rotate(q, k, positions, rotary, False, _head_major)
-        return out[0] if k is None else tuple(out)
+        ctx.token_major = (_token_major(q), k is not None and _token_major(k))
+        out = _forward(q, k, positions, pos_stride, freqs)
+        return out[0] if k is None else out
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk=None):
-        positions, = ctx.saved_tensors
-        grads = [g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad)]
-        order = iter([t for t, g in zip(ctx.token_major, grads) if g is not None])
-
-        def make(g):
-            B, H, S, D = g.shape
-            if next(order):
-                return torch.empty(B, S, H, D, dtype=g.dtype, device=g.device).transpose(1, 2)
-            return _head_major(g)
-
-        if all(g is None for g in grads):
-            return None, None, None, None
-        with on_device(positions):
-            dq, dk = _rotate(*grads, positions, ctx.rotary, True, make)
-        return dq, dk, None, None
+    def backward(ctx, *grads):
+        # the wrapper, which a second derivative would need to fail in, costs the host 5 us of a first one
+        return (_rotary_backward_once if torch.is_grad_enabled() else _rotary_backward)(ctx, *grads)
 
 
-def rotary(q, k, positions, freqs):
+def rotary(q, k, positions, pos_stride, freqs):
     with on_device(q):
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            out = _Rotary.apply(q, k, positions, freqs)
+            out = _Rotary.apply(q, k, positions, pos_stride, freqs)
             return (out, None) if k is None else out
-        return tuple(_rotate(q, k, positions, freqs, False, _head_major))
+        return _forward(q, k, positions, pos_stride, freqs)
+
+
+def _norm_forward(q, k, q_weight, k_weight, positions, pos_stride, freqs, eps):
+    out_q, out_k = q.new_empty(q.shape), k.new_empty(k.shape)
+    some_q, some_k = q.numel() > 0, k.numel() > 0
+    if some_q or some_k:
+        call("tt_norm_rotary_fwd", _pack(q if some_q else None, k if some_k else None, out_q, out_k, positions, pos_stride, freqs, False, eps, q_weight,
+                                         k_weight) + _NO_BACKWARD, stream())
+    return out_q, out_k
+
+
+_TAIL = struct.Struct("@PP 6l PP P l")
+
+
+def _norm_backward(ctx, gq, gk):
+    q, k, q_weight, k_weight, positions = ctx.saved_tensors
+    with on_device(q):
+        gq, gk = _rows(gq), _rows(gk)
+        dq, dk = _ordered(q, _token_major(q)), _ordered(k, _token_major(k))
+        dqw, dkw = q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
+        some_q, some_k = q.numel() > 0, k.numel() > 0
+        for some, dw in ((some_q, dqw), (some_k, dkw)):
+            if not some:
+                dw.zero_()
+        if some_q or some_k:
+            head = _pack(q if some_q else None, k if some_k else None, dq, dk, positions, ctx.pos_stride, ctx.freqs, False, ctx.eps, q_weight, k_weight)
+            size = _lib.lib().tt_rotary_partial_floats(head + _NO_BACKWARD)
+            partials = q.new_empty((max(size, 1),), dtype=torch.float32)
+            call("tt_norm_rotary_bwd", head + _TAIL.pack(gq.data_ptr(), gk.data_ptr(), *gq.stride()[:3], *gk.stride()[:3], dqw.data_ptr(), dkw.data_ptr(),
+                                                         partials.data_ptr(), size), stream())
+    a, b, c, d = ctx.needs_input_grad[:4]
+    return dq if a else None, dk if b else None, dqw if c else None, dkw if d else None, None, None, None, None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
 
 
 class _NormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, freqs, eps):
-        q, k, q_weight, k_weight = _rows(q), _rows(k), q_weight.contiguous(), k_weight.contiguous()
-        out = [_head_major(q), _head_major(k)]
-        if out[0].numel() or out[1].numel():
-            _native("tt_norm_rotary_fwd", *[t if t.numel() else None for t in (q, k)], *out, positions, freqs, eps=eps, weights=(q_weight, k_weight))
+    def forward(ctx, q, k, q_weight, k_weight, positions, pos_stride, freqs, eps):
         ctx.save_for_backward(q, k, q_weight, k_weight, positions)
-        ctx.freqs, ctx.eps = freqs, eps
-        return tuple(out)
+        ctx.pos_stride, ctx.freqs, ctx.eps = pos_stride, freqs, eps
+        return _norm_forward(q, k, q_weight, k_weight, positions, pos_stride, freqs, eps)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, positions = ctx.saved_tensors
-        with on_device(q):
-            gq, gk = _rows(gq), _rows(gk)
-            dq, dk = _like(q), _like(k)
-            dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
-            ins, outs, grads, weights, dws = [], [], [], [], []
-            for x, dx, g, w, dw in ((q, dq, gq, q_weight, dqw), (k, dk, gk, k_weight, dkw)):
-                some = x.numel() > 0
-                if not some:
-                    dw.zero_()
-                for into, t in zip((ins, outs, grads, weights, dws), (x, dx, g, w, dw)):
-                    into.append(t if some else None)
-            if ins[0] is not None or ins[1] is not None:
-                kw = dict(eps=ctx.eps, weights=weights, grads=grads, dweights=dws)
-                n = _lib.lib().tt_rotary_partial_floats(_native(None, *ins, *outs, positions, ctx.freqs, **kw))
-                partials = torch.empty(max(n, 1), dtype=torch.float32, device=q.device)
-                _native("tt_norm_rotary_bwd", *ins, *outs, positions, ctx.freqs, partials=partials, **kw)
-        need = ctx.needs_input_grad
-        return tuple(t if n else None for t, n in zip((dq, dk, dqw, dkw), need)) + (None, None, None)
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, gq, gk)
 
 
-def qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps):
+def qk_norm_rotary(q, k, q_weight, k_weight, positions, pos_stride, freqs, eps):
     with on_device(q):
-        return _NormRotary.apply(q, k, q_weight, k_weight, positions, freqs, float(eps))
+        q, k, q_weight, k_weight = _rows(q), _rows(k), q_weight.contiguous(), k_weight.contiguous()
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+            return _NormRotary.apply(q, k, q_weight, k_weight, positions, pos_stride, freqs, float(eps))
+        return _norm_forward(q, k, q_weight, k_weight, positions, pos_stride, freqs, float(eps))
