@@ -139,3 +139,6 @@ template <int N> __device__ __forceinline__ bool all_small(const Cap& k, const u
 int tt_make_tmap_bhsd(CUtensorMap* out, const void* base, int batch, int heads, int tokens, int head_dim, const long* stride, int box_rows);
 // validates what every entry point needs; fills in nothing
 int tt_ranges_check(const tt_ranges_args* a);
+// few queries (attn_ranges_few.cu)
+bool tt_ranges_few_rows(const tt_ranges_args& a);
+int tt_attn_ranges_few(const tt_ranges_args& a, cudaStream_t st);

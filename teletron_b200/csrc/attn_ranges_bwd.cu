@@ -449,15 +449,17 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         const float2 n2 = h ? make_float2(-d4.z, -d4.w) : make_float2(-d4.x, -d4.y);
                         float2 ds = __fmul2_rn(make_float2(__uint_as_float(a[k]), __uint_as_float(a[k + 1])),
                                                __fadd2_rn(make_float2(__uint_as_float(g[i]), __uint_as_float(g[i + 1])), n2));
-                        if (!clean) {           // dP of a key or a query that no run reaches may be anything
-                            if (!(see >> k & 1u)) ds.x = 0.f;
-                            if (!(see >> (k + 1) & 1u)) ds.y = 0.f;
+                        float2 slope = make_float2(1.f, 1.f);
+                        if (MODE != kPlain && p.cap.out != 0.f) slope = unpack2<false>(tk[k >> 1]);
+                        if (!clean) {           // dP and the slope of a key or a query that no run reaches may be anything
+                            if (!(see >> k & 1u)) ds.x = slope.x = 0.f;
+                            if (!(see >> (k + 1) & 1u)) ds.y = slope.y = 0.f;
                         }
                         if (MODE == kGeneralDbias) {
                             a[k] = __float_as_uint(ds.x);
                             a[k + 1] = __float_as_uint(ds.y);
                         }
-                        if (MODE != kPlain && p.cap.out != 0.f) ds = __fmul2_rn(ds, unpack2<false>(tk[k >> 1]));
+                        if (MODE != kPlain) ds = __fmul2_rn(ds, slope);
                         // rounded to the operands' type, as the products take it: half a step of each dS
                         dk[i >> 1] = pack2<BF16>(ds.x, ds.y);
                     }

@@ -477,6 +477,7 @@ int pick(const tt_ranges_args& a, const FwdParams& p, int mode, int dev, cudaStr
 extern "C" int tt_attn_ranges_fwd(const tt_ranges_args* a, void* stream) {
     int rc = tt_ranges_check(a);
     if (rc != TT_OK) return rc;
+    if (tt_ranges_few_rows(*a)) return tt_attn_ranges_few(*a, (cudaStream_t)stream);
     const int dev = tt_device().dev;
     FwdParams p;
     p.plan = plan_ptr(*a);

@@ -196,9 +196,11 @@ typedef struct {
     void *dq, *dk, *dv;
     long dq_stride[3], dk_stride[3], dv_stride[3];
     float* dbias;                       /* [q_heads, 2 * max_distance + 1] or null */
-    float* partials;                    /* scratch [batch, q_heads, tiles of queries, 2 * max_distance + 1] where dbias is wanted */
+    float* partials;                    /* scratch: forward of tt_attn_ranges_fwd_floats (none: null); backward, where dbias is wanted,
+                                         * [batch, q_heads, tiles of queries, 2 * max_distance + 1] */
     int* status;
 } tt_ranges_args;
+long tt_attn_ranges_fwd_floats(const tt_ranges_args* args);     /* touches no device memory */
 int tt_attn_ranges_fwd(const tt_ranges_args* args, void* stream);
 int tt_attn_ranges_bwd(const tt_ranges_args* args, void* stream);
 

@@ -61,10 +61,10 @@ def _load() -> Optional[ctypes.CDLL]:
     for name in ("tt_gemm_bf16", "tt_gemm2_bf16"):
         getattr(lib, name).argtypes = [vp] * 5 + [ci] * 3 + [cl] * 3 + [ci] * 3 + [vp] * 2
     lib.tt_gemm2_bf16_splitk.argtypes = [vp] * 5 + [ci] * 3 + [cl] * 3 + [ci] * 4 + [vp] * 3
-    lib.tt_rotary_partial_floats.restype = cl
     for name in ("tt_rotary", "tt_norm_rotary_fwd", "tt_norm_rotary_bwd", "tt_attn_ranges_fwd", "tt_attn_ranges_bwd"):
         getattr(lib, name).argtypes = [ctypes.c_char_p, vp]
-    lib.tt_rotary_partial_floats.argtypes = [ctypes.c_char_p]
+    for name in ("tt_rotary_partial_floats", "tt_attn_ranges_fwd_floats"):
+        getattr(lib, name).argtypes, getattr(lib, name).restype = [ctypes.c_char_p], cl
     lib.tt_gemm2_bf16_two.argtypes = [vp] * 5 + [ci] * 4 + [cl] * 4 + [ci] + [vp] * 3
     _lib = lib
     return lib

@@ -193,8 +193,9 @@ def supported(q, k, v, ranges, distance_bias) -> bool:
 _HEAD = struct.Struct("@l iiii iiii PPP 9l PPP PP ff")           # everything that the forward kernel reads but the status word
 _TAIL = struct.Struct("@PP PPP 9l PP P")
 _ARGS = struct.Struct("@l iiii iiii PPP 9l PPP PP ff PP PPP 9l PP P")
-_NO_BACKWARD = bytes(_TAIL.size - 8)
-_STATUS = struct.Struct("@P")
+_NO_BACKWARD = bytes(_TAIL.size - 16)
+_SCRATCH = struct.Struct("@PP")
+FEW_ROWS = 32           # queries of a group that the kernels for few queries take
 
 
 def _rows(t):
@@ -227,8 +228,14 @@ def _forward(q, k, v, ranges, scale, softcap, bias, wide):
     out = q.new_empty((B, n, hq * D))
     out32 = q.new_empty((B, n, hq * D), dtype=torch.float32) if wide else None
     lse = q.new_empty((B, hq, (n + TILE - 1) // TILE * TILE), dtype=torch.float32)
-    call("tt_attn_ranges_fwd", _pack(q, k, v, ranges, out, out32, lse, scale, softcap, bias) + _NO_BACKWARD + _STATUS.pack(status_tensor(q.device).data_ptr()),
-         stream())
+    head, status = _pack(q, k, v, ranges, out, out32, lse, scale, softcap, bias) + _NO_BACKWARD, status_tensor(q.device).data_ptr()
+    scratch = None
+    if not wide and n * (hq // k.shape[1]) <= FEW_ROWS:
+        size = _lib.lib().tt_attn_ranges_fwd_floats(head + _SCRATCH.pack(0, status))
+        if size:
+            scratch = q.new_empty((size,), dtype=torch.float32)
+            _lib.LAUNCHES += 1          # the join
+    call("tt_attn_ranges_fwd", head + _SCRATCH.pack(0 if scratch is None else scratch.data_ptr(), status), stream())
     return out, out32, lse
 
 

@@ -273,3 +273,36 @@ def test_projection_rotation_and_attention_together():
     for a, b in zip(got, want):
         # nine roundings to 2^-8 between input and gradient, each of independent elements: a relative norm of 9 * 2^-8 bounds them all
         assert float((a.double() - b).norm() / b.norm()) < 9 * 2 ** -8
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, FP16), (128, BF16)])
+@pytest.mark.parametrize("n,hq,hk", [(1, 1, 1), (1, 32, 1), (2, 32, 2), (16, 2, 2), (17, 1, 1), (32, 2, 2), (33, 2, 2), (5, 24, 4)])
+def test_few_queries(n, hq, hk, D, dtype):
+    """Both sides of the borders between the kernels for few queries (16 and 32 rows of a group) and the one for tiles."""
+    lengths = torch.tensor([1500, n, 700], device="cuda")
+    kw = dict(causal=True, kv_valid_len=lengths, query_start=lengths - n)
+    check(3, n, 1500, hq, hk, D, dtype, train=False, **kw)
+    check(3, n, 1500, hq, hk, D, dtype, R=60, softcap=8.0, scale=-0.2, **kw)
+    check(2, n, n, hq, hk, D, dtype, documents=[0, (n + 1) // 2, n], causal=True)
+    check(2, n, 300, hq, hk, D, dtype, False, kv_valid_len=torch.tensor([0, 299], device="cuda"))
+
+
+def test_few_queries_over_one_long_cache():
+    check(1, 1, 40000, 4, 1, 64, BF16, train=False, causal=True, query_start=39999)
+    check(1, 3, 20001, 2, 2, 128, BF16, train=False, causal=True, query_start=20000 - 2, token_major=False)
+
+
+def test_few_queries_past_32_bits_of_elements():
+    """A cache whose last rows lie beyond 2^32 elements: two samples, far apart in one allocation."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("not enough device memory")
+    far = 2 ** 32 // (2 * 64) + 8
+    buf = torch.empty(far * 2 * 64 + 600 * 2 * 64, device="cuda", dtype=BF16)
+    k = torch.as_strided(buf, (2, 2, 300, 64), (far * 2 * 64, 64, 128, 1))
+    k.copy_(torch.randn(2, 2, 300, 64, device="cuda"))
+    q = torch.randn(2, 4, 1, 64, device="cuda").to(BF16)
+    r = ops.key_ranges(1, 300, batch=2, causal=True, query_start=299, device="cuda")
+    assert torch.equal(ops.masked_attention(q, k, k, r), ops.masked_attention(q, k.contiguous(), k.contiguous(), r))
+    q = torch.randn(2, 4, 300, 64, device="cuda").to(BF16)
+    r = ops.key_ranges(300, batch=2, causal=True, device="cuda")
+    assert torch.equal(ops.masked_attention(q, k, k, r), ops.masked_attention(q, k.contiguous(), k.contiguous(), r))
