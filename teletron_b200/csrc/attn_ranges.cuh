@@ -76,6 +76,42 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, abort_flag));
 }
 
+// The items of a CTA: its own block index, then ones of the launch that have not been started, so that an item's first loads and products
+// run behind the last one's.  The loading warp asks for the next item when it begins one; every role reads the answer when it is through.
+struct Queue {
+    static constexpr int kBytes = 64;               // two answers of 16 bytes, two pairs of barriers
+    uint32_t base;
+    int n = 0;                                      // items begun
+    __device__ __forceinline__ uint32_t answer() const { return base + 16u * (n & 1); }
+    __device__ __forceinline__ uint32_t full() const { return base + 32u + 8u * (n & 1); }
+    __device__ __forceinline__ uint32_t empty() const { return base + 48u + 8u * (n & 1); }
+    __device__ __forceinline__ void init(int readers) const {         // one thread
+        for (int i = 0; i < 2; ++i) {
+            sm100::mbar_init(base + 32u + 8u * i, 1);
+            sm100::mbar_init(base + 48u + 8u * i, readers);
+        }
+    }
+    // the loading warp, once per item; its `lead` lane asks
+    __device__ __forceinline__ bool ask(bool lead, volatile int* abort_flag) const {
+        if (!warp_wait(empty(), (uint32_t)(n >> 1) & 1u ^ 1u, abort_flag)) return false;
+        if (lead) {
+            sm100::fence_proxy_async();             // the readers of the answer before last were ordinary loads
+            sm100::mbar_arrive_expect_tx(full(), 16);
+            sm100::launch_take(answer(), full());
+        }
+        return true;
+    }
+    __device__ __forceinline__ uint32_t parity() const { return (uint32_t)(n >> 1) & 1u; }
+    // the next item's block index, once full() has completed; a reader is a whole warp, of which one lane arrives, or a single thread
+    template <bool WARP> __device__ __forceinline__ bool next(bool arrive, int* x, int* y, int* z) {
+        const bool ok = sm100::launch_taken(answer(), x, y, z);
+        if (WARP) __syncwarp();
+        if (arrive) sm100::mbar_arrive(empty());
+        ++n;
+        return ok;
+    }
+};
+
 // Bits [lo, hi) of a 32-bit word, for any lo and hi.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
     const uint32_t below_hi = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u;

@@ -243,6 +243,31 @@ __device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t* r) 
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---------------------------------------------------------------- work that the launch has not started yet
+// A running CTA takes over a CTA of its own grid that has not been launched: the answer, 16 bytes, lands in shared memory and completes on a
+// barrier.  After an answer of "none left" no CTA may ask again.
+__device__ __forceinline__ void launch_take(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+// Its block index, or false.
+__device__ __forceinline__ bool launch_taken(uint32_t answer, int* x, int* y, int* z) {
+    uint32_t ok, a, b, c;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%4];\n\t"
+        "mov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, h;\n\t}"
+        : "=r"(ok), "=r"(a), "=r"(b), "=r"(c)
+        : "r"(answer)
+        : "memory");
+    *x = (int)a;
+    *y = (int)b;
+    *z = (int)c;
+    return ok != 0;
+}
+
 // ---------------------------------------------------------------- CTA pairs (cluster of two, cta_group::2)
 constexpr uint32_t kPeerMask = 0xFEFFFFFFu;             // clears the bit that tells the two CTAs of a pair apart
 
