@@ -132,6 +132,27 @@ __device__ __forceinline__ void clear_rows(uint32_t tile, int slabs, uint4 bits,
     }
 }
 
+// 64 bytes of each of a warp's 32 rows to memory through 2 KB of shared memory: a lane has its row's four 16-byte pieces, and stores the pieces of
+// eight rows with three others (stored by the lanes that have them, 32 rows' pieces are as many lines an instruction, and the output of two
+// tiles of 128 x 128 took 5000 clocks).  `dst(row)`: where a row's 64 bytes go, or null.
+template <typename F> __device__ __forceinline__ void store_rows64(uint32_t stage, int lane, const uint4* piece, F&& dst) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)), "r"(piece[q].x), "r"(piece[q].y),
+                     "r"(piece[q].z), "r"(piece[q].w)
+                     : "memory");
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2), q = lane & 3;
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + row * 64 + ((q ^ (row >> 1 & 3)) << 4)) : "memory");
+        uint4* to = reinterpret_cast<uint4*>(dst(row));
+        if (to != nullptr) to[q] = v;
+    }
+    __syncwarp();
+}
+
 // cap tanh(scale z / cap) log2(e) of raw scores z, in the log2 domain.  Where all of a warp's scores are small against the cap the odd Taylor
 // series up to the ninth power (|u| <= 0.3: the next term is below 2^-24 of the value) takes six packed multiply-adds a pair; else
 // tanh u = 1 - 2 / (1 + e^2u), two special functions a score, exact to a few roundings of the cap.

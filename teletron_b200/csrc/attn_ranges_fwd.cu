@@ -46,9 +46,11 @@ template <int D> struct Layout {
     static constexpr int kTileBytes = kSlabs * kSlab;
     static constexpr int kStages = D == 64 ? 4 : 2;         // of keys and of values each
     static constexpr int kBars = 2 + 5 * kStages + 2 + 4 + 2 + 2;
-    static constexpr int kFixed = (2 + 2 * kStages) * kTileBytes + (kBars + 1) / 2 * 16 + Queue::kBytes;
-    static constexpr int smem(int R) { return kFixed + 1024 + (R >= 0 ? 2 * (2 * R + 1 + 2 * kPad) * 4 : 0); }
+    static constexpr int kFixed = (2 + 2 * kStages) * kTileBytes + 8 * 2048 + (kBars + 1) / 2 * 16 + Queue::kBytes + 16;      // 16: abort flag, tensor memory's address
+    // dynamic shared memory is declared to start at a 1024-byte boundary, and there is no static one ahead of it
+    static constexpr int smem(int R) { return kFixed + (R >= 0 ? 2 * (2 * R + 1 + 2 * kPad) * 4 : 0); }
 };
+static_assert(Layout<128>::smem(TT_RANGES_MAX_DISTANCE) <= 232448, "shared memory of an SM");
 
 enum { kPlain = 0, kGeneral = 1, kGeneralWide = 2 };
 
@@ -63,14 +65,18 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     using L = Layout<D>;
     constexpr bool GEN = MODE != kPlain, WIDE = MODE == kGeneralWide;
     constexpr int kStages = L::kStages, kTileBytes = L::kTileBytes;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ volatile int abort_flag;
-    __shared__ uint32_t tmem_base_slot;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem_raw + L::kFixed - 16);
+    uint32_t& tmem_base_slot = *reinterpret_cast<uint32_t*>(smem_raw + L::kFixed - 8);
 
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sQ = base, sK = base + 2 * kTileBytes, sV = sK + kStages * kTileBytes, bars = sV + kStages * kTileBytes;
+    const uint32_t base = smem_u32(smem_raw);
+    if (base & 1023u) {                 // the swizzled tiles would be read wrongly
+        if (threadIdx.x == 0) atomicExch(p.status, TT_ERR_ARG);
+        return;
+    }
+    const uint32_t sQ = base, sK = base + 2 * kTileBytes, sV = sK + kStages * kTileBytes, stages = sV + kStages * kTileBytes, bars = stages + 8 * 2048;
     const uint32_t queue_base = bars + (L::kBars + 1) / 2 * 16;
-    float* table = reinterpret_cast<float*>(smem_raw + (queue_base - smem_u32(smem_raw)) + Queue::kBytes);
+    float* table = reinterpret_cast<float*>(smem_raw + L::kFixed);
     const uint32_t q_full = bars, q_empty = bars + 8u;
     auto k_full = [&](int s) { return bars + 8u * (2 + s); };
     auto k_empty = [&](int s) { return bars + 8u * (2 + kStages + s); };
@@ -484,26 +490,34 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tc_fence_after();
             const bool none = !some || l == 0.f;           // sees nothing, or nothing but scores of -inf
             const float inv = none ? 0.f : 1.f / l;
-            const long at = (((long)w.b * p.q_len + row) * p.q_heads + w.head) * D;
-            uint16_t* orow = reinterpret_cast<uint16_t*>(p.out) + at;
+            const int row0 = row - lane;
+            const long at = (((long)w.b * p.q_len + row0) * p.q_heads + w.head) * D, pitch = (long)p.q_heads * D;
+            uint16_t* const out = reinterpret_cast<uint16_t*>(p.out) + at;
+            const uint32_t stage = stages + (warp - 2) * 2048;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t r[32];
                 tmem_ld_32x32(tO + c * 32, r);
                 tmem_ld_wait();
-                if (!real) continue;
-                float o[32];
+                uint4 piece[4];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = none ? 0.f : __uint_as_float(r[i]) * inv;
+                for (int i = 0; i < 32; ++i) r[i] = none ? 0u : __float_as_uint(__uint_as_float(r[i]) * inv);
+                const float* o = reinterpret_cast<const float*>(r);
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<uint4*>(orow + c * 32 + g * 8) =
-                        make_uint4(pack2<BF16>(o[g * 8], o[g * 8 + 1]), pack2<BF16>(o[g * 8 + 2], o[g * 8 + 3]), pack2<BF16>(o[g * 8 + 4], o[g * 8 + 5]),
-                                   pack2<BF16>(o[g * 8 + 6], o[g * 8 + 7]));
+                    piece[g] = make_uint4(pack2<BF16>(o[g * 8], o[g * 8 + 1]), pack2<BF16>(o[g * 8 + 2], o[g * 8 + 3]),
+                                          pack2<BF16>(o[g * 8 + 4], o[g * 8 + 5]), pack2<BF16>(o[g * 8 + 6], o[g * 8 + 7]));
+                store_rows64(stage, lane, piece, [&](int i) { return row0 + i < p.q_len ? out + i * pitch + c * 32 : nullptr; });
                 if (WIDE) {
 #pragma unroll
-                    for (int g = 0; g < 8; ++g)
-                        *reinterpret_cast<float4*>(p.out32 + at + c * 32 + g * 4) = make_float4(o[g * 4], o[g * 4 + 1], o[g * 4 + 2], o[g * 4 + 3]);
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int i = half * 16 + g * 4;
+                            piece[g] = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+                        }
+                        store_rows64(stage, lane, piece, [&](int i) { return row0 + i < p.q_len ? p.out32 + at + i * pitch + c * 32 + half * 16 : nullptr; });
+                    }
                 }
             }
             if (w.qt < p.plan.q_tiles)
