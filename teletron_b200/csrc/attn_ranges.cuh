@@ -77,7 +77,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // The items of a CTA: its own block index, then ones of the launch that have not been started, so that an item's first loads and products
-// run behind the last one's.  The loading warp asks for the next item when it begins one; every role reads the answer when it is through.
+// run behind the last one's.  The loading warp asks for the next item when all of one's loads are under way (at its beginning, long items were
+// claimed by CTAs that were busy while others ran dry: 21 % on a causal mask's dK dV); every role reads the answer when it is through.
 struct Queue {
     static constexpr int kBytes = 64;               // two answers of 16 bytes, two pairs of barriers
     uint32_t base;

@@ -47,8 +47,10 @@ template <int D, bool KVS, int MODE> struct Layout {
     static constexpr int kTileBytes = kSlabs * kSlab;
     static constexpr int kRing1 = MODE == kGeneralDbias && D == 128 ? 2 : 3, kRing2 = D == 64 ? 3 : 2;
     static constexpr int kStats = KVS ? (kRing1 + kRing2) * kTile * 4 : 0;      // lse with every slot of Q, delta with every slot of dO
-    static constexpr int kBars = 1 + 3 * kRing1 + 3 * kRing2 + 7;
-    static constexpr int kFixed = (2 + kRing1 + kRing2) * kTileBytes + kStats + (kBars + 1) / 2 * 16 + 16;      // barriers, the abort flag and the tensor memory's address
+    static constexpr int kBars = 2 + 3 * kRing1 + 3 * kRing2 + 7;
+    static constexpr int kStage = D == 64 ? 16 * 2048 : 0;      // rows on their way out (heads of 128 leave no room)
+    // barriers, the queue, the abort flag and the tensor memory's address
+    static constexpr int kFixed = (2 + kRing1 + kRing2) * kTileBytes + kStats + kStage + (kBars + 1) / 2 * 16 + Queue::kBytes + 16;
     // dynamic shared memory is declared to start at a 1024-byte boundary, and there is no static one ahead of it
     static constexpr int smem(int R) { return kFixed + (MODE == kGeneralDbias ? (2 * 16 * 64 + 2 * R + 1 + 2 * kDiagPad) * 4 : 0); }
 };
@@ -72,58 +74,74 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t sA1 = base, sA2 = base + kTileBytes;
     const uint32_t sRing1 = base + 2 * kTileBytes, sRing2 = sRing1 + kRing1 * kTileBytes;
     const uint32_t sLse = sRing2 + kRing2 * kTileBytes, sDelta = sLse + kRing1 * kTile * 4;     // KVS
-    const uint32_t bars = sRing2 + kRing2 * kTileBytes + L::kStats;
+    const uint32_t stages = sRing2 + kRing2 * kTileBytes + L::kStats, bars = stages + L::kStage;
     float* scratch = reinterpret_cast<float*>(smem_raw + L::kFixed);      // [2][16 warps][64]: diagonals of a warp's block
     float* diag = scratch + 2 * 16 * 64;                                                                // [2 R + 1 + 2 kDiagPad]
-    const uint32_t a_full = bars;
-    auto b1_full = [&](int s) { return bars + 8u * (1 + s); };
-    auto b1_empty = [&](int s) { return bars + 8u * (1 + kRing1 + s); };
-    auto b1_clean = [&](int s) { return bars + 8u * (1 + 2 * kRing1 + s); };
-    auto b2_full = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + s); };
-    auto b2_empty = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + kRing2 + s); };
-    auto b2_clean = [&](int s) { return bars + 8u * (1 + 3 * kRing1 + 2 * kRing2 + s); };
-    const uint32_t s_full = bars + 8u * (1 + 3 * kRing1 + 3 * kRing2);      // T1 holds this chunk's scores
+    const uint32_t a_full = bars, a_empty = bars + 8u;
+    auto b1_full = [&](int s) { return bars + 8u * (2 + s); };
+    auto b1_empty = [&](int s) { return bars + 8u * (2 + kRing1 + s); };
+    auto b1_clean = [&](int s) { return bars + 8u * (2 + 2 * kRing1 + s); };
+    auto b2_full = [&](int s) { return bars + 8u * (2 + 3 * kRing1 + s); };
+    auto b2_empty = [&](int s) { return bars + 8u * (2 + 3 * kRing1 + kRing2 + s); };
+    auto b2_clean = [&](int s) { return bars + 8u * (2 + 3 * kRing1 + 2 * kRing2 + s); };
+    const uint32_t s_full = bars + 8u * (2 + 3 * kRing1 + 3 * kRing2);      // T1 holds this chunk's scores
     auto dp_full = [&](int c) { return s_full + 8u + (KVS ? 0u : 40u * (uint32_t)(c & 1)); };      // the chunk's dP is there (dQ: two buffers)
     const uint32_t p_ready = s_full + 16u;                     // every softmax warp has read the scores
     const uint32_t ds_ready = s_full + 24u;                    // P and dS have been written over dP
     const uint32_t acc_final = s_full + 32u;
     const uint32_t diag_ready = s_full + 40u;                  // every softmax warp has left its diagonals in the scratch
 
+    Queue queue{bars + (L::kBars + 1) / 2 * 16};
+
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int b = blockIdx.z;
-    const PlanView plan = p.plan.sample(b);
-    const int tile = KVS ? blockIdx.x : gridDim.x - 1 - blockIdx.x;         // the longest runs of a causal mask first
-    const int r0 = tile * kTile;
-    const int head0 = KVS ? blockIdx.y * p.group : blockIdx.y, kv_head = KVS ? blockIdx.y : blockIdx.y / p.group;
-    int lo = 0, hi = 0;
-    if (KVS) {
-        const int2 k = plan.k_tiles[tile];
-        lo = k.x;
-        hi = k.y;
-    } else {
-        const int4 r = plan.q_tiles[tile];
-        if (r.x < r.y) {
-            lo = r.x / kTile;
-            hi = (r.y + kTile - 1) / kTile;
+    // An item: a stationary tile of 128 rows from r0 on and the streamed tiles [lo, hi), KVS for all heads of the group one after the other
+    struct Item {
+        int b, tile, head, kv_head, lo, per_head, chunks;       // head: the first one
+    };
+    auto item_at = [&](int bx, int by, int bz) {
+        Item w;
+        w.b = bz;
+        w.tile = KVS ? bx : (int)gridDim.x - 1 - bx;         // the longest runs of a causal mask first
+        w.head = KVS ? by * p.group : by;
+        w.kv_head = KVS ? by : by / p.group;
+        const PlanView plan = p.plan.sample(bz);
+        int hi = 0;
+        w.lo = 0;
+        if (KVS) {
+            const int2 k = plan.k_tiles[w.tile];
+            w.lo = k.x;
+            hi = k.y;
+        } else {
+            const int4 r = plan.q_tiles[w.tile];
+            if (r.x < r.y) {
+                w.lo = r.x / kTile;
+                hi = (r.y + kTile - 1) / kTile;
+            }
         }
-    }
-    const int per_head = max(hi - lo, 0);
-    const int n_chunks = per_head * (KVS ? p.group : 1);
+        w.per_head = max(hi - w.lo, 0);
+        w.chunks = w.per_head * (KVS ? p.group : 1);
+        return w;
+    };
     struct Chunk {
         int head, t;
     };
-    auto chunk_at = [&](int c) {        // KVS: the queries of head after head
-        if (!KVS) return Chunk{head0, lo + c};
-        const int g = c / per_head;
-        return Chunk{head0 + g, lo + c - g * per_head};
+    auto chunk_at = [&](const Item& w, int c) {
+        if (!KVS) return Chunk{w.head, w.lo + c};
+        const int g = c / w.per_head;
+        return Chunk{w.head + g, w.lo + c - g * w.per_head};
     };
     auto lds4 = [](uint32_t at, float4& v) { asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at)); };
     // a streamed tile with rows that no run reaches: queries that see nothing, keys that nothing sees
-    auto is_dirty = [&](int c) { return c < n_chunks ? (KVS ? plan.q_tiles[chunk_at(c).t].w == 0 : plan.dirty[lo + c] != 0) : false; };
+    auto is_dirty = [&](const Item& w, const PlanView& plan, int c) {
+        return c < w.chunks ? (KVS ? plan.q_tiles[chunk_at(w, c).t].w == 0 : plan.dirty[w.lo + c] != 0) : false;
+    };
+    int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
         mbar_init(a_full, 1);
+        mbar_init(a_empty, 1);
+        queue.init(2 + 4 * kGroups);
         for (int s = 0; s < kRing1; ++s) {
             mbar_init(b1_full(s), 1);
             mbar_init(b1_empty(s), 1);
@@ -159,65 +177,77 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 0) {
         // ------------------------------------------------------------ loads
         const bool lead = elect_one();
-        if (lead && n_chunks > 0) {
-            mbar_arrive_expect_tx(a_full, 2 * kTileBytes);
-#pragma unroll
-            for (int h = 0; h < L::kSlabs; ++h) {
-                tma_load_4d(sA1 + h * kSlab, KVS ? &tmK : &tmQ, a_full, h * 64, r0, KVS ? kv_head : head0, b);
-                tma_load_4d(sA2 + h * kSlab, KVS ? &tmV : &tmDO, a_full, h * 64, r0, KVS ? kv_head : head0, b);
-            }
-        }
-        bool dirty = is_dirty(0);
-        for (int c = 0; c < n_chunks; ++c) {
-            const int s1 = c % kRing1, s2 = c % kRing2;
-            const uint32_t ph1 = (uint32_t)(c / kRing1) & 1u, ph2 = (uint32_t)(c / kRing2) & 1u;
-            const Chunk ch = chunk_at(c);
-            const int row = ch.t * kTile, head = KVS ? ch.head : kv_head;
-            const bool dirty_next = is_dirty(c + 1);
-            const uint32_t d1 = sRing1 + s1 * kTileBytes, d2 = sRing2 + s2 * kTileBytes;
-            if (!warp_wait(b1_empty(s1), ph1 ^ 1u, &abort_flag)) goto done;
-            if (lead) {
-                mbar_arrive_expect_tx(b1_full(s1), kTileBytes + (KVS ? kTile * 4 : 0));
-                if (KVS) bulk_load_1d(sLse + s1 * kTile * 4, p.lse + (((long)b * p.q_heads + head) * p.plan.q_tiles + ch.t) * kTile, kTile * 4, b1_full(s1));
-#pragma unroll
-                for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d1 + h * kSlab, KVS ? &tmQ : &tmK, b1_full(s1), h * 64, row, head, b);
-            }
-            if (!warp_wait(b2_empty(s2), ph2 ^ 1u, &abort_flag)) goto done;
-            if (lead) {
-                mbar_arrive_expect_tx(b2_full(s2), kTileBytes + (KVS ? kTile * 4 : 0));
-                if (KVS) bulk_load_1d(sDelta + s2 * kTile * 4, p.delta + (((long)b * p.q_heads + head) * p.plan.q_tiles + ch.t) * kTile, kTile * 4, b2_full(s2));
-#pragma unroll
-                for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d2 + h * kSlab, KVS ? &tmDO : &tmV, b2_full(s2), h * 64, row, head, b);
-            }
-            __syncwarp();
-            if (dirty) {        // their P and dS are 0, and 0 times a NaN is a NaN
-                uint4 bits;
-                if (KVS) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int i = row + q * 32 + lane;
-                        w[q] = __ballot_sync(0xffffffffu, i < p.q_len && plan.first[i] >= plan.behind[i]);
-                    }
-                    bits = make_uint4(w[0], w[1], w[2], w[3]);
-                } else {
-                    bits = plan.dead[ch.t];
-                }
-                if (!warp_wait(b1_full(s1), ph1, &abort_flag)) goto done;
-                clear_rows(d1, L::kSlabs, bits, lane);
-                if (KVS) {      // V only meets dS through a selection by the mask
-                    if (!warp_wait(b2_full(s2), ph2, &abort_flag)) goto done;
-                    clear_rows(d2, L::kSlabs, bits, lane);
-                }
-                fence_proxy_async();
-                __syncwarp();
+        int i = 0, n_some = 0;              // chunks, and items that have any, so far
+        do {
+            const Item w = item_at(bx, by, bz);
+            const PlanView plan = p.plan.sample(w.b);
+            if (w.chunks > 0) {
+                if (!warp_wait(a_empty, (uint32_t)n_some & 1u ^ 1u, &abort_flag)) goto done;
                 if (lead) {
-                    mbar_arrive(b1_clean(s1));
-                    if (KVS) mbar_arrive(b2_clean(s2));
+                    mbar_arrive_expect_tx(a_full, 2 * kTileBytes);
+#pragma unroll
+                    for (int h = 0; h < L::kSlabs; ++h) {
+                        tma_load_4d(sA1 + h * kSlab, KVS ? &tmK : &tmQ, a_full, h * 64, w.tile * kTile, KVS ? w.kv_head : w.head, w.b);
+                        tma_load_4d(sA2 + h * kSlab, KVS ? &tmV : &tmDO, a_full, h * 64, w.tile * kTile, KVS ? w.kv_head : w.head, w.b);
+                    }
                 }
+                ++n_some;
             }
-            dirty = dirty_next;
-        }
+            bool dirty = is_dirty(w, plan, 0);
+            for (int c = 0; c < w.chunks; ++c, ++i) {
+                const int s1 = i % kRing1, s2 = i % kRing2;
+                const uint32_t ph1 = (uint32_t)(i / kRing1) & 1u, ph2 = (uint32_t)(i / kRing2) & 1u;
+                const Chunk ch = chunk_at(w, c);
+                const int row = ch.t * kTile, head = KVS ? ch.head : w.kv_head;
+                const bool dirty_next = is_dirty(w, plan, c + 1);
+                const uint32_t d1 = sRing1 + s1 * kTileBytes, d2 = sRing2 + s2 * kTileBytes;
+                const long stat = (((long)w.b * p.q_heads + head) * p.plan.q_tiles + ch.t) * kTile;
+                if (!warp_wait(b1_empty(s1), ph1 ^ 1u, &abort_flag)) goto done;
+                if (lead) {
+                    mbar_arrive_expect_tx(b1_full(s1), kTileBytes + (KVS ? kTile * 4 : 0));
+                    if (KVS) bulk_load_1d(sLse + s1 * kTile * 4, p.lse + stat, kTile * 4, b1_full(s1));
+#pragma unroll
+                    for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d1 + h * kSlab, KVS ? &tmQ : &tmK, b1_full(s1), h * 64, row, head, w.b);
+                }
+                if (!warp_wait(b2_empty(s2), ph2 ^ 1u, &abort_flag)) goto done;
+                if (lead) {
+                    mbar_arrive_expect_tx(b2_full(s2), kTileBytes + (KVS ? kTile * 4 : 0));
+                    if (KVS) bulk_load_1d(sDelta + s2 * kTile * 4, p.delta + stat, kTile * 4, b2_full(s2));
+#pragma unroll
+                    for (int h = 0; h < L::kSlabs; ++h) tma_load_4d(d2 + h * kSlab, KVS ? &tmDO : &tmV, b2_full(s2), h * 64, row, head, w.b);
+                }
+                __syncwarp();
+                if (dirty) {        // their P and dS are 0, and 0 times a NaN is a NaN
+                    uint4 bits;
+                    if (KVS) {
+                        uint32_t m[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int r = row + q * 32 + lane;
+                            m[q] = __ballot_sync(0xffffffffu, r < p.q_len && plan.first[r] >= plan.behind[r]);
+                        }
+                        bits = make_uint4(m[0], m[1], m[2], m[3]);
+                    } else {
+                        bits = plan.dead[ch.t];
+                    }
+                    if (!warp_wait(b1_full(s1), ph1, &abort_flag)) goto done;
+                    clear_rows(d1, L::kSlabs, bits, lane);
+                    if (KVS) {      // V only meets dS through a selection by the mask
+                        if (!warp_wait(b2_full(s2), ph2, &abort_flag)) goto done;
+                        clear_rows(d2, L::kSlabs, bits, lane);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lead) {
+                        mbar_arrive(b1_clean(s1));
+                        if (KVS) mbar_arrive(b2_clean(s2));
+                    }
+                }
+                dirty = dirty_next;
+            }
+            if (!queue.ask(lead, &abort_flag)) goto done;
+            if (!warp_wait(queue.full(), queue.parity(), &abort_flag)) goto done;
+        } while (queue.next<true>(lead, &bx, &by, &bz));
     } else if (warp == 1) {
         // ------------------------------------------------------------ products
         if (elect_one()) {
@@ -240,329 +270,406 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                                  (first && kk == 0) ? 0u : 1u);
             };
             uint32_t cleaned1 = 0, cleaned2 = 0;        // bit s: parity of the cleaned uses of slot s
-            auto wait_b1 = [&](int c, bool dirty) {
-                const int s = c % kRing1;
-                if (!dirty) return mbar_wait(b1_full(s), (uint32_t)(c / kRing1) & 1u, &abort_flag);
+            auto wait_b1 = [&](int i, bool dirty) {
+                const int s = i % kRing1;
+                if (!dirty) return mbar_wait(b1_full(s), (uint32_t)(i / kRing1) & 1u, &abort_flag);
                 const uint32_t par = cleaned1 >> s & 1u;
                 cleaned1 ^= 1u << s;
                 return mbar_wait(b1_clean(s), par, &abort_flag);
             };
-            auto wait_b2 = [&](int c, bool dirty) {
-                const int s = c % kRing2;
-                if (!KVS || !dirty) return mbar_wait(b2_full(s), (uint32_t)(c / kRing2) & 1u, &abort_flag);
+            auto wait_b2 = [&](int i, bool dirty) {
+                const int s = i % kRing2;
+                if (!KVS || !dirty) return mbar_wait(b2_full(s), (uint32_t)(i / kRing2) & 1u, &abort_flag);
                 const uint32_t par = cleaned2 >> s & 1u;
                 cleaned2 ^= 1u << s;
                 return mbar_wait(b2_clean(s), par, &abort_flag);
             };
-            if (n_chunks > 0) {
-                const bool dirty = is_dirty(0);
-                if (!mbar_wait(a_full, 0, &abort_flag)) goto done;
-                if (!wait_b1(0, dirty)) goto done;
-                tc_fence_after();
-                issue_t(kT1, sA1, sRing1);
-                umma_commit(s_full);
-                if (!wait_b2(0, dirty)) goto done;
-                tc_fence_after();
-                issue_t(kT2, sA2, sRing2);
-                umma_commit(dp_full(0));
-                if (!KVS) umma_commit(b2_empty(0));
-            }
-            for (int c = 0; c < n_chunks; ++c) {
-                const uint32_t par = (uint32_t)c & 1u;
-                const bool more = c + 1 < n_chunks;
-                const bool dirty_next = is_dirty(c + 1);
-                const uint32_t next1 = sRing1 + (c + 1) % kRing1 * kTileBytes, next2 = sRing2 + (c + 1) % kRing2 * kTileBytes;
-                if (!mbar_wait(p_ready, par, &abort_flag)) goto done;
-                tc_fence_after();
-                if (KVS) {
-                    // T1 holds P: dV takes it while dS is formed, then the next chunk's scores take T1
-                    issue_acc(kAcc1, kT1, sRing2 + c % kRing2 * kTileBytes, c == 0);                    // dV += P^T dO
-                    if (more) {
-                        if (!wait_b1(c + 1, dirty_next)) goto done;
-                        tc_fence_after();
-                        issue_t(kT1, sA1, next1);
-                        umma_commit(s_full);
-                    }
-                    if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
+            auto slot1 = [&](int i) { return sRing1 + i % kRing1 * kTileBytes; };
+            auto slot2 = [&](int i) { return sRing2 + i % kRing2 * kTileBytes; };
+            auto t2_of = [&](int i) { return KVS || !(i & 1) ? kT2 : kT3; };
+            int i = 0, n_some = 0;              // chunks, and items that have any, so far
+            do {
+                const Item w = item_at(bx, by, bz);
+                const PlanView plan = p.plan.sample(w.b);
+                if (w.chunks > 0) {
+                    const bool dirty = is_dirty(w, plan, 0);
+                    if (!mbar_wait(a_full, (uint32_t)n_some++ & 1u, &abort_flag)) goto done;
+                    if (!wait_b1(i, dirty)) goto done;
                     tc_fence_after();
-                    issue_acc(kAcc2, kT2, sRing1 + c % kRing1 * kTileBytes, c == 0);                    // dK += dS^T Q
-                    umma_commit(b1_empty(c % kRing1));
-                    umma_commit(b2_empty(c % kRing2));         // not behind dV: delta lies in the slot until dS is formed
-                    if (more) {
-                        if (!wait_b2(c + 1, dirty_next)) goto done;
-                        tc_fence_after();
-                        issue_t(kT2, sA2, next2);
-                        umma_commit(dp_full(c + 1));
-                    }
-                } else {
-                    // the scores have been read: the next chunk's, and its dP in the other buffer, overlap this chunk's dS
-                    if (more) {
-                        if (!wait_b1(c + 1, dirty_next)) goto done;
-                        tc_fence_after();
-                        issue_t(kT1, sA1, next1);
-                        umma_commit(s_full);
-                        if (!wait_b2(c + 1, dirty_next)) goto done;
-                        tc_fence_after();
-                        issue_t(c & 1 ? kT2 : kT3, sA2, next2);
-                        umma_commit(dp_full(c + 1));
-                        umma_commit(b2_empty((c + 1) % kRing2));
-                    }
-                    if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
+                    issue_t(kT1, sA1, slot1(i));
+                    umma_commit(s_full);
+                    if (!wait_b2(i, dirty)) goto done;
                     tc_fence_after();
-                    issue_acc(kAcc1, c & 1 ? kT3 : kT2, sRing1 + c % kRing1 * kTileBytes, c == 0);      // dQ += dS K
-                    umma_commit(b1_empty(c % kRing1));
+                    issue_t(t2_of(i), sA2, slot2(i));
+                    umma_commit(dp_full(i));
+                    if (!KVS) umma_commit(b2_empty(i % kRing2));
+                    if (w.chunks == 1) umma_commit(a_empty);
                 }
-            }
-            umma_commit(acc_final);
+                for (int c = 0; c < w.chunks; ++c, ++i) {
+                    const uint32_t par = (uint32_t)i & 1u;
+                    const bool more = c + 1 < w.chunks;
+                    const bool dirty_next = is_dirty(w, plan, c + 1);
+                    if (!mbar_wait(p_ready, par, &abort_flag)) goto done;
+                    tc_fence_after();
+                    if (KVS) {
+                        // T1 holds P: dV takes it while dS is formed, then the next chunk's scores take T1
+                        issue_acc(kAcc1, kT1, slot2(i), c == 0);                    // dV += P^T dO
+                        if (more) {
+                            if (!wait_b1(i + 1, dirty_next)) goto done;
+                            tc_fence_after();
+                            issue_t(kT1, sA1, slot1(i + 1));
+                            umma_commit(s_full);
+                        }
+                        if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
+                        tc_fence_after();
+                        issue_acc(kAcc2, kT2, slot1(i), c == 0);                    // dK += dS^T Q
+                        umma_commit(b1_empty(i % kRing1));
+                        umma_commit(b2_empty(i % kRing2));         // not behind dV: delta lies in the slot until dS is formed
+                        if (more) {
+                            if (!wait_b2(i + 1, dirty_next)) goto done;
+                            tc_fence_after();
+                            issue_t(kT2, sA2, slot2(i + 1));
+                            umma_commit(dp_full(i + 1));
+                        }
+                    } else {
+                        // the scores have been read: the next chunk's, and its dP in the other buffer, overlap this chunk's dS
+                        if (more) {
+                            if (!wait_b1(i + 1, dirty_next)) goto done;
+                            tc_fence_after();
+                            issue_t(kT1, sA1, slot1(i + 1));
+                            umma_commit(s_full);
+                            if (!wait_b2(i + 1, dirty_next)) goto done;
+                            tc_fence_after();
+                            issue_t(t2_of(i + 1), sA2, slot2(i + 1));
+                            umma_commit(dp_full(i + 1));
+                            umma_commit(b2_empty((i + 1) % kRing2));
+                        }
+                        if (!mbar_wait(ds_ready, par, &abort_flag)) goto done;
+                        tc_fence_after();
+                        issue_acc(kAcc1, t2_of(i), slot1(i), c == 0);               // dQ += dS K
+                        umma_commit(b1_empty(i % kRing1));
+                    }
+                    if (c + 2 == w.chunks) umma_commit(a_empty);        // the item's last scores and dP: the next one's operands may come
+                }
+                if (w.chunks > 0) umma_commit(acc_final);
+                if (!mbar_wait(queue.full(), queue.parity(), &abort_flag)) goto done;
+            } while (queue.next<false>(true, &bx, &by, &bz));
         }
     } else {
         // ------------------------------------------------------------ P and dS
         const int part = (warp - 2) >> 2, quad = warp & 3;
-        const int row = r0 + quad * 32 + lane;                  // key (KVS) or query
         const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
         const uint32_t t1 = tmem + lane_sel + kT1 + part * kCols, t2 = tmem + lane_sel + kT2 + part * kCols;
-        const int start = plan.start;
-        float my_lse = 0.f, my_delta = 0.f;
-        int first = 0, behind = 0;
-        if (!KVS) {
-            const long at = ((long)b * p.q_heads + head0) * p.plan.q_tiles * kTile + row;
-            my_lse = p.lse[at];             // +inf behind the last query: its P is 0
-            my_delta = p.delta[at];
-            if (row < p.q_len) {
-                first = plan.first[row];
-                behind = plan.behind[row];
-            }
-        }
-        float far_sum = 0.f, near_sum = 0.f;    // of dS beyond the largest distance: ahead of the query, behind it
-        int n_diag = 0;
-        for (int c = 0; c < n_chunks; ++c) {
-            const uint32_t par = (uint32_t)c & 1u;
-            const Chunk ch = chunk_at(c);
-            const int col0 = ch.t * kTile + part * kCols;         // first streamed row of this thread's 32
-            uint32_t see = 0xffffffffu;
-            if (KVS) {
-                const int4 r = plan.q_tiles[ch.t];
-                if (r.z > r0 || r.w < min(r0 + kTile, p.kv_len)) {         // some query does not see all of these keys
-                    const int i = col0 + lane, k0 = r0 + quad * 32;
-                    uint32_t mine = 0u;                                    // keys of this warp that query `lane` sees
-                    if (i < p.q_len) mine = bits_between(plan.first[i] - k0, plan.behind[i] - k0);
-                    see = 0u;
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) see |= (__shfl_sync(0xffffffffu, mine, q) >> lane & 1u) << q;
+        // what a thread needs of an item; the next one's is read ahead of this one's results
+        struct Mine {
+            Item w;
+            float lse, delta;
+            int first, behind, start;
+        };
+        auto mine_of = [&](int x, int y, int z) {
+            Mine v;
+            v.w = item_at(x, y, z);
+            const PlanView plan = p.plan.sample(v.w.b);
+            v.start = plan.start;
+            v.lse = v.delta = 0.f;
+            v.first = v.behind = 0;
+            if (!KVS) {
+                const int row = v.w.tile * kTile + quad * 32 + lane;
+                const long at = ((long)v.w.b * p.q_heads + v.w.head) * p.plan.q_tiles * kTile + row;
+                v.lse = p.lse[at];             // +inf behind the last query: its P is 0
+                v.delta = p.delta[at];
+                if (row < p.q_len) {
+                    v.first = plan.first[row];
+                    v.behind = plan.behind[row];
                 }
-            } else {
-                see = bits_between(first - col0, behind - col0);
             }
-            const bool clean = __all_sync(0xffffffffu, see == 0xffffffffu);
-            // distance of column i: base + i * step
-            const int pos0 = KVS ? row - (start + col0) : col0 - (start + row);
-            bool at_end = false;
-            float end_bias = 0.f;
-            const float* bias_row = nullptr;
-            if (MODE != kPlain && p.R >= 0) {
-                bias_row = p.bias + (long)ch.head * (2 * p.R + 1) + p.R;
-                const int w0 = __shfl_sync(0xffffffffu, pos0, 0), w31 = __shfl_sync(0xffffffffu, pos0, 31);
-                const int least = KVS ? w0 - 31 : w31, most = KVS ? w31 : w0 + 31;
-                at_end = most <= -p.R || least >= p.R;
-                if (at_end) end_bias = bias_row[least >= p.R ? p.R : -p.R] * kLog2e;
-            }
-            uint32_t tk[MODE != kPlain ? 16 : 1], a[32];
-            if (!warp_wait(s_full, par, &abort_flag)) goto done;
-            tc_fence_after();
-            tmem_ld_32x32(t1, a);
-            tmem_ld_wait();
-            if (MODE != kPlain) {           // raw scores to the log2 domain
-                if (p.cap.out != 0.f) {
-                    const bool small = all_small<32>(p.cap, a);
+            return v;
+        };
+        Mine v = mine_of(bx, by, bz);
+        int i = 0, n_diag = 0, n_final = 0;
+        bool go = true;
+        while (go) {
+            const Item w = v.w;
+            const PlanView plan = p.plan.sample(w.b);
+            const int r0 = w.tile * kTile, row = r0 + quad * 32 + lane;         // key (KVS) or query
+            const int start = v.start;
+            float far_sum = 0.f, near_sum = 0.f;    // of dS beyond the largest distance: ahead of the query, behind it
+            float far_p = 0.f, near_p = 0.f, all_sum = 0.f;     // of P there, and of all dS
+            for (int c = 0; c < w.chunks; ++c, ++i) {
+                const uint32_t par = (uint32_t)i & 1u;
+                const Chunk ch = chunk_at(w, c);
+                const int col0 = ch.t * kTile + part * kCols;         // first streamed row of this thread's 32
+                uint32_t see = 0xffffffffu;
+                if (KVS) {
+                    const int4 r = plan.q_tiles[ch.t];
+                    if (r.z > r0 || r.w < min(r0 + kTile, p.kv_len)) {         // some query does not see all of these keys
+                        const int q = col0 + lane, k0 = r0 + quad * 32;
+                        uint32_t mine = 0u;                                    // keys of this warp that query `lane` sees
+                        if (q < p.q_len) mine = bits_between(plan.first[q] - k0, plan.behind[q] - k0);
+                        see = 0u;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 z = make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
-                        const float2 y = small ? cap_small(p.cap, z) : make_float2(cap_any(p.cap, z.x), cap_any(p.cap, z.y));
-                        const float2 t = __fmul2_rn(y, make_float2(p.cap.inv_out, p.cap.inv_out));
-                        const float2 slope = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
-                        // the cap's slope in fp16: 2^-11 of a factor that is rounded to 16 bits with its dS below
-                        tk[i] = pack2<false>(slope.x, slope.y);
-                        a[2 * i] = __float_as_uint(y.x);
-                        a[2 * i + 1] = __float_as_uint(y.y);
+                        for (int e = 0; e < 32; ++e) see |= (__shfl_sync(0xffffffffu, mine, e) >> lane & 1u) << e;
                     }
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * p.scale_log2);
+                    see = bits_between(v.first - col0, v.behind - col0);
                 }
-                if (p.R >= 0) {
+                const bool clean = __all_sync(0xffffffffu, see == 0xffffffffu);
+                // distance of column e: pos0 + e, KVS pos0 - e
+                const int pos0 = KVS ? row - (start + col0) : col0 - (start + row);
+                bool at_end = false, inside = false;
+                float end_bias = 0.f;
+                const float* bias_row = nullptr;
+                if (MODE != kPlain && p.R >= 0) {
+                    bias_row = p.bias + (long)ch.head * (2 * p.R + 1) + p.R;
+                    const int w0 = __shfl_sync(0xffffffffu, pos0, 0), w31 = __shfl_sync(0xffffffffu, pos0, 31);
+                    const int least = KVS ? w0 - 31 : w31, most = KVS ? w31 : w0 + 31;
+                    at_end = most <= -p.R || least >= p.R;
+                    inside = least >= -p.R && most <= p.R;
+                    if (at_end) end_bias = bias_row[least >= p.R ? p.R : -p.R] * kLog2e;
+                }
+                uint32_t tk[MODE != kPlain ? 16 : 1], a[32];
+                if (!warp_wait(s_full, par, &abort_flag)) goto done;
+                tc_fence_after();
+                tmem_ld_32x32(t1, a);
+                tmem_ld_wait();
+                if (MODE != kPlain) {           // raw scores to the log2 domain
+                    if (p.cap.out != 0.f) {
+                        const bool small = all_small<32>(p.cap, a);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int d = KVS ? pos0 - i : pos0 + i;
-                        const float add = at_end ? end_bias : bias_row[max(-p.R, min(p.R, d))] * kLog2e;
-                        a[i] = __float_as_uint(__uint_as_float(a[i]) + add);
+                        for (int e = 0; e < 16; ++e) {
+                            const float2 z = make_float2(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]));
+                            const float2 y = small ? cap_small(p.cap, z) : make_float2(cap_any(p.cap, z.x), cap_any(p.cap, z.y));
+                            const float2 t = __fmul2_rn(y, make_float2(p.cap.inv_out, p.cap.inv_out));
+                            const float2 slope = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
+                            // the cap's slope in fp16: 2^-11 of a factor that is rounded to 16 bits with its dS below
+                            tk[e] = pack2<false>(slope.x, slope.y);
+                            a[2 * e] = __float_as_uint(y.x);
+                            a[2 * e + 1] = __float_as_uint(y.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * p.scale_log2);
+                    }
+                    if (p.R >= 0) {
+                        if (at_end) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) + end_bias);
+                        } else if (inside) {
+                            const float* entry = bias_row + pos0;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(fmaf(__ldg(KVS ? entry - e : entry + e), kLog2e, __uint_as_float(a[e])));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                a[e] = __float_as_uint(fmaf(__ldg(bias_row + max(-p.R, min(p.R, KVS ? pos0 - e : pos0 + e))), kLog2e, __uint_as_float(a[e])));
+                        }
                     }
                 }
-            }
-            // P in 32 bits over the scores
-            if (KVS && !warp_wait(b1_full(c % kRing1), (uint32_t)(c / kRing1) & 1u, &abort_flag)) goto done;       // has the copied lse: long complete
+                // P in 32 bits over the scores
+                if (KVS && !warp_wait(b1_full(i % kRing1), (uint32_t)(i / kRing1) & 1u, &abort_flag)) goto done;       // has the copied lse: long complete
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                float4 l4 = make_float4(my_lse, my_lse, my_lse, my_lse);
-                if (KVS) lds4(sLse + ((c % kRing1) * kTile + part * kCols + 4 * q) * 4, l4);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int i = 4 * q + 2 * h;
-                    const float2 s2 = make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-                    const float2 n2 = h ? make_float2(-l4.z, -l4.w) : make_float2(-l4.x, -l4.y);
-                    const float2 y = MODE == kPlain ? __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), n2) : __fadd2_rn(s2, n2);
-                    a[i] = __float_as_uint(exp2f(y.x));
-                    a[i + 1] = __float_as_uint(exp2f(y.y));
-                }
-            }
-            if (!clean) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (!(see >> i & 1u)) a[i] = 0u;
-            }
-            if (KVS) {          // rounded for the product only: half a step of the operands' type
-                uint32_t pk[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) pk[i] = pack2<BF16>(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
-                tmem_st_32x16(t1, pk);
-                tmem_st_wait();
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready);
-
-            const uint32_t t2c = KVS || !(c & 1) ? t2 : t2 + (kT3 - kT2);
-            if (!warp_wait(dp_full(c), KVS ? par : (uint32_t)(c >> 1) & 1u, &abort_flag)) goto done;
-            tc_fence_after();
-            if (KVS && !warp_wait(b2_full(c % kRing2), (uint32_t)(c / kRing2) & 1u, &abort_flag)) goto done;       // and delta
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t g[16], dk[8];
-                tmem_ld_32x16(t2c + 16 * half, g);
-                tmem_ld_wait();
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float4 d4 = make_float4(my_delta, my_delta, my_delta, my_delta);
-                    if (KVS) lds4(sDelta + ((c % kRing2) * kTile + part * kCols + 16 * half + 4 * q) * 4, d4);
+                for (int q = 0; q < 8; ++q) {
+                    float4 l4 = make_float4(v.lse, v.lse, v.lse, v.lse);
+                    if (KVS) lds4(sLse + ((i % kRing1) * kTile + part * kCols + 4 * q) * 4, l4);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int i = 4 * q + 2 * h, k = 16 * half + i;
-                        const float2 n2 = h ? make_float2(-d4.z, -d4.w) : make_float2(-d4.x, -d4.y);
-                        float2 ds = __fmul2_rn(make_float2(__uint_as_float(a[k]), __uint_as_float(a[k + 1])),
-                                               __fadd2_rn(make_float2(__uint_as_float(g[i]), __uint_as_float(g[i + 1])), n2));
-                        float2 slope = make_float2(1.f, 1.f);
-                        if (MODE != kPlain && p.cap.out != 0.f) slope = unpack2<false>(tk[k >> 1]);
-                        if (!clean) {           // dP and the slope of a key or a query that no run reaches may be anything
-                            if (!(see >> k & 1u)) ds.x = slope.x = 0.f;
-                            if (!(see >> (k + 1) & 1u)) ds.y = slope.y = 0.f;
-                        }
-                        if (MODE == kGeneralDbias) {
-                            a[k] = __float_as_uint(ds.x);
-                            a[k + 1] = __float_as_uint(ds.y);
-                        }
-                        if (MODE != kPlain) ds = __fmul2_rn(ds, slope);
-                        // rounded to the operands' type, as the products take it: half a step of each dS
-                        dk[i >> 1] = pack2<BF16>(ds.x, ds.y);
+                        const int e = 4 * q + 2 * h;
+                        const float2 s2 = make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1]));
+                        const float2 n2 = h ? make_float2(-l4.z, -l4.w) : make_float2(-l4.x, -l4.y);
+                        const float2 y = MODE == kPlain ? __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), n2) : __fadd2_rn(s2, n2);
+                        a[e] = __float_as_uint(exp2f(y.x));
+                        a[e + 1] = __float_as_uint(exp2f(y.y));
                     }
                 }
-                tmem_st_32x8(t2c + 8 * half, dk);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(ds_ready);
+                if (!clean) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(see >> e & 1u)) a[e] = 0u;
+                }
+                if (KVS) {          // rounded for the product only: half a step of the operands' type
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) pk[e] = pack2<BF16>(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]));
+                    tmem_st_32x16(t1, pk);
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready);
 
-            if (MODE == kGeneralDbias) {
+                // beyond the largest distance the bias's gradient takes sums only
                 const int corner = ch.t * kTile - (start + r0);         // distance of the tile's first key from its first query
-                if (corner + kTile - 1 <= -p.R || corner - kTile + 1 >= p.R) {
+                const bool beyond = MODE == kGeneralDbias && (corner + kTile - 1 <= -p.R || corner - kTile + 1 >= p.R);
+                if (MODE == kGeneralDbias && beyond) {
                     float s = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s += __uint_as_float(a[i]);
-                    if (corner < 0) near_sum += s;
-                    else far_sum += s;
-                } else {
-                    // Sums along the diagonals of the warp's 32 x 32 block: a partial sum moves down one row per column.  Slot
-                    // c - row + 31; what leaves the last row at column c is slot c, what is left at the end belongs to slots 62 - row.
-                    float* slots = scratch + ((n_diag & 1) * 16 + part * 4 + quad) * 64;
-                    float acc = 0.f;
+                    for (int e = 0; e < 32; ++e) s += __uint_as_float(a[e]);
+                    if (corner < 0) near_p += s;
+                    else far_p += s;
+                }
+
+                const uint32_t t2c = KVS || !(i & 1) ? t2 : t2 + (kT3 - kT2);
+                if (!warp_wait(dp_full(i), KVS ? par : (uint32_t)(i >> 1) & 1u, &abort_flag)) goto done;
+                tc_fence_after();
+                if (KVS && !warp_wait(b2_full(i % kRing2), (uint32_t)(i / kRing2) & 1u, &abort_flag)) goto done;       // and delta
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float above = __shfl_up_sync(0xffffffffu, acc, 1);
-                        acc = (lane == 0 ? 0.f : above) + __uint_as_float(a[i]);
-                        if (lane == 31) slots[i] = acc;
-                    }
-                    if (lane < 31) slots[62 - lane] = acc;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(diag_ready);
-                    if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
-                    // one diagonal of the tile a thread, its warps' shares in a fixed order
-                    const int x = (int)threadIdx.x - 64;
-                    if (x < 2 * kTile - 1) {
-                        const int d = x - (kTile - 1);
-                        float s = 0.f;
-                        for (int q = 0; q < 4; ++q)
-                            for (int k = 0; k < 4; ++k) {
-                                const int slot = d - 32 * (k - q) + 31;
-                                if (slot >= 0 && slot < 63) s += scratch[((n_diag & 1) * 16 + k * 4 + q) * 64 + slot];
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t g[16], dk[8];
+                    tmem_ld_32x16(t2c + 16 * half, g);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float4 d4 = make_float4(v.delta, v.delta, v.delta, v.delta);
+                        if (KVS) lds4(sDelta + ((i % kRing2) * kTile + part * kCols + 16 * half + 4 * q) * 4, d4);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int e = 4 * q + 2 * h, k = 16 * half + e;
+                            const float2 n2 = h ? make_float2(-d4.z, -d4.w) : make_float2(-d4.x, -d4.y);
+                            float2 ds = __fmul2_rn(make_float2(__uint_as_float(a[k]), __uint_as_float(a[k + 1])),
+                                                   __fadd2_rn(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), n2));
+                            float2 slope = make_float2(1.f, 1.f);
+                            if (MODE != kPlain && p.cap.out != 0.f) slope = unpack2<false>(tk[k >> 1]);
+                            if (!clean) {           // dP and the slope of a key or a query that no run reaches may be anything
+                                if (!(see >> k & 1u)) ds.x = slope.x = 0.f;
+                                if (!(see >> (k + 1) & 1u)) ds.y = slope.y = 0.f;
                             }
-                        diag[kDiagPad + p.R + corner + d] += s;
+                            if (MODE == kGeneralDbias) {
+                                a[k] = __float_as_uint(ds.x);
+                                a[k + 1] = __float_as_uint(ds.y);
+                            }
+                            if (MODE != kPlain) ds = __fmul2_rn(ds, slope);
+                            // rounded to the operands' type, as the products take it: half a step of each dS
+                            dk[e >> 1] = pack2<BF16>(ds.x, ds.y);
+                        }
                     }
-                    ++n_diag;
+                    tmem_st_32x8(t2c + 8 * half, dk);
                 }
-            }
-        }
-        if (MODE == kGeneralDbias) {
-            // the sums beyond the largest distance, warp by warp; then this tile's row of the table
-            for (int o = 16; o > 0; o >>= 1) {
-                near_sum += __shfl_xor_sync(0xffffffffu, near_sum, o);
-                far_sum += __shfl_xor_sync(0xffffffffu, far_sum, o);
-            }
-            float* slots = scratch + (n_diag & 1) * 16 * 64;
-            if (lane == 0) {
-                slots[2 * (part * 4 + quad)] = near_sum;
-                slots[2 * (part * 4 + quad) + 1] = far_sum;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(diag_ready);
-            if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
-            float* out = p.partials + (((long)b * p.q_heads + head0) * p.plan.q_tiles + tile) * (2 * p.R + 1);
-            for (int e = (int)threadIdx.x - 64; e < 2 * p.R + 1; e += kThreads - 64) {
-                float s = diag[kDiagPad + e];
-                if (e == 0) {
-                    for (int i = 0; i < kDiagPad; ++i) s += diag[i];
-                    for (int i = 0; i < 16; ++i) s += slots[2 * i];
-                }
-                if (e == 2 * p.R) {
-                    for (int i = 0; i < kDiagPad; ++i) s += diag[kDiagPad + 2 * p.R + 1 + i];
-                    for (int i = 0; i < 16; ++i) s += slots[2 * i + 1];
-                }
-                out[e] = s;
-            }
-        }
-        // ------------------------------------------------------------ gradients
-        if (!warp_wait(acc_final, 0, &abort_flag)) goto done;
-        tc_fence_after();
-        const bool store = row < (KVS ? p.kv_len : p.q_len);
-#pragma unroll 1
-        for (int which = 0; which < (KVS ? 2 : 1); ++which) {
-            const long* st = which == 0 ? p.s1 : p.s2;
-            uint16_t* dst = reinterpret_cast<uint16_t*>(which == 0 ? p.out1 : p.out2) + b * st[0] + (KVS ? kv_head : head0) * st[1] + row * st[2];
-            const float mul = n_chunks == 0 ? 0.f : (KVS && which == 0) ? 1.f : p.scale;         // dV is unscaled
-            const uint32_t tacc = tmem + lane_sel + (which == 0 ? kAcc1 : kAcc2);
-#pragma unroll 1
-            for (int cch = part; cch < D / 32; cch += kGroups) {        // the warpgroups share the accumulator's columns
-                uint32_t r[32];
-                tmem_ld_32x32(tacc + cch * 32, r);
-                tmem_ld_wait();
-                if (!store) continue;
-                float o[32];
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_ready);
+
+                if (MODE == kGeneralDbias) {
+                    float s = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = n_chunks == 0 ? 0.f : __uint_as_float(r[i]) * mul;
+                    for (int e = 0; e < 32; ++e) s += __uint_as_float(a[e]);
+                    all_sum += s;
+                    if (beyond) {
+                        if (corner < 0) near_sum += s;
+                        else far_sum += s;
+                    } else {
+                        // Sums along the diagonals of the warp's 32 x 32 block: a partial sum moves down one row per column.  Slot
+                        // c - row + 31; what leaves the last row at column c is slot c, what is left at the end belongs to slots 62 - row.
+                        float* slots = scratch + ((n_diag & 1) * 16 + part * 4 + quad) * 64;
+                        float acc = 0.f;
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<uint4*>(dst + cch * 32 + g * 8) =
-                        make_uint4(pack2<BF16>(o[g * 8], o[g * 8 + 1]), pack2<BF16>(o[g * 8 + 2], o[g * 8 + 3]), pack2<BF16>(o[g * 8 + 4], o[g * 8 + 5]),
-                                   pack2<BF16>(o[g * 8 + 6], o[g * 8 + 7]));
+                        for (int e = 0; e < 32; ++e) {
+                            const float above = __shfl_up_sync(0xffffffffu, acc, 1);
+                            acc = (lane == 0 ? 0.f : above) + __uint_as_float(a[e]);
+                            if (lane == 31) slots[e] = acc;
+                        }
+                        if (lane < 31) slots[62 - lane] = acc;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(diag_ready);
+                        if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+                        // one diagonal of the tile a thread, its warps' shares in a fixed order
+                        const int x = (int)threadIdx.x - 64;
+                        if (x < 2 * kTile - 1) {
+                            const int d = x - (kTile - 1);
+                            float sum = 0.f;
+                            for (int q = 0; q < 4; ++q)
+                                for (int k = 0; k < 4; ++k) {
+                                    const int slot = d - 32 * (k - q) + 31;
+                                    if (slot >= 0 && slot < 63) sum += scratch[((n_diag & 1) * 16 + k * 4 + q) * 64 + slot];
+                                }
+                            diag[kDiagPad + p.R + corner + d] += sum;
+                        }
+                        ++n_diag;
+                    }
+                }
             }
+            if (MODE == kGeneralDbias) {
+                // The sums beyond the largest distance are sums of whole rows, and a row of dS sums to nothing: what it sums to is delta's
+                // error, which leaves them again by its share of P.  Row by row over the four parts of the row, then row after row.
+                float* slots = scratch + (n_diag & 1) * 16 * 64;
+                slots[(part * 4 + quad) * 64 + lane] = all_sum;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(diag_ready);
+                if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+                float over = 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) over += slots[(q * 4 + quad) * 64 + lane];
+                near_sum -= near_p * over;
+                far_sum -= far_p * over;
+                for (int o = 16; o > 0; o >>= 1) {
+                    near_sum += __shfl_xor_sync(0xffffffffu, near_sum, o);
+                    far_sum += __shfl_xor_sync(0xffffffffu, far_sum, o);
+                }
+                ++n_diag;
+                slots = scratch + (n_diag & 1) * 16 * 64;
+                if (lane == 0) {
+                    slots[2 * (part * 4 + quad)] = near_sum;
+                    slots[2 * (part * 4 + quad) + 1] = far_sum;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(diag_ready);
+                if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+                ++n_diag;
+                float* out = p.partials + (((long)w.b * p.q_heads + w.head) * p.plan.q_tiles + w.tile) * (2 * p.R + 1);
+                for (int e = (int)threadIdx.x - 64; e < 2 * p.R + 1; e += kThreads - 64) {
+                    float s = diag[kDiagPad + e];
+                    if (e == 0) {
+                        for (int q = 0; q < kDiagPad; ++q) s += diag[q];
+                        for (int q = 0; q < 16; ++q) s += slots[2 * q];
+                    }
+                    if (e == 2 * p.R) {
+                        for (int q = 0; q < kDiagPad; ++q) s += diag[kDiagPad + 2 * p.R + 1 + q];
+                        for (int q = 0; q < 16; ++q) s += slots[2 * q + 1];
+                    }
+                    out[e] = s;
+                }
+                // cleared for the next item once all have read it; its first addition is behind another wait of all
+                __syncwarp();
+                if (lane == 0) mbar_arrive(diag_ready);
+                if (!warp_wait(diag_ready, (uint32_t)n_diag & 1u, &abort_flag)) goto done;
+                ++n_diag;
+                for (int e = (int)threadIdx.x - 64; e < 2 * p.R + 1 + 2 * kDiagPad; e += kThreads - 64) diag[e] = 0.f;
+            }
+            // ------------------------------------------------------------ gradients
+            if (!warp_wait(queue.full(), queue.parity(), &abort_flag)) goto done;
+            go = queue.next<true>(lane == 0, &bx, &by, &bz);
+            if (go) v = mine_of(bx, by, bz);
+            if (w.chunks > 0 && !warp_wait(acc_final, (uint32_t)n_final++ & 1u, &abort_flag)) goto done;
+            tc_fence_after();
+            const int rows = KVS ? p.kv_len : p.q_len, row0 = row - lane;
+#pragma unroll 1
+            for (int which = 0; which < (KVS ? 2 : 1); ++which) {
+                const long* st = which == 0 ? p.s1 : p.s2;
+                uint16_t* const dst = reinterpret_cast<uint16_t*>(which == 0 ? p.out1 : p.out2) + w.b * st[0] + (KVS ? w.kv_head : w.head) * st[1] + row0 * st[2];
+                const float mul = (KVS && which == 0) ? 1.f : p.scale;         // dV is unscaled
+                const uint32_t tacc = tmem + lane_sel + (which == 0 ? kAcc1 : kAcc2);
+#pragma unroll 1
+                for (int cch = part; cch < D / 32; cch += kGroups) {        // the warpgroups share the accumulator's columns
+                    uint32_t r[32];
+                    tmem_ld_32x32(tacc + cch * 32, r);
+                    tmem_ld_wait();
+                    float o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = w.chunks == 0 ? 0.f : __uint_as_float(r[e]) * mul;
+                    uint4 piece[4];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        piece[g] = make_uint4(pack2<BF16>(o[g * 8], o[g * 8 + 1]), pack2<BF16>(o[g * 8 + 2], o[g * 8 + 3]),
+                                              pack2<BF16>(o[g * 8 + 4], o[g * 8 + 5]), pack2<BF16>(o[g * 8 + 6], o[g * 8 + 7]));
+                    if (L::kStage > 0) {
+                        store_rows64(stages + (warp - 2) * 2048, lane, piece, [&](int e) { return row0 + e < rows ? dst + e * st[2] + cch * 32 : nullptr; });
+                    } else if (row < rows) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4*>(dst + lane * st[2] + cch * 32 + g * 8) = piece[g];
+                    }
+                }
+            }
+            tc_fence_before();          // ahead of the arrivals that let the next item's first products overwrite the accumulators
         }
     }
 

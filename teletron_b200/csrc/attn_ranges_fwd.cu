@@ -163,7 +163,6 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         do {
             const Item w = item_at(bx, by, bz);
             const PlanView plan = p.plan.sample(w.b);
-            if (!queue.ask(lead, &abort_flag)) goto done;
             if (w.lo < w.hi) {
                 if (!warp_wait(q_empty, (uint32_t)n_some & 1u ^ 1u, &abort_flag)) goto done;
                 if (lead) {
@@ -203,6 +202,7 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 }
                 dirty = dirty_next;
             }
+            if (!queue.ask(lead, &abort_flag)) goto done;
             if (!warp_wait(queue.full(), queue.parity(), &abort_flag)) goto done;
             __syncwarp();
         } while (queue.next<true>(lead, &bx, &by, &bz));
