@@ -74,6 +74,14 @@ template <int V> __device__ __forceinline__ void add_product(float* x, const flo
     pairwise<V>([&](int e) { put2(x, e, __ffma2_rn(at2(y, e), at2(z, e), at2(x, e))); }, [&](int e) { x[e] += y[e] * z[e]; });
 }
 
+template <int V> __device__ __forceinline__ float total(float* x) {
+#pragma unroll
+    for (int n = V / 2; n >= 2; n /= 2)
+#pragma unroll
+        for (int e = 0; e < n; e += 2) put2(x, e, __fadd2_rn(at2(x, e), at2(x, e + n)));
+    return V > 1 ? x[0] + x[1] : x[0];
+}
+
 // A lane's share of a head: NV chunks of V pairs, each as two vectors of V elements at off0 and off1.  In the half layout the vectors hold the
 // pairs' first and second elements; in the interleaved one V / 2 whole pairs each, and full-width vectors lie one lane apart, so that a
 // group of lanes reads neighbouring addresses.  Chunks behind the rotated elements pass.
@@ -153,24 +161,33 @@ template <typename T, int V, bool WHOLE> __device__ __forceinline__ void pack(co
     }
 }
 
-// (a, b) -> (a c - b s, b c + a s) for the pairs that are rotated; the second half of a chunk of whole pairs has a flag of its own
-template <int V, bool WHOLE> __device__ __forceinline__ void rotate(float* a, float* b, const float* c, const float* s, bool rot0, bool rot1) {
+// (a, b) -> (a c - b s, b c + a s) for the pairs that are rotated (`partial`: not all are); the second half of a chunk of whole pairs has a flag
+// of its own
+template <int V, bool WHOLE> __device__ __forceinline__ void rotate(float* a, float* b, const float* c, const float* s, bool partial, bool rot0, bool rot1) {
     float y[V], z[V];
     pairwise<V>(
         [&](int e) {
-            const float2 a2 = at2(a, e), b2 = at2(b, e), c2 = at2(c, e), s2 = at2(s, e), n2 = make_float2(-s2.x, -s2.y);
-            put2(y, e, __ffma2_rn(a2, c2, __fmul2_rn(b2, n2)));
+            const float2 a2 = at2(a, e), b2 = at2(b, e), c2 = at2(c, e), s2 = at2(s, e);
+            const float2 t = __fmul2_rn(b2, s2);
+            put2(y, e, __ffma2_rn(a2, c2, make_float2(-t.x, -t.y)));
             put2(z, e, __ffma2_rn(b2, c2, __fmul2_rn(a2, s2)));
         },
         [&](int e) {
             y[e] = a[e] * c[e] - b[e] * s[e];
             z[e] = b[e] * c[e] + a[e] * s[e];
         });
+    if (partial) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const bool rot = WHOLE && e >= V / 2 ? rot1 : rot0;
+            y[e] = rot ? y[e] : a[e];
+            z[e] = rot ? z[e] : b[e];
+        }
+    }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const bool rot = WHOLE && e >= V / 2 ? rot1 : rot0;
-        a[e] = rot ? y[e] : a[e];
-        b[e] = rot ? z[e] : b[e];
+        a[e] = y[e];
+        b[e] = z[e];
     }
 }
 
@@ -218,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
         rot0[i] = WHOLE ? geo.off0[i] < 2 * P : (l + (i << log_l)) * V < P;
         rot1[i] = geo.off1[i] < 2 * P;
     }
+    const bool partial = 2 * P < (2 * V * NV << log_l);         // some lane has elements that are not rotated, or none at all
     const uint32_t cos_table = sm100::smem_u32(&angle[warp][0][0]);
     const int only = MODE != kNormBwd ? -1 : (int)blockIdx.x >= a.ctas_q ? 1 : 0;
     const int cta = (int)blockIdx.x - (only == 1 ? a.ctas_q : 0), n_ctas = only < 0 ? (int)gridDim.x : only ? (int)gridDim.x - a.ctas_q : a.ctas_q;
@@ -333,9 +351,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
                         add_product<V>(sq, f0[i], f0[i]);
                         add_product<V>(sq, f1[i], f1[i]);
                     }
-                    float ss = sq[0];
-#pragma unroll
-                    for (int e = 1; e < V; ++e) ss += sq[e];
+                    const float ss = total<V>(sq);
                     const float r = rsqrtf(group_sum(ss) * a.inv_D + a.eps);
                     float g0[NV][V], g1[NV][V], dots[V];
 #pragma unroll
@@ -354,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
                             geo.angles(cos_table, i, l, log_l, P, cs);
                             geo.angles(cos_table + 4 * (kMaxD / 2), i, l, log_l, P, sn);
                             unpack<T, V, WHOLE>(pg0[i], pg1[i], g0[i], g1[i]);
-                            rotate<V, WHOLE>(g0[i], g1[i], cs, sn, rot0[i], rot1[i]);
+                            rotate<V, WHOLE>(g0[i], g1[i], cs, sn, partial, rot0[i], rot1[i]);
                             add_product<V>(acc0[i], g0[i], f0[i]);
                             add_product<V>(acc1[i], g1[i], f1[i]);
                             mul<V>(g0[i], w0);
@@ -364,19 +380,20 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
                         }
                     }
                     if (MODE == kNormBwd) {
-                        float dot = dots[0];
-#pragma unroll
-                        for (int e = 1; e < V; ++e) dot += dots[e];
-                        dot = -group_sum(dot) * a.inv_D;
+                        const float dot = -group_sum(total<V>(dots)) * a.inv_D;
 #pragma unroll
                         for (int i = 0; i < NV; ++i) {
-                            scale<V>(f0[i], dot);
-                            scale<V>(f1[i], dot);
-#pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                f0[i][e] = r * (g0[i][e] + f0[i][e]);
-                                f1[i][e] = r * (g1[i][e] + f1[i][e]);
-                            }
+                            // r (g' w - x^ mean(g' w x^))
+                            pairwise<V>(
+                                [&](int e) {
+                                    const float2 d2 = make_float2(dot, dot), r2 = make_float2(r, r);
+                                    put2(f0[i], e, __fmul2_rn(r2, __ffma2_rn(at2(f0[i], e), d2, at2(g0[i], e))));
+                                    put2(f1[i], e, __fmul2_rn(r2, __ffma2_rn(at2(f1[i], e), d2, at2(g1[i], e))));
+                                },
+                                [&](int e) {
+                                    f0[i][e] = r * (g0[i][e] + f0[i][e] * dot);
+                                    f1[i][e] = r * (g1[i][e] + f1[i][e] * dot);
+                                });
                         }
                     }
                 }
@@ -386,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
                         float cs[V], sn[V];
                         geo.angles(cos_table, i, l, log_l, P, cs);
                         geo.angles(cos_table + 4 * (kMaxD / 2), i, l, log_l, P, sn);
-                        rotate<V, WHOLE>(f0[i], f1[i], cs, sn, rot0[i], rot1[i]);
+                        rotate<V, WHOLE>(f0[i], f1[i], cs, sn, partial, rot0[i], rot1[i]);
                     }
                     Pack<T, V> o0, o1;
                     pack<T, V, WHOLE>(f0[i], f1[i], o0, o1);

@@ -212,7 +212,7 @@ def _rows(t):
 def _like(x):
     """A gradient in ``x``'s order of heads and tokens."""
     B, H, S, D = x.shape
-    return x.new_empty((B, S, H, D)).transpose(1, 2) if x.stride(1) < x.stride(2) else x.new_empty((B, H, S, D))
+    return x.new_empty_strided((B, H, S, D), (S * H * D, D, H * D, 1)) if x.stride(1) < x.stride(2) else x.new_empty((B, H, S, D))
 
 
 def _pack(q, k, v, ranges, out, out32, lse, scale, softcap, bias):

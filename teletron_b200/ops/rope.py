@@ -203,7 +203,7 @@ def _ordered(x, token_major: bool):
     """An empty tensor of ``x``'s shape in the given order of heads and tokens: the gradient of a token-major projection's view then needs
     no transposition."""
     B, H, S, D = x.shape
-    return x.new_empty((B, S, H, D)).transpose(1, 2) if token_major else x.new_empty((B, H, S, D))
+    return x.new_empty_strided((B, H, S, D), (S * H * D, D, H * D, 1)) if token_major else x.new_empty((B, H, S, D))
 
 
 def _token_major(x) -> bool:
