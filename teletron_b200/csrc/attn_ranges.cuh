@@ -76,6 +76,19 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, sm100::mbar_wait(bar, parity, abort_flag));
 }
 
+// Grids are (tiles, heads, samples), the long runs of causal masks first.  Where all heads' long runs should come ahead of all short ones (a causal
+// mask: the last heads' long ones would be started when other CTAs run dry) the tiles are the slowest index instead of the fastest, in which
+// CTAs that run together share a head's operands.
+struct Order {
+    int tiles_last;
+    dim3 grid(int tiles, int heads, int batch) const { return tiles_last ? dim3(heads, batch, tiles) : dim3(tiles, heads, batch); }
+    __device__ __forceinline__ int tile(int x, int, int z) const { return tiles_last ? z : x; }
+    __device__ __forceinline__ int head(int x, int y, int) const { return tiles_last ? x : y; }
+    __device__ __forceinline__ int sample(int, int y, int z) const { return tiles_last ? y : z; }
+    __device__ __forceinline__ int tiles() const { return tiles_last ? (int)gridDim.z : (int)gridDim.x; }
+};
+inline Order make_order(const tt_ranges_args& a, int tiles) { return Order{a.causal && tiles <= 65535 ? 1 : 0}; }
+
 // The items of a CTA: its own block index, then ones of the launch that have not been started, so that an item's first loads and products
 // run behind the last one's.  The loading warp asks for the next item when all of one's loads are under way (at its beginning, long items were
 // claimed by CTAs that were busy while others ran dry: 21 % on a causal mask's dK dV); every role reads the answer when it is through.

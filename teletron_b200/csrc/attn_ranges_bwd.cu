@@ -32,6 +32,7 @@ enum { kPlain = 0, kGeneral = 1, kGeneralDbias = 2 };
 
 struct BwdParams {
     PlanPtr plan;
+    Order order;
     const float *lse, *delta, *bias;
     void *out1, *out2;                  // dQ / dV and dK
     long s1[3], s2[3];                  // their strides
@@ -100,11 +101,13 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     };
     auto item_at = [&](int bx, int by, int bz) {
         Item w;
-        w.b = bz;
-        w.tile = KVS ? bx : (int)gridDim.x - 1 - bx;         // the longest runs of a causal mask first
-        w.head = KVS ? by * p.group : by;
-        w.kv_head = KVS ? by : by / p.group;
-        const PlanView plan = p.plan.sample(bz);
+        const int head = p.order.head(bx, by, bz);
+        w.b = p.order.sample(bx, by, bz);
+        w.tile = p.order.tile(bx, by, bz);
+        if (!KVS) w.tile = p.order.tiles() - 1 - w.tile;
+        w.head = KVS ? head * p.group : head;
+        w.kv_head = KVS ? head : head / p.group;
+        const PlanView plan = p.plan.sample(w.b);
         int hi = 0;
         w.lo = 0;
         if (KVS) {
@@ -770,8 +773,9 @@ int launch(const tt_ranges_args& a, const Maps& m, BwdParams p, int dev, cudaStr
         p.s1[i] = KVS ? a.dv_stride[i] : a.dq_stride[i];
         p.s2[i] = KVS ? a.dk_stride[i] : 0;
     }
-    const dim3 grid(KVS ? p.plan.k_tiles : p.plan.q_tiles, KVS ? a.k_heads : a.q_heads, a.batch);
-    kern<<<grid, kThreads, L::smem(a.max_distance), st>>>(m.q, m.k, m.v, m.dout, p);
+    const int tiles = KVS ? p.plan.k_tiles : p.plan.q_tiles;
+    p.order = make_order(a, tiles);
+    kern<<<p.order.grid(tiles, KVS ? a.k_heads : a.q_heads, a.batch), kThreads, L::smem(a.max_distance), st>>>(m.q, m.k, m.v, m.dout, p);
     TT_CHECK_LAUNCH();
     return TT_OK;
 }

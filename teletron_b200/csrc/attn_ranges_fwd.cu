@@ -32,6 +32,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 struct FwdParams {
     PlanPtr plan;
+    Order order;
     void* out;
     float *out32, *lse;
     const float* bias;
@@ -98,14 +99,14 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     };
     auto item_at = [&](int bx, int by, int bz) {
         Item w;
-        w.b = bz;
-        const int x = (int)gridDim.x - 1 - bx;
+        w.b = p.order.sample(bx, by, bz);
+        const int x = p.order.tiles() - 1 - p.order.tile(bx, by, bz), head = p.order.head(bx, by, bz);
         w.qt[0] = p.pair_heads ? x : 2 * x;
         w.qt[1] = p.pair_heads ? x : 2 * x + 1;
-        w.h[0] = p.pair_heads ? 2 * by : by;
+        w.h[0] = p.pair_heads ? 2 * head : head;
         w.h[1] = p.pair_heads ? w.h[0] + 1 : w.h[0];
         w.kv_head = w.h[0] / p.group;
-        const PlanView plan = p.plan.sample(bz);
+        const PlanView plan = p.plan.sample(w.b);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             w.a[t] = make_int2(0, 0);
@@ -540,7 +541,7 @@ done:
 }
 
 template <int D, bool BF16, int MODE>
-int launch(const tt_ranges_args& a, const FwdParams& p, int dev, cudaStream_t st) {
+int launch(const tt_ranges_args& a, FwdParams p, int dev, cudaStream_t st) {
     CUtensorMap tq, tk, tv;
     int rc;
     if ((rc = tt_make_tmap_bhsd(&tq, a.q, a.batch, a.q_heads, a.q_len, D, a.q_stride, kTile)) != TT_OK) return rc;
@@ -554,8 +555,9 @@ int launch(const tt_ranges_args& a, const FwdParams& p, int dev, cudaStream_t st
         configured[dev] = true;
     }
     const int tiles = p.plan.q_tiles;
-    const dim3 grid(p.pair_heads ? tiles : (tiles + 1) / 2, p.pair_heads ? a.q_heads / 2 : a.q_heads, a.batch);
-    kern<<<grid, kThreads, Layout<D>::smem(MODE != kPlain ? a.max_distance : -1), st>>>(tq, tk, tv, p);
+    const int items = p.pair_heads ? tiles : (tiles + 1) / 2;
+    p.order = make_order(a, items);
+    kern<<<p.order.grid(items, p.pair_heads ? a.q_heads / 2 : a.q_heads, a.batch), kThreads, Layout<D>::smem(MODE != kPlain ? a.max_distance : -1), st>>>(tq, tk, tv, p);
     TT_CHECK_LAUNCH();
     return TT_OK;
 }

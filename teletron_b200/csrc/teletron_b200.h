@@ -183,6 +183,7 @@ int tt_key_ranges(int* plan, int batch, int q_len, int kv_len, int causal, const
 typedef struct {
     long struct_size;                   /* sizeof(tt_ranges_args) */
     int batch, q_heads, k_heads, q_len, kv_len, head_dim, dtype, max_distance;      /* max_distance -1: no bias */
+    int causal, reserved;               /* causal: runs grow with the query (an order of work, no mask: that is the plan's) */
     const void *q, *k, *v;              /* [batch, heads, tokens, head_dim], strides {batch, head, token} in elements, multiples of 8 */
     long q_stride[3], k_stride[3], v_stride[3];
     void* out;                          /* [batch, q_len, q_heads * head_dim] */

@@ -94,7 +94,7 @@ class Encoders:
 
     @staticmethod
     def build_default(device, dtype=torch.bfloat16, vae_tiling: bool = True, max_text_len: int = 256,
-                      preset: str = "default", text_dim: int = 4096, pooled_dim: int = 768) -> "Encoders":
+                      preset: str = "default", text_dim: int = 4096, pooled_dim: int = 768, native_attention: bool = False) -> "Encoders":
         """The real encoders (random weights unless paths are configured): a 32-layer LLaMA-style decoder, CLIP-L text
         and the 3-D causal VAE; ``preset="tiny"`` shrinks all three for CPU tests."""
         from ..models.vae import AutoencoderKLHunyuanVideo
@@ -102,11 +102,11 @@ class Encoders:
         if preset == "tiny":
             vae = AutoencoderKLHunyuanVideo(block_out_channels=(32, 32, 32, 32)).to(device, dtype).eval()
             llama = LlamaTextEncoder(max_length=max_text_len, device=device, dtype=dtype,
-                                     config=llama_config(2, text_dim, 4, 2, 2 * text_dim, 1000))
+                                     config=llama_config(2, text_dim, 4, 2, 2 * text_dim, 1000), native_attention=native_attention)
             clip = ClipTextEncoder(device=device, dtype=dtype, max_length=16, config=clip_text_config(2, pooled_dim, 4, 500, 16))
         else:
             vae = AutoencoderKLHunyuanVideo().to(device, dtype).eval()
-            llama = LlamaTextEncoder(max_length=max_text_len, device=device, dtype=dtype)
+            llama = LlamaTextEncoder(max_length=max_text_len, device=device, dtype=dtype, native_attention=native_attention)
             clip = ClipTextEncoder(device=device, dtype=dtype)
         vae.enable_tiling(vae_tiling)
         sf = 0.476986
@@ -211,7 +211,8 @@ def producer_process(args, train_valid_test_datasets_provider: Callable, encoder
     spec = spec_from_args(args)
     enc = encoders or Encoders.build_default(device, args.params_dtype, vae_tiling=bool(args.vae_tiling),
                                              max_text_len=args.encoder_max_text_len, preset=args.encoder_preset,
-                                             text_dim=args.encoder_text_dim, pooled_dim=args.encoder_pooled_dim)
+                                             text_dim=args.encoder_text_dim, pooled_dim=args.encoder_pooled_dim,
+                                             native_attention=getattr(args, "encoder_native_attention", False))
     # handshake: every consumer tells us the iteration it resumes from (training.py:208-220, producer.py:137-153)
     start = {}
     reqs = []

@@ -1,0 +1,122 @@
+"""The text encoders' self-attention on this package's operators instead of their library's.
+
+:func:`use_native_attention` exchanges the attention modules of an installed ``LlamaModel`` or ``T5EncoderModel`` for ones that keep their
+weights and call :mod:`teletron_b200.ops`: rotation by half layout with the configuration's scaling and causal masked attention with
+shared key heads (``llama``), masked attention with the learned bias of the distance (``t5``).  The reference runs both encoders through that
+library (``teletron/models/hunyuanvideo/text_encoder.py:125-238``).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch import nn
+
+from .. import ops
+
+
+def distance_buckets(max_distance: int, num_buckets: int, bidirectional: bool = True, device=None) -> torch.Tensor:
+    """Bucket of every distance ``-max_distance .. max_distance`` (key position - query position): half of a side's buckets hold one
+    distance each, the others grow with its logarithm up to ``max_distance``, from where on all share the last."""
+    d = torch.arange(-max_distance, max_distance + 1, device=device)
+    out = torch.zeros_like(d)
+    if bidirectional:
+        num_buckets //= 2
+        out = (d > 0).long() * num_buckets
+        d = d.abs()
+    else:
+        d = (-d).clamp_min(0)
+    exact = num_buckets // 2
+    large = exact + (torch.log(d.clamp_min(1).float() / exact) / math.log(max_distance / exact) * (num_buckets - exact)).long()
+    return out + torch.where(d < exact, d, large.clamp_max(num_buckets - 1))
+
+
+def prompt_ranges(mask: Optional[torch.Tensor], batch: int, length: int, causal: bool, device) -> ops.KeyRanges:
+    """Runs of keys for prompts that are padded on one side; ``mask [batch, length]`` on the host (it comes from the tokenizer)."""
+    if mask is None or bool(mask.bool().all()):
+        return ops.key_ranges(length, batch=batch, causal=causal, device=device)
+    mask = mask.bool().cpu()
+    n = mask.sum(dim=1)
+    at = torch.arange(length)
+    if torch.equal(mask, at < n[:, None]):          # padded tokens see the prompt, as in the library; nobody sees them
+        return ops.key_ranges(length, batch=batch, causal=causal, kv_valid_len=n, device=device)
+    if torch.equal(mask, at >= length - n[:, None]):
+        return ops.key_ranges(length, batch=batch, causal=causal, documents=torch.stack([length - n, torch.full_like(n, length)], dim=1), device=device)
+    raise ValueError("native attention takes prompts that are padded on one side")
+
+
+class _Shared:
+    """What the layers of one call share."""
+    ranges: Optional[ops.KeyRanges] = None
+    positions: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+
+
+class LlamaSelfAttention(nn.Module):
+    def __init__(self, inner: nn.Module, freqs: ops.Rotary, shared: _Shared):
+        super().__init__()
+        self.q_proj, self.k_proj, self.v_proj, self.o_proj = inner.q_proj, inner.k_proj, inner.v_proj, inner.o_proj
+        self.head_dim, self.scaling = inner.head_dim, inner.scaling
+        self.freqs, self.shared = freqs, shared
+
+    def forward(self, hidden_states, **_):
+        B, L, _ = hidden_states.shape
+        q, k, v = (p(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
+        q, k = ops.rotary(q, k, self.shared.positions, self.freqs)
+        return self.o_proj(ops.masked_attention(q, k, v, self.shared.ranges, scale=self.scaling)), None
+
+
+class T5SelfAttention(nn.Module):
+    def __init__(self, inner: nn.Module, shared: _Shared):
+        super().__init__()
+        self.q, self.k, self.v, self.o = inner.q, inner.k, inner.v, inner.o
+        if inner.has_relative_attention_bias:
+            self.relative_attention_bias = inner.relative_attention_bias
+        self.head_dim, self.shared = inner.key_value_proj_dim, shared
+
+    def forward(self, hidden_states, **_):
+        B, L, _ = hidden_states.shape
+        q, k, v = (p(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2) for p in (self.q, self.k, self.v))
+        o = ops.masked_attention(q, k, v, self.shared.ranges, scale=1.0, distance_bias=self.shared.bias)
+        return self.o(o.to(self.o.weight.dtype)), None
+
+
+class _NativeLlama:
+    def __init__(self, model):
+        self.shared, cfg = _Shared(), model.config
+        rope = dict(getattr(cfg, "rope_parameters", None) or {})
+        head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+        freqs = ops.rotary_frequencies(int(head_dim * rope.get("partial_rotary_factor", 1.0)), float(rope.get("rope_theta", getattr(cfg, "rope_theta", 10000.0))),
+                                       scaling=rope, device=model.embed_tokens.weight.device)
+        for layer in model.layers:
+            layer.self_attn = LlamaSelfAttention(layer.self_attn, freqs, self.shared)
+
+    def prepare(self, mask, batch, length, device):
+        self.shared.positions = torch.arange(length, device=device, dtype=torch.int32)
+        self.shared.ranges = prompt_ranges(mask, batch, length, True, device)
+
+
+class _NativeT5:
+    def __init__(self, model):
+        self.shared, cfg = _Shared(), model.config
+        for block in model.encoder.block:
+            block.layer[0].SelfAttention = T5SelfAttention(block.layer[0].SelfAttention, self.shared)
+        self.table = model.encoder.block[0].layer[0].SelfAttention.relative_attention_bias
+        self.buckets = distance_buckets(cfg.relative_attention_max_distance, cfg.relative_attention_num_buckets, device=self.table.weight.device)
+
+    def prepare(self, mask, batch, length, device):
+        self.shared.ranges = prompt_ranges(mask, batch, length, False, device)
+        self.shared.bias = self.table.weight[self.buckets].t().float().contiguous()
+
+
+def use_native_attention(model):
+    """Exchanges the attention modules of a ``LlamaModel`` or ``T5EncoderModel`` in place.  Returns an object whose
+    ``prepare(mask, batch, length, device)`` has to be called ahead of each call of the model, with the tokenizer's mask or None."""
+    kind = type(model).__name__
+    if kind == "LlamaModel":
+        return _NativeLlama(model)
+    if kind == "T5EncoderModel":
+        return _NativeT5(model)
+    raise ValueError(f"native attention is there for LlamaModel and T5EncoderModel, not for {kind}")

@@ -51,10 +51,17 @@ def clip_text_config(num_layers: int = 12, hidden: int = 768, heads: int = 12, v
                           num_attention_heads=heads, max_position_embeddings=max_len, projection_dim=hidden)
 
 
-class LlamaTextEncoder:
-    """``prompts -> (last_hidden_state [B, L, hidden], mask [B, L])`` (mode ``llama`` of the reference's PromptEncoder)."""
+def _native_attention(model):
+    from .text_attention import use_native_attention
+    return use_native_attention(model)
 
-    def __init__(self, model_path: Optional[str] = None, max_length: int = 256, device=None, dtype=torch.bfloat16, config=None):
+
+class LlamaTextEncoder:
+    """``prompts -> (last_hidden_state [B, L, hidden], mask [B, L])`` (mode ``llama`` of the reference's PromptEncoder).
+    ``native_attention``: rotation and attention by this package's kernels (:mod:`.text_attention`)."""
+
+    def __init__(self, model_path: Optional[str] = None, max_length: int = 256, device=None, dtype=torch.bfloat16, config=None,
+                 native_attention: bool = False):
         from transformers import LlamaModel
         self.max_length = max_length
         self.device = device
@@ -71,6 +78,7 @@ class LlamaTextEncoder:
             self._hash = HashTokenizer(cfg.vocab_size, max_length)
         for p in self.model.parameters():
             p.requires_grad_(False)
+        self.native = _native_attention(self.model) if native_attention else None
 
     def tokenize(self, prompts: Sequence[str]):
         if self._hash is not None:
@@ -81,6 +89,10 @@ class LlamaTextEncoder:
     @torch.no_grad()
     def __call__(self, prompts: Sequence[str]) -> Tuple[torch.Tensor, torch.Tensor]:
         ids, mask = self.tokenize(prompts)
+        if self.native is not None:
+            device = self.model.embed_tokens.weight.device
+            self.native.prepare(mask, *ids.shape, device)
+            return self.model(input_ids=ids.to(device), use_cache=False).last_hidden_state, mask.to(device).bool()
         ids, mask = ids.to(self.device), mask.to(self.device)
         out = self.model(input_ids=ids, attention_mask=mask)
         return out.last_hidden_state, mask.bool()
@@ -126,7 +138,7 @@ def t5_config(num_layers: int = 24, hidden: int = 4096, heads: int = 64, ffn: in
 class _HFTextModel:
     """One Hugging Face text model + tokenizer (a hashing stand-in when no weights are given)."""
 
-    def __init__(self, kind: str, model_path: Optional[str], max_length: int, device, dtype, config=None):
+    def __init__(self, kind: str, model_path: Optional[str], max_length: int, device, dtype, config=None, native_attention: bool = False):
         import transformers
         cls = {"clip": transformers.CLIPTextModel, "clip_proj": transformers.CLIPTextModelWithProjection,
                "t5": transformers.T5EncoderModel}[kind]
@@ -143,6 +155,7 @@ class _HFTextModel:
             self._hash = HashTokenizer(cfg.vocab_size, max_length, pad_id=0)
         for p in self.model.parameters():
             p.requires_grad_(False)
+        self.native = _native_attention(self.model) if native_attention else None
 
     def tokenize(self, prompts, max_length=None):
         n = max_length or self.max_length
@@ -152,6 +165,10 @@ class _HFTextModel:
         return t.input_ids, t.attention_mask
 
     def __call__(self, ids, mask, **kw):
+        if self.native is not None:
+            device = next(self.model.parameters()).device
+            self.native.prepare(mask, *ids.shape, device)
+            return self.model(input_ids=ids.to(device), **kw)
         return self.model(input_ids=ids.to(self.device), attention_mask=None if mask is None else mask.to(self.device), **kw)
 
 
@@ -167,18 +184,21 @@ class PromptEncoder:
 
     Returns ``(embeds, masks)``; ``masks`` is ``None`` unless ``with_attention_mask`` (then the masks are also passed to
     the encoders, as in the reference).  Without ``model_path`` the models are built from configs with random weights and a
-    hashing tokenizer (``configs``: one config per tower)."""
+    hashing tokenizer (``configs``: one config per tower).  ``native_attention`` (``llama``, ``t5``): this package's kernels."""
 
     MODES = ("llama", "clip_text", "clip_text_proj", "clip_text_and_proj", "t5")
 
     def __init__(self, mode: str, model_path: Optional[str] = None, device=None, dtype=None, max_length: Optional[int] = None,
-                 configs: Optional[Sequence] = None):
+                 configs: Optional[Sequence] = None, native_attention: bool = False):
         if dtype is None:
             dtype = torch.float16 if (device is not None and "cuda" in str(device)) else torch.float32
         if isinstance(dtype, str):
             dtype = getattr(torch, dtype)
         if mode not in self.MODES:
             raise ValueError(f"Unsupported mode: {mode}")
+        if native_attention and mode not in ("llama", "t5"):
+            raise ValueError(f"native attention is there for the modes llama and t5, not for {mode}")
+        self.native_attention = native_attention
         self.mode, self.model_path, self.device, self.dtype = mode, model_path, device, dtype
         self.max_length = max_length or (256 if mode in ("llama", "t5") else 77)
         self.configs = list(configs) if configs else None
@@ -197,13 +217,15 @@ class PromptEncoder:
             return
         paths, cfg = self._paths(), (self.configs or [None, None]) + [None]
         if self.mode == "llama":
-            self.encoders = [LlamaTextEncoder(paths[0], self.max_length, self.device, self.dtype, config=cfg[0])]
+            self.encoders = [LlamaTextEncoder(paths[0], self.max_length, self.device, self.dtype, config=cfg[0],
+                                              native_attention=self.native_attention)]
         elif self.mode == "clip_text_and_proj":
             self.encoders = [_HFTextModel("clip", paths[0], self.max_length, self.device, self.dtype, cfg[0]),
                              _HFTextModel("clip_proj", paths[1], self.max_length, self.device, self.dtype, cfg[1])]
         else:
             kind = {"clip_text": "clip", "clip_text_proj": "clip_proj", "t5": "t5"}[self.mode]
-            self.encoders = [_HFTextModel(kind, paths[0], self.max_length, self.device, self.dtype, cfg[0])]
+            self.encoders = [_HFTextModel(kind, paths[0], self.max_length, self.device, self.dtype, cfg[0],
+                                          native_attention=self.native_attention)]
 
     @torch.no_grad()
     def __call__(self, prompt, max_length: Optional[int] = None, with_attention_mask: bool = False):

@@ -38,6 +38,7 @@ class KeyRanges:
     behind: torch.Tensor
     query_start: Optional[torch.Tensor]
     plan: Optional[torch.Tensor]
+    causal: bool = False            # runs grow with the query: what the kernels begin with
 
     @property
     def device(self):
@@ -131,7 +132,7 @@ def key_ranges(q_len: int, kv_len: Optional[int] = None, *, batch: int = 1, caus
         start = torch.full((batch,), start_int, dtype=torch.int32, device=device)
     if device.type != "cuda" or not _lib.available() or min(q_len, kv_len, batch) == 0:
         first, behind = _runs(q_len, kv_len, batch, causal, documents, prefix_len, prefix, kv_valid, start, device)
-        return KeyRanges(batch, q_len, kv_len, first, behind, start, None)
+        return KeyRanges(batch, q_len, kv_len, first, behind, start, None, bool(causal))
     at = _layout(batch, q_len, kv_len)
     with torch.cuda.device(device):
         plan = torch.empty(at.ints, dtype=torch.int32, device=device)
@@ -141,7 +142,7 @@ def key_ranges(q_len: int, kv_len: Optional[int] = None, *, batch: int = 1, caus
              ptr(kv_valid), ptr(start), stream())
     rows = batch * q_len
     return KeyRanges(batch, q_len, kv_len, plan[at.first:at.first + rows].view(batch, q_len), plan[at.behind:at.behind + rows].view(batch, q_len),
-                     start, plan)
+                     start, plan, bool(causal))
 
 
 class _Layout(ctypes.Structure):
@@ -190,9 +191,9 @@ def supported(q, k, v, ranges, distance_bias) -> bool:
 
 # ------------------------------------------------------------------------------------------------ native calls
 
-_HEAD = struct.Struct("@l iiii iiii PPP 9l PPP PP ff")           # everything that the forward kernel reads but the status word
+_HEAD = struct.Struct("@l iiii iiii ii PPP 9l PPP PP ff")           # everything that the forward kernel reads but the status word
 _TAIL = struct.Struct("@PP PPP 9l PP P")
-_ARGS = struct.Struct("@l iiii iiii PPP 9l PPP PP ff PP PPP 9l PP P")
+_ARGS = struct.Struct("@l iiii iiii ii PPP 9l PPP PP ff PP PPP 9l PP P")
 _NO_BACKWARD = bytes(_TAIL.size - 16)
 _SCRATCH = struct.Struct("@PP")
 FEW_ROWS = 32           # queries of a group that the kernels for few queries take
@@ -217,7 +218,7 @@ def _like(x):
 
 def _pack(q, k, v, ranges, out, out32, lse, scale, softcap, bias):
     B, hq, n, D = q.shape
-    return _HEAD.pack(_ARGS.size, B, hq, k.shape[1], n, k.shape[2], D, _DTYPES[q.dtype], -1 if bias is None else bias.shape[1] >> 1,
+    return _HEAD.pack(_ARGS.size, B, hq, k.shape[1], n, k.shape[2], D, _DTYPES[q.dtype], -1 if bias is None else bias.shape[1] >> 1, ranges.causal, 0,
                       q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
                       out.data_ptr(), 0 if out32 is None else out32.data_ptr(), lse.data_ptr(), ranges.plan.data_ptr(),
                       0 if bias is None else bias.data_ptr(), scale, softcap)

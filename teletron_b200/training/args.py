@@ -106,6 +106,8 @@ def _add_parallel_args(p):
     g.add_argument("--encoder-text-dim", type=int, default=None)
     g.add_argument("--encoder-pooled-dim", type=int, default=None)
     g.add_argument("--encoder-max-text-len", type=int, default=256)
+    g.add_argument("--encoder-native-attention", action="store_true",
+                   help="rotation and attention of the LLaMA text encoder by this package's kernels instead of its library's")
     g.add_argument("--nccl-communicator-config-path", type=str, default=None,
                    help="YAML file {group kind: {cga_cluster_size, max_ctas, min_ctas}} applied to the NCCL communicators of those groups")
     g.add_argument("--tp-comm-overlap", action="store_true",

@@ -92,7 +92,7 @@ def test_gradients_against_differences():
     d = torch.randn(4, 5)
     step = 2.0 ** -6
     ends = [(ops.masked_attention(q, k, v, r, distance_bias=bias.detach() + s * d) * w).sum() for s in (step, -step)]
-    assert abs(float(ends[0] - ends[1]) / (2 * step) - float((g * d).sum())) < 1e-2 * float(g.norm() * d.norm())
+    assert abs(float((ends[0] - ends[1]).detach()) / (2 * step) - float((g * d).sum())) < 1e-2 * float(g.norm() * d.norm())
 
 
 def test_empty_operands():
@@ -116,7 +116,7 @@ def test_native_arguments_are_checked_ahead_of_any_launch():
 
     def pack(scale=1.0, softcap=0.0, plan=256, bias=0, dout=0, **kw):
         f = {**fields, **kw}
-        return A._ARGS.pack(f["size"], f["batch"], f["q_heads"], f["k_heads"], f["q_len"], f["kv_len"], f["head_dim"], f["dtype"], f["distance"],
+        return A._ARGS.pack(f["size"], f["batch"], f["q_heads"], f["k_heads"], f["q_len"], f["kv_len"], f["head_dim"], f["dtype"], f["distance"], 0, 0,
                             256, 256, 256, *[64] * 9, 256, 0, 256, plan, bias, scale, softcap, dout, 0, 0, 0, 0, *[0] * 9, 0, 0, 256)
 
     for kw, code in ((dict(size=8), 1), (dict(batch=0), 1), (dict(batch=65536), 1), (dict(k_heads=3), 1), (dict(q_len=0), 1), (dict(kv_len=2 ** 30 + 1), 1),

@@ -272,7 +272,7 @@ def test_projection_rotation_and_attention_together():
     want = (ref, *torch.autograd.grad(ref, (xd, wd), dout.double()))
     for a, b in zip(got, want):
         # nine roundings to 2^-8 between input and gradient, each of independent elements: a relative norm of 9 * 2^-8 bounds them all
-        assert float((a.double() - b).norm() / b.norm()) < 9 * 2 ** -8
+        assert float((a.detach().double() - b.detach()).norm() / b.detach().norm()) < 9 * 2 ** -8
 
 
 @pytest.mark.parametrize("D,dtype", [(64, BF16), (128, FP16), (128, BF16)])

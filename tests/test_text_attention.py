@@ -1,0 +1,117 @@
+"""The text encoders on this package's rotation and attention against the same weights on their library's."""
+
+import copy
+
+import pytest
+import torch
+
+from teletron_b200.models.text_attention import distance_buckets, prompt_ranges, use_native_attention
+from teletron_b200.models.text_encoders import LlamaTextEncoder, PromptEncoder, clip_text_config, llama_config, t5_config
+
+PROMPTS = ["a short prompt", "another slightly longer prompt here with words", "x"]
+
+
+def _llama(**kw):
+    torch.manual_seed(0)
+    cfg = llama_config(3, 64, 4, 2, 128, 1000)
+    return cfg, LlamaTextEncoder(max_length=24, dtype=torch.float32, config=cfg, **kw)
+
+
+@pytest.mark.parametrize("scaling", [None, dict(rope_type="llama3", factor=4.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                                                original_max_position_embeddings=16, rope_theta=500000.0)])
+def test_llama_states_equal_the_librarys(scaling):
+    torch.manual_seed(0)
+    cfg = llama_config(3, 64, 4, 2, 128, 1000)
+    if scaling is not None:
+        cfg.rope_parameters = scaling
+    plain = LlamaTextEncoder(max_length=24, dtype=torch.float32, config=cfg)
+    native = copy.deepcopy(plain)
+    native.native = use_native_attention(native.model)
+    want, mask = plain(PROMPTS)
+    got, got_mask = native(PROMPTS)
+    assert torch.equal(mask, got_mask)
+    # fp32 throughout: three layers of products over at most 128 terms, states of the order of 1
+    assert torch.allclose(got, want, atol=2e-4, rtol=0)
+    # a prompt by itself, not padded
+    assert torch.allclose(native(PROMPTS[:1])[0][:, :4], want[:1, :4], atol=2e-4, rtol=0)
+
+
+def test_t5_states_equal_the_librarys():
+    torch.manual_seed(1)
+    plain = PromptEncoder("t5", max_length=200, dtype=torch.float32, configs=[t5_config(2, 32, 4, 64, 300)])
+    plain.load_model()
+    native = copy.deepcopy(plain)
+    native.encoders[0].native = use_native_attention(native.encoders[0].model)
+    for p in (plain, native):           # a table whose entries differ
+        w = p.encoders[0].model.encoder.block[0].layer[0].SelfAttention.relative_attention_bias.weight
+        w.copy_(torch.linspace(-2, 2, w.numel()).view_as(w))
+    for with_mask in (False, True):
+        want, mask = plain(PROMPTS, with_attention_mask=with_mask)
+        got, _ = native(PROMPTS, with_attention_mask=with_mask)
+        assert torch.allclose(got, want, atol=2e-4, rtol=0)
+
+
+def test_buckets_are_the_librarys():
+    from transformers.models.t5.modeling_t5 import T5Attention
+    for R, n, both in ((128, 32, True), (64, 16, True), (128, 32, False), (20, 8, False)):
+        d = torch.arange(-R, R + 1)
+        want = T5Attention._relative_position_bucket(d, bidirectional=both, num_buckets=n, max_distance=R)
+        assert torch.equal(distance_buckets(R, n, both), want)
+
+
+def test_prompts_padded_on_either_side():
+    right = torch.tensor([[1, 1, 0, 0], [1, 1, 1, 1]])
+    r = prompt_ranges(right, 2, 4, True, "cpu")
+    assert r.behind.tolist() == [[1, 2, 2, 2], [1, 2, 3, 4]] and not bool(r.first.any())
+    r = prompt_ranges(right.flip(1), 2, 4, True, "cpu")
+    assert r.first.tolist() == [[0, 0, 2, 2], [0, 0, 0, 0]] and r.behind.tolist() == [[0, 0, 3, 4], [1, 2, 3, 4]]
+    with pytest.raises(ValueError):
+        prompt_ranges(torch.tensor([[1, 0, 1, 0]]), 1, 4, True, "cpu")
+
+
+def test_refusals_and_flag():
+    with pytest.raises(ValueError):
+        PromptEncoder("clip_text", native_attention=True)
+    with pytest.raises(ValueError):
+        use_native_attention(torch.nn.Linear(2, 2))
+    cfg, enc = _llama(native_attention=True)
+    assert enc.native is not None and _llama()[1].native is None
+    emb, mask = PromptEncoder("llama", max_length=10, dtype=torch.float32, configs=[cfg], native_attention=True)(PROMPTS, with_attention_mask=True)
+    assert emb.shape == (3, 10, 64) and mask.shape == (3, 10)
+    from teletron_b200.training.args import parse_args
+    assert parse_args(argv=["--encoder-native-attention"]).encoder_native_attention is True
+    assert clip_text_config() is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_llama_on_the_kernels(dtype):
+    """Heads of 128, shared, padded prompts; nearer to the fp32 states than a fiftieth, as the library's own are."""
+    torch.manual_seed(2)
+    cfg = llama_config(2, 512, 4, 2, 1024, 1000)
+    exact = LlamaTextEncoder(max_length=256, dtype=torch.float32, config=cfg, device="cuda")
+    native = copy.deepcopy(exact)
+    native.model.to(dtype)
+    native.native = use_native_attention(native.model)
+    from teletron_b200.ops import _lib
+    want, mask = exact(PROMPTS)
+    before = _lib.LAUNCHES
+    got, _ = native(PROMPTS)
+    assert _lib.LAUNCHES - before == 2 + 2 * 2          # the plan, then rotation and attention of each layer
+    assert float((got.float() - want)[mask].norm() / want[mask].norm()) < 0.02
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_t5_on_the_kernels(dtype):
+    torch.manual_seed(3)
+    exact = PromptEncoder("t5", max_length=300, dtype=torch.float32, configs=[t5_config(2, 256, 4, 512, 300)], device="cuda")
+    exact.load_model()
+    native = copy.deepcopy(exact)
+    native.encoders[0].model.to(dtype)
+    native.encoders[0].native = use_native_attention(native.encoders[0].model)
+    long = [" ".join(f"w{i}" for i in range(250)), "a b c"]
+    want, masks = exact(long, with_attention_mask=True)
+    got, _ = native(long, with_attention_mask=True)
+    keep = masks.bool().to(want.device)
+    assert float((got.float() - want)[keep].norm() / want[keep].norm()) < 0.02
