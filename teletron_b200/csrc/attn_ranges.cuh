@@ -198,9 +198,13 @@ __device__ __forceinline__ float2 cap_small(const Cap& k, float2 z) {
 __device__ __forceinline__ float cap_any(const Cap& k, float z) { return k.out * (1.f - __fdividef(2.f, 1.f + exp2f(z * k.two_u))); }
 // whether the largest magnitude of N scores of every lane is one of the series
 template <int N> __device__ __forceinline__ bool all_small(const Cap& k, const uint32_t* z) {
-    float m = 0.f;
+    float m = 0.f, m2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(__uint_as_float(z[i])));
+    for (int i = 0; i < N; i += 4) {        // three-input maxima
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(__uint_as_float(z[i]))), "f"(fabsf(__uint_as_float(z[i + 1]))));
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(m2) : "f"(fabsf(__uint_as_float(z[i + 2]))), "f"(fabsf(__uint_as_float(z[i + 3]))));
+    }
+    m = fmaxf(m, m2);
     return __all_sync(0xffffffffu, m <= k.small);
 }
 

@@ -15,6 +15,8 @@
 // 0 loads, warp 1 issues, sixteen warps turn T1, T2 into P and dS (a thread: one stationary row, 32 streamed ones).
 #include <limits.h>
 
+#include <type_traits>
+
 #include "attn_ranges.cuh"
 
 namespace {
@@ -28,7 +30,8 @@ constexpr int kThreads = 64 + kGroups * 128;
 constexpr int kSlab = kTile * 128;
 constexpr int kDiagPad = 256;                               // a tile that is not wholly beyond the largest distance reaches at most 254 past it
 
-enum { kPlain = 0, kGeneral = 1, kGeneralDbias = 2 };
+// scores: scaled; capped; with a bias and maybe a cap; the same for a bias that gets a gradient
+enum { kPlain = 0, kCapped = 1, kGeneral = 2, kGeneralDbias = 3 };
 
 struct BwdParams {
     PlanPtr plan;
@@ -134,6 +137,10 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         return Chunk{w.head + g, w.lo + c - g * w.per_head};
     };
     auto lds4 = [](uint32_t at, float4& v) { asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at)); };
+    auto slope_of = [&](float2 y) {         // of the cap, from capped scores in the log2 domain
+        const float2 t = __fmul2_rn(y, make_float2(p.cap.inv_out, p.cap.inv_out));
+        return __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
+    };
     // a streamed tile with rows that no run reaches: queries that see nothing, keys that nothing sees
     auto is_dirty = [&](const Item& w, const PlanView& plan, int c) {
         return c < w.chunks ? (KVS ? plan.q_tiles[chunk_at(w, c).t].w == 0 : plan.dirty[w.lo + c] != 0) : false;
@@ -422,7 +429,7 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 bool at_end = false, inside = false;
                 float end_bias = 0.f;
                 const float* bias_row = nullptr;
-                if (MODE != kPlain && p.R >= 0) {
+                if (MODE >= kGeneral) {
                     bias_row = p.bias + (long)ch.head * (2 * p.R + 1) + p.R;
                     const int w0 = __shfl_sync(0xffffffffu, pos0, 0), w31 = __shfl_sync(0xffffffffu, pos0, 31);
                     const int least = KVS ? w0 - 31 : w31, most = KVS ? w31 : w0 + 31;
@@ -430,69 +437,79 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     inside = least >= -p.R && most <= p.R;
                     if (at_end) end_bias = bias_row[least >= p.R ? p.R : -p.R] * kLog2e;
                 }
-                uint32_t tk[MODE != kPlain ? 16 : 1], a[32];
+                uint32_t tk[MODE >= kGeneral ? 16 : 1], a[32];
                 if (!warp_wait(s_full, par, &abort_flag)) goto done;
                 tc_fence_after();
                 tmem_ld_32x32(t1, a);
                 tmem_ld_wait();
-                if (MODE != kPlain) {           // raw scores to the log2 domain
-                    if (p.cap.out != 0.f) {
-                        const bool small = all_small<32>(p.cap, a);
+                // raw scores to the log2 domain (kPlain: with the exponential)
+                if (MODE == kCapped || (MODE >= kGeneral && p.cap.out != 0.f)) {
+                    if (all_small<32>(p.cap, a)) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float2 z = make_float2(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]));
-                            const float2 y = small ? cap_small(p.cap, z) : make_float2(cap_any(p.cap, z.x), cap_any(p.cap, z.y));
-                            const float2 t = __fmul2_rn(y, make_float2(p.cap.inv_out, p.cap.inv_out));
-                            const float2 slope = __ffma2_rn(t, make_float2(-t.x, -t.y), make_float2(1.f, 1.f));
-                            // the cap's slope in fp16: 2^-11 of a factor that is rounded to 16 bits with its dS below
-                            tk[e] = pack2<false>(slope.x, slope.y);
-                            a[2 * e] = __float_as_uint(y.x);
-                            a[2 * e + 1] = __float_as_uint(y.y);
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 y = cap_small(p.cap, make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])));
+                            a[e] = __float_as_uint(y.x);
+                            a[e + 1] = __float_as_uint(y.y);
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * p.scale_log2);
+                        for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(cap_any(p.cap, __uint_as_float(a[e])));
                     }
-                    if (p.R >= 0) {
-                        if (at_end) {
+                    if (MODE >= kGeneral) {         // the slope ahead of the bias, in fp16: 2^-11 of a factor that is rounded to 16 bits with its dS below
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) + end_bias);
-                        } else if (inside) {
-                            const float* entry = bias_row + pos0;
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(fmaf(__ldg(KVS ? entry - e : entry + e), kLog2e, __uint_as_float(a[e])));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                a[e] = __float_as_uint(fmaf(__ldg(bias_row + max(-p.R, min(p.R, KVS ? pos0 - e : pos0 + e))), kLog2e, __uint_as_float(a[e])));
+                        for (int e = 0; e < 16; ++e) {
+                            const float2 f = slope_of(make_float2(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1])));
+                            tk[e] = pack2<false>(f.x, f.y);
                         }
                     }
+                } else if (MODE >= kGeneral) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) * p.scale_log2);
                 }
-                // P in 32 bits over the scores
-                if (KVS && !warp_wait(b1_full(i % kRing1), (uint32_t)(i / kRing1) & 1u, &abort_flag)) goto done;       // has the copied lse: long complete
+                if (MODE >= kGeneral) {
+                    if (at_end) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    float4 l4 = make_float4(v.lse, v.lse, v.lse, v.lse);
-                    if (KVS) lds4(sLse + ((i % kRing1) * kTile + part * kCols + 4 * q) * 4, l4);
+                        for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__uint_as_float(a[e]) + end_bias);
+                    } else if (inside) {
+                        const float* entry = bias_row + pos0;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int e = 4 * q + 2 * h;
-                        const float2 s2 = make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1]));
-                        const float2 n2 = h ? make_float2(-l4.z, -l4.w) : make_float2(-l4.x, -l4.y);
-                        const float2 y = MODE == kPlain ? __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), n2) : __fadd2_rn(s2, n2);
-                        a[e] = __float_as_uint(exp2f(y.x));
-                        a[e + 1] = __float_as_uint(exp2f(y.y));
+                        for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(fmaf(__ldg(KVS ? entry - e : entry + e), kLog2e, __uint_as_float(a[e])));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            a[e] = __float_as_uint(fmaf(__ldg(bias_row + max(-p.R, min(p.R, KVS ? pos0 - e : pos0 + e))), kLog2e, __uint_as_float(a[e])));
                     }
                 }
-                if (!clean) {
+                if (KVS && !warp_wait(b1_full(i % kRing1), (uint32_t)(i / kRing1) & 1u, &abort_flag)) goto done;       // has the copied lse: long complete
+                // P in 32 bits over the scores.  For the product with dO it is rounded, half a step of the operands' type; for dS it stays, behind a
+                // cap alone times the cap's slope.
+                uint32_t pk[KVS ? 16 : 1];
+                auto exponentials = [&](auto whole) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!(see >> e & 1u)) a[e] = 0u;
-                }
-                if (KVS) {          // rounded for the product only: half a step of the operands' type
-                    uint32_t pk[16];
+                    for (int q = 0; q < 8; ++q) {
+                        float4 l4 = make_float4(v.lse, v.lse, v.lse, v.lse);
+                        if (KVS) lds4(sLse + ((i % kRing1) * kTile + part * kCols + 4 * q) * 4, l4);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) pk[e] = pack2<BF16>(__uint_as_float(a[2 * e]), __uint_as_float(a[2 * e + 1]));
+                        for (int h = 0; h < 2; ++h) {
+                            const int e = 4 * q + 2 * h;
+                            const float2 s2 = make_float2(__uint_as_float(a[e]), __uint_as_float(a[e + 1]));
+                            const float2 n2 = h ? make_float2(-l4.z, -l4.w) : make_float2(-l4.x, -l4.y);
+                            const float2 y = MODE == kPlain ? __ffma2_rn(s2, make_float2(p.scale_log2, p.scale_log2), n2) : __fadd2_rn(s2, n2);
+                            float2 pr = make_float2(exp2f(y.x), exp2f(y.y)), f = MODE == kCapped ? slope_of(s2) : make_float2(1.f, 1.f);
+                            if (!whole) {       // P and slope of a key or a query that no run reaches may be anything
+                                if (!(see >> e & 1u)) pr.x = f.x = 0.f;
+                                if (!(see >> (e + 1) & 1u)) pr.y = f.y = 0.f;
+                            }
+                            if (KVS) pk[e >> 1] = pack2<BF16>(pr.x, pr.y);
+                            if (MODE == kCapped) pr = __fmul2_rn(pr, f);
+                            a[e] = __float_as_uint(pr.x);
+                            a[e + 1] = __float_as_uint(pr.y);
+                        }
+                    }
+                };
+                if (clean) exponentials(std::true_type());
+                else exponentials(std::false_type());
+                if (KVS) {
                     tmem_st_32x16(t1, pk);
                     tmem_st_wait();
                 }
@@ -530,17 +547,17 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                             const float2 n2 = h ? make_float2(-d4.z, -d4.w) : make_float2(-d4.x, -d4.y);
                             float2 ds = __fmul2_rn(make_float2(__uint_as_float(a[k]), __uint_as_float(a[k + 1])),
                                                    __fadd2_rn(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), n2));
-                            float2 slope = make_float2(1.f, 1.f);
-                            if (MODE != kPlain && p.cap.out != 0.f) slope = unpack2<false>(tk[k >> 1]);
-                            if (!clean) {           // dP and the slope of a key or a query that no run reaches may be anything
-                                if (!(see >> k & 1u)) ds.x = slope.x = 0.f;
-                                if (!(see >> (k + 1) & 1u)) ds.y = slope.y = 0.f;
+                            float2 f = make_float2(1.f, 1.f);
+                            if (MODE >= kGeneral && p.cap.out != 0.f) f = unpack2<false>(tk[k >> 1]);
+                            if (!clean) {           // dP and slope of a key or a query that no run reaches may be anything
+                                if (!(see >> k & 1u)) ds.x = f.x = 0.f;
+                                if (!(see >> (k + 1) & 1u)) ds.y = f.y = 0.f;
                             }
                             if (MODE == kGeneralDbias) {
                                 a[k] = __float_as_uint(ds.x);
                                 a[k + 1] = __float_as_uint(ds.y);
                             }
-                            if (MODE != kPlain) ds = __fmul2_rn(ds, slope);
+                            if (MODE >= kGeneral) ds = __fmul2_rn(ds, f);
                             // rounded to the operands' type, as the products take it: half a step of each dS
                             dk[e >> 1] = pack2<BF16>(ds.x, ds.y);
                         }
@@ -796,10 +813,13 @@ int run(const tt_ranges_args& a, const BwdParams& p, int dev, int sms, cudaStrea
     else
         ranges_delta_kernel<D, BF16, false><<<grid, 256, 0, st>>>(p.plan, (const uint16_t*)a.dout, a.out, a.delta, rows, a.q_len, a.q_heads);
     TT_CHECK_LAUNCH();
-    const bool gen = a.softcap > 0.f || a.max_distance >= 0;
-    rc = gen ? launch<D, BF16, true, kGeneral>(a, m, p, dev, st) : launch<D, BF16, true, kPlain>(a, m, p, dev, st);
+    const bool bias = a.max_distance >= 0, cap = a.softcap > 0.f;
+    rc = bias ? launch<D, BF16, true, kGeneral>(a, m, p, dev, st)
+         : cap ? launch<D, BF16, true, kCapped>(a, m, p, dev, st) : launch<D, BF16, true, kPlain>(a, m, p, dev, st);
     if (rc != TT_OK) return rc;
-    if (a.dbias == nullptr) return gen ? launch<D, BF16, false, kGeneral>(a, m, p, dev, st) : launch<D, BF16, false, kPlain>(a, m, p, dev, st);
+    if (a.dbias == nullptr)
+        return bias ? launch<D, BF16, false, kGeneral>(a, m, p, dev, st)
+               : cap ? launch<D, BF16, false, kCapped>(a, m, p, dev, st) : launch<D, BF16, false, kPlain>(a, m, p, dev, st);
     if ((rc = launch<D, BF16, false, kGeneralDbias>(a, m, p, dev, st)) != TT_OK) return rc;
     const int entries = 2 * a.max_distance + 1;
     ranges_dbias_kernel<<<dim3((entries + 31) / 32, a.q_heads), 1024, 0, st>>>(a.partials, a.dbias, a.batch, a.q_heads, p.plan.q_tiles, entries);
