@@ -507,7 +507,10 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         }
                     }
                 };
-                if (clean) exponentials(std::true_type());
+                // With stationary queries one form for both is the faster one (3430 -> 2960 us at 32656 packed tokens), with stationary keys two are
+                // (4556 against 4658).
+                if (!KVS) exponentials(clean);
+                else if (clean) exponentials(std::true_type());
                 else exponentials(std::false_type());
                 if (KVS) {
                     tmem_st_32x16(t1, pk);

@@ -376,7 +376,9 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 for (int c = 0; c < kTile / 32; ++c) tmem_ld_32x32(tS + c * 32, r + c * 32);
                 tmem_ld_wait();
                 if (GEN) {
+                    float factor = p.scale_log2;            // what is left of the scale
                     if (p.cap.out != 0.f) {
+                        factor = 1.f;
                         if (all_small<kTile>(p.cap, r)) {
 #pragma unroll
                             for (int i = 0; i < kTile; i += 2) {
@@ -388,21 +390,29 @@ ranges_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                             for (int i = 0; i < kTile; ++i) r[i] = __float_as_uint(cap_any(p.cap, __uint_as_float(r[i])));
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kTile; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * p.scale_log2);
                     }
-                    if (p.R >= 0) {
-                        const float* zero = my_table + kPad + p.R;          // entry of distance 0
-                        const int pos0 = pos - lane;                        // of the warp's first row
-                        if (k0 + kTile - 1 - pos0 <= -p.R || k0 - pos0 - 31 >= p.R) {       // all at the table's end
-                            const float far = zero[k0 - pos0 > 0 ? p.R : -p.R];
+                    const float2 f2 = make_float2(factor, factor);
+                    const int pos0 = pos - lane;                        // of the warp's first row
+                    if (p.R < 0 || k0 + kTile - 1 - pos0 <= -p.R || k0 - pos0 - 31 >= p.R) {       // no bias, or all at the table's end
+                        const float far = p.R < 0 ? 0.f : my_table[kPad + p.R + (k0 - pos0 > 0 ? p.R : -p.R)];
+                        if (p.R >= 0 || p.cap.out == 0.f) {
 #pragma unroll
-                            for (int i = 0; i < kTile; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + far);
-                        } else {
-                            const float* row_table = zero + (k0 - pos);
+                            for (int i = 0; i < kTile; i += 2) {
+                                const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2, make_float2(far, far));
+                                r[i] = __float_as_uint(y.x);
+                                r[i + 1] = __float_as_uint(y.y);
+                            }
+                        }
+                    } else {
+                        const uint32_t entry = smem_u32(my_table) + 4 * (kPad + p.R + k0 - pos);
 #pragma unroll
-                            for (int i = 0; i < kTile; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + row_table[i]);
+                        for (int i = 0; i < kTile; i += 2) {
+                            float2 add;
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(add.x) : "r"(entry + 4 * i));
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(add.y) : "r"(entry + 4 * i + 4));
+                            const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2, add);
+                            r[i] = __float_as_uint(y.x);
+                            r[i + 1] = __float_as_uint(y.y);
                         }
                     }
                 }
