@@ -192,6 +192,23 @@ template <int V, bool WHOLE> __device__ __forceinline__ void rotate(float* a, fl
 }
 
 enum { kRotate = 0, kNorm = 1, kNormBwd = 2 };
+constexpr int kAhead = 2;           // rows that the asynchronous copies run ahead
+constexpr int ring_bytes(int vector_bytes, int nv, int mode) {
+    return vector_bytes >= 4 ? kWarps * (kAhead + 1) * (mode == kNormBwd ? 4 : 2) * nv * 32 * vector_bytes : 0;
+}
+
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool in) {         // zeros where not in
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(in ? BYTES : 0) : "memory");
+}
+template <typename R> __device__ __forceinline__ R load_shared(uint32_t from) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (sizeof(R) == 16)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+    else if (sizeof(R) == 8) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(from) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v.x) : "r"(from) : "memory");
+    return *reinterpret_cast<const R*>(&v);
+}
 
 // Queries or keys.  Read from the constant bank where it is used (the index is the same for a whole CTA).
 struct Side {
@@ -214,12 +231,12 @@ struct Params {
 // A group of 2^log_l lanes holds one head of one token; a warp's groups take consecutive heads.  A unit is a token with all heads of q and k
 // (`whole`), or with `hpu` heads of one of them; consecutive warps take consecutive tokens, whose rows are neighbours in the head-major
 // output.  The norm's backward keeps q and k apart, since a CTA sums one weight's gradient: CTAs below ctas_q work on q, the others on k.
-// The next row's loads are under way behind a row's arithmetic, and registers are held down for more warps: rotating 24 + 24 heads of 32400
-// tokens there and back took 367 us without the loads ahead, 331 with them and three CTAs an SM, 288 with four (5.5 TB/s; the norm's
-// forward 211 with two and 175 with three).
 template <typename T, int V, int NV, bool INTER, int MODE, int LOGL>
-__global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm ? 3 : 2) rotary_kernel(const __grid_constant__ Params a, const int any_log_l) {
-    constexpr bool WHOLE = Geometry<V, NV, INTER>::kWhole;
+__global__ void __launch_bounds__(kThreads, MODE == kRotate ? 3 : MODE == kNorm ? 3 : 2) rotary_kernel(const __grid_constant__ Params a, const int any_log_l) {
+    constexpr bool WHOLE = Geometry<V, NV, INTER>::kWhole, ASYNC = V * sizeof(T) >= 4;
+    constexpr int VB = V * sizeof(T), kVectors = (MODE == kNormBwd ? 4 : 2) * NV;         // of a lane and row
+    extern __shared__ __align__(16) uint8_t ring_raw[];
+    const uint32_t ring = sm100::smem_u32(ring_raw);
     __shared__ alignas(16) float angle[kWarps][2][kMaxD / 2];         // cos, sin
     __shared__ float fold[MODE == kNormBwd ? kWarps : 1][MODE == kNormBwd ? kMaxD : 1];
     const int log_l = LOGL >= 0 ? LOGL : any_log_l;
@@ -254,47 +271,144 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
         return v;
     };
 
-    for (long unit = (long)cta * kWarps + warp; unit < units; unit += (long)n_ctas * kWarps) {
-        int part = 0;
+    // A unit's token and heads: of q and k, or (last == which + 1) of one of them.
+    struct Unit {
+        long b;
+        int t, part, which, last;
+    };
+    auto unit_at = [&](long unit) {
+        Unit w;
         long token = unit;
+        w.part = 0;
         if (parts > 1) {
-            part = (int)(unit / a.batch_tokens);
-            token = unit - (long)part * a.batch_tokens;
+            w.part = (int)(unit / a.batch_tokens);
+            token = unit - (long)w.part * a.batch_tokens;
         }
-        long b = 0;
-        int t = (int)token;
+        w.b = 0;
+        w.t = (int)token;
         if (a.batch_tokens > a.tokens) {
-            b = a.batch_tokens <= INT_MAX ? (int)token / a.tokens : token / a.tokens;
-            t = (int)(token - b * a.tokens);
+            w.b = a.batch_tokens <= INT_MAX ? (int)token / a.tokens : token / a.tokens;
+            w.t = (int)(token - w.b * a.tokens);
         }
-        int which = only >= 0 ? only : !a.whole && part >= a.side[0].parts ? 1 : 0;
-        if (only < 0 && which) part -= a.side[0].parts;
-        const int last = only < 0 && a.whole ? 2 : which + 1;
-        bool angles_done = false;
-        for (; which < last; ++which) {
-            const Side& side = a.side[which];
-            const int h_end = min(side.heads, (part + 1) * side.hpu);
-            int h0 = part * side.hpu + sub;
-            if (h0 - sub >= h_end) continue;        // no heads
-            const T* xr = (const T*)side.x + b * side.xs[0] + t * side.xs[2] + h0 * side.xs[1];
-            const T* gr = (const T*)side.g + b * side.gs[0] + t * side.gs[2] + h0 * side.gs[1];
-            T* yr = (T*)side.y + b * side.ys[0] + t * side.ys[2] + h0 * side.ys[1];
-            Pack<T, V> nx0[NV], nx1[NV], ng0[NV], ng1[NV], pw0[NV], pw1[NV];
-            auto load = [&] {           // rows behind the last head are 0: they count for nothing in the weights' gradient
-                const bool ok = h0 < h_end;
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    nx0[i] = nx1[i] = Pack<T, V>();
-                    if (ok && in0[i]) nx0[i].load(xr + geo.off0[i]);
-                    if (ok && in1[i]) nx1[i].load(xr + geo.off1[i]);
-                    if (MODE == kNormBwd) {
-                        ng0[i] = ng1[i] = Pack<T, V>();
-                        if (ok && in0[i]) ng0[i].load(gr + geo.off0[i]);
-                        if (ok && in1[i]) ng1[i].load(gr + geo.off1[i]);
-                    }
+        w.which = only >= 0 ? only : !a.whole && w.part >= a.side[0].parts ? 1 : 0;
+        if (only < 0 && w.which) w.part -= a.side[0].parts;
+        w.last = only < 0 && a.whole ? 2 : w.which + 1;
+        return w;
+    };
+    const long unit_step = (long)n_ctas * kWarps, first_unit = (long)cta * kWarps + warp;
+
+    // Loads run kAhead rows ahead of the arithmetic, over the borders of heads, q and k, and tokens: vectors are copied asynchronously into
+    // slots of shared memory that a lane has to itself, which costs no registers.  (24 + 24 heads of 32400 tokens with one row ahead in registers:
+    // rotation there and back 289 us, the norm's forward 176 and backward 281; so 252, 139 and 198.)  Single elements of 16 bits, which
+    // the copies do not take, go through registers, one row ahead.
+    struct Rows {
+        long unit;
+        int which, last, part, t, h0, h_end;
+        long b;
+        const T *x, *g;
+        bool any;
+    } ahead;
+    auto enter = [&] {              // the first rows of side ahead.which, or of the next one that has any
+        while (true) {
+            if (ahead.which < ahead.last) {
+                const Side& side = a.side[ahead.which];
+                ahead.h0 = ahead.part * side.hpu + sub;
+                ahead.h_end = min(side.heads, (ahead.part + 1) * side.hpu);
+                if (ahead.h0 - sub < ahead.h_end) {
+                    ahead.x = (const T*)side.x + ahead.b * side.xs[0] + ahead.t * side.xs[2] + ahead.h0 * side.xs[1];
+                    if (MODE == kNormBwd) ahead.g = (const T*)side.g + ahead.b * side.gs[0] + ahead.t * side.gs[2] + ahead.h0 * side.gs[1];
+                    return;
                 }
-            };
-            load();         // under way while the angles are formed
+                ++ahead.which;
+                continue;
+            }
+            ahead.unit += unit_step;
+            ahead.any = ahead.unit < units;
+            if (!ahead.any) return;
+            const Unit w = unit_at(ahead.unit);
+            ahead.which = w.which;
+            ahead.last = w.last;
+            ahead.part = w.part;
+            ahead.b = w.b;
+            ahead.t = w.t;
+        }
+    };
+    auto advance = [&] {
+        ahead.h0 += rows;
+        if (ahead.h0 - sub < ahead.h_end) {
+            ahead.x += rows * a.side[ahead.which].xs[1];
+            if (MODE == kNormBwd) ahead.g += rows * a.side[ahead.which].gs[1];
+        } else {
+            ++ahead.which;
+            enter();
+        }
+    };
+    Pack<T, V> nx0[NV], nx1[NV], ng0[NV], ng1[NV];
+    const uint32_t slots = ring + ((uint32_t)warp * (kAhead + 1) * kVectors * 32 + lane) * VB;
+    int fetched = 0, taken = 0;     // of kAhead + 1 slots
+    auto fetch = [&] {              // rows behind the last head are 0: they count for nothing in the weights' gradient
+        const bool ok = ahead.any && ahead.h0 < ahead.h_end;
+        if (ASYNC) {
+            uint32_t to = slots + fetched * (kVectors * 32 * VB);
+#pragma unroll
+            for (int i = 0; i < NV; ++i, to += kVectors / NV * 32 * VB) {
+                const bool c0 = ok && in0[i], c1 = ok && in1[i];
+                copy_async<VB < 4 ? 4 : VB>(to, c0 ? (const void*)(ahead.x + geo.off0[i]) : a.half_turns, c0);
+                copy_async<VB < 4 ? 4 : VB>(to + 32 * VB, c1 ? (const void*)(ahead.x + geo.off1[i]) : a.half_turns, c1);
+                if (MODE == kNormBwd) {
+                    copy_async<VB < 4 ? 4 : VB>(to + 64 * VB, c0 ? (const void*)(ahead.g + geo.off0[i]) : a.half_turns, c0);
+                    copy_async<VB < 4 ? 4 : VB>(to + 96 * VB, c1 ? (const void*)(ahead.g + geo.off1[i]) : a.half_turns, c1);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fetched = fetched == kAhead ? 0 : fetched + 1;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                nx0[i] = nx1[i] = Pack<T, V>();
+                if (ok && in0[i]) nx0[i].load(ahead.x + geo.off0[i]);
+                if (ok && in1[i]) nx1[i].load(ahead.x + geo.off1[i]);
+                if (MODE == kNormBwd) {
+                    ng0[i] = ng1[i] = Pack<T, V>();
+                    if (ok && in0[i]) ng0[i].load(ahead.g + geo.off0[i]);
+                    if (ok && in1[i]) ng1[i].load(ahead.g + geo.off1[i]);
+                }
+            }
+        }
+        if (ahead.any) advance();
+    };
+    if (first_unit < units) {
+        const Unit w = unit_at(first_unit);
+        ahead = {first_unit, w.which, w.last, w.part, w.t, 0, 0, w.b, nullptr, nullptr, true};
+        enter();
+#pragma unroll
+        for (int i = 0; i < (ASYNC ? kAhead : 1); ++i) fetch();
+    }
+
+    for (long unit = first_unit; unit < units; unit += unit_step) {
+        Unit w = unit_at(unit);
+        {       // every pair's angle once per token and warp, spread over the lanes
+            const long at = w.b * a.pos_stride[0] + w.t * a.pos_stride[2];
+            __syncwarp();
+            for (int p = lane; p < P; p += 32) {
+                const long q = at + (a.axis != nullptr ? a.axis[p] * a.pos_stride[1] : 0L);
+                const double pos = a.pos_is_64 ? (double)((const long long*)a.positions)[q] : (double)((const int*)a.positions)[q];
+                const double h = pos * a.half_turns[p];                // angle / pi
+                float c, s;
+                sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
+                const int place = Geometry<V, NV, INTER>::place(p, P);
+                angle[warp][0][place] = c * a.amplitude;
+                angle[warp][1][place] = s * a.sin_amplitude;
+            }
+            __syncwarp();
+        }
+        for (; w.which < w.last; ++w.which) {
+            const Side& side = a.side[w.which];
+            const int h_end = min(side.heads, (w.part + 1) * side.hpu);
+            int h0 = w.part * side.hpu + sub;
+            if (h0 - sub >= h_end) continue;        // no heads
+            T* yr = (T*)side.y + w.b * side.ys[0] + w.t * side.ys[2] + h0 * side.ys[1];
+            Pack<T, V> pw0[NV], pw1[NV];
             if (MODE != kRotate) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
@@ -302,43 +416,34 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
                     if (in1[i]) pw1[i].load((const T*)side.w + geo.off1[i]);
                 }
             }
-            if (!angles_done) {     // every pair's angle once per warp, spread over the lanes
-                const long at = b * a.pos_stride[0] + t * a.pos_stride[2];
-                __syncwarp();
-                for (int p = lane; p < P; p += 32) {
-                    const long q = at + (a.axis != nullptr ? a.axis[p] * a.pos_stride[1] : 0L);
-                    const double pos = a.pos_is_64 ? (double)((const long long*)a.positions)[q] : (double)((const int*)a.positions)[q];
-                    const double h = pos * a.half_turns[p];                // angle / pi
-                    float c, s;
-                    sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
-                    const int place = Geometry<V, NV, INTER>::place(p, P);
-                    angle[warp][0][place] = c * a.amplitude;
-                    angle[warp][1][place] = s * a.sin_amplitude;
-                }
-                __syncwarp();
-                angles_done = true;
-            }
-            while (true) {
+            for (; h0 - sub < h_end; h0 += rows, yr += rows * side.ys[1]) {
                 Pack<T, V> px0[NV], px1[NV], pg0[NV], pg1[NV];
+                if (ASYNC) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+                    uint32_t from = slots + taken * (kVectors * 32 * VB);
+                    using R = typename Pack<T, V>::R;
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    px0[i] = nx0[i];
-                    px1[i] = nx1[i];
-                    if (MODE == kNormBwd) {
-                        pg0[i] = ng0[i];
-                        pg1[i] = ng1[i];
+                    for (int i = 0; i < NV; ++i, from += kVectors / NV * 32 * VB) {
+                        px0[i].raw = load_shared<R>(from);
+                        px1[i].raw = load_shared<R>(from + 32 * VB);
+                        if (MODE == kNormBwd) {
+                            pg0[i].raw = load_shared<R>(from + 64 * VB);
+                            pg1[i].raw = load_shared<R>(from + 96 * VB);
+                        }
+                    }
+                    taken = taken == kAhead ? 0 : taken + 1;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        px0[i] = nx0[i];
+                        px1[i] = nx1[i];
+                        if (MODE == kNormBwd) {
+                            pg0[i] = ng0[i];
+                            pg1[i] = ng1[i];
+                        }
                     }
                 }
-                const bool mine = h0 < h_end;
-                T* out = yr;
-                h0 += rows;
-                const bool more = h0 - sub < h_end;
-                if (more) {         // the next row's loads are under way behind this one's arithmetic
-                    xr += rows * side.xs[1];
-                    gr += rows * side.gs[1];
-                    yr += rows * side.ys[1];
-                    load();
-                }
+                fetch();
                 float f0[NV][V], f1[NV][V];
 #pragma unroll
                 for (int i = 0; i < NV; ++i) unpack<T, V, WHOLE>(px0[i], px1[i], f0[i], f1[i]);
@@ -407,13 +512,13 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 4 : MODE == kNorm 
                     }
                     Pack<T, V> o0, o1;
                     pack<T, V, WHOLE>(f0[i], f1[i], o0, o1);
-                    if (mine && in0[i]) o0.store(out + geo.off0[i]);
-                    if (mine && in1[i]) o1.store(out + geo.off1[i]);
+                    if (h0 < h_end && in0[i]) o0.store(yr + geo.off0[i]);
+                    if (h0 < h_end && in1[i]) o1.store(yr + geo.off1[i]);
                 }
-                if (!more) break;
             }
         }
     }
+    if (ASYNC) asm volatile("cp.async.wait_all;" ::: "memory");
     if (MODE == kNormBwd) {     // this CTA's share of the weight gradient, in a fixed order
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -560,23 +665,35 @@ Params params(const tt_rotary_args& a, const Plan& p, int mode) {
 }
 
 template <typename T, int V, int NV, bool INTER, int LOGL = -1>
-void launch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
+int launch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
     const int grid = p.ctas_q + p.ctas_k;
     const Params k = params(a, p, mode);
-    if (mode == kRotate) rotary_kernel<T, V, NV, INTER, kRotate, LOGL><<<grid, kThreads, 0, st>>>(k, p.log_l);
-    else if (mode == kNorm) rotary_kernel<T, V, NV, INTER, kNorm, LOGL><<<grid, kThreads, 0, st>>>(k, p.log_l);
-    else rotary_kernel<T, V, NV, INTER, kNormBwd, LOGL><<<grid, kThreads, 0, st>>>(k, p.log_l);
+    const int ring = ring_bytes(V * sizeof(T), NV, mode);
+    if (mode == kRotate) rotary_kernel<T, V, NV, INTER, kRotate, LOGL><<<grid, kThreads, ring, st>>>(k, p.log_l);
+    else if (mode == kNorm) rotary_kernel<T, V, NV, INTER, kNorm, LOGL><<<grid, kThreads, ring, st>>>(k, p.log_l);
+    else {
+        static bool configured[64] = {false};         // per device: the attribute belongs to the device's context
+        const int dev = tt_device().dev;
+        if (!configured[dev]) {         // 64 KB with the static part
+            cudaError_t e = cudaFuncSetAttribute(rotary_kernel<T, V, NV, INTER, kNormBwd, LOGL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 ring_bytes(V * sizeof(T), NV, kNormBwd));
+            if (e != cudaSuccess) return tt_record_cuda(e);
+            configured[dev] = true;
+        }
+        rotary_kernel<T, V, NV, INTER, kNormBwd, LOGL><<<grid, kThreads, ring, st>>>(k, p.log_l);
+    }
+    return TT_OK;
 }
 
 // Full-width vectors of 16-bit heads of 64 and 128 (four and eight lanes) have the lanes of a head compiled in.
 template <typename T>
-void dispatch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
+int dispatch(const tt_rotary_args& a, const Plan& p, int mode, cudaStream_t st) {
     constexpr int W = 16 / sizeof(T), A = W == 8 ? 3 : -1, B = W == 8 ? 2 : -1;
-    if (p.width == W && W == 8 && p.log_l == 3) a.interleaved ? launch<T, W, 1, true, A>(a, p, mode, st) : launch<T, W, 1, false, A>(a, p, mode, st);
-    else if (p.width == W && W == 8 && p.log_l == 2) a.interleaved ? launch<T, W, 1, true, B>(a, p, mode, st) : launch<T, W, 1, false, B>(a, p, mode, st);
-    else if (p.width == W) a.interleaved ? launch<T, W, 1, true>(a, p, mode, st) : launch<T, W, 1, false>(a, p, mode, st);
-    else if (p.width == 2) a.interleaved ? launch<T, 2, 2, true>(a, p, mode, st) : launch<T, 2, 2, false>(a, p, mode, st);
-    else a.interleaved ? launch<T, 1, 4, true>(a, p, mode, st) : launch<T, 1, 4, false>(a, p, mode, st);
+    if (p.width == W && W == 8 && p.log_l == 3) return a.interleaved ? launch<T, W, 1, true, A>(a, p, mode, st) : launch<T, W, 1, false, A>(a, p, mode, st);
+    if (p.width == W && W == 8 && p.log_l == 2) return a.interleaved ? launch<T, W, 1, true, B>(a, p, mode, st) : launch<T, W, 1, false, B>(a, p, mode, st);
+    if (p.width == W) return a.interleaved ? launch<T, W, 1, true>(a, p, mode, st) : launch<T, W, 1, false>(a, p, mode, st);
+    if (p.width == 2) return a.interleaved ? launch<T, 2, 2, true>(a, p, mode, st) : launch<T, 2, 2, false>(a, p, mode, st);
+    return a.interleaved ? launch<T, 1, 4, true>(a, p, mode, st) : launch<T, 1, 4, false>(a, p, mode, st);
 }
 
 int check(const tt_rotary_args* a) {
@@ -601,9 +718,9 @@ int run(const tt_rotary_args* a, int mode, void* stream) {
     const Plan p = plan(*a, tt_device().sms, mode);
     if (mode == kNormBwd && a->partial_floats < (long)(p.ctas_q + p.ctas_k) * a->head_dim) return TT_ERR_ARG;
     cudaStream_t st = (cudaStream_t)stream;
-    if (a->dtype == TT_BF16) dispatch<__nv_bfloat16>(*a, p, mode, st);
-    else if (a->dtype == TT_FP16) dispatch<__half>(*a, p, mode, st);
-    else dispatch<float>(*a, p, mode, st);
+    const int rc2 = a->dtype == TT_BF16 ? dispatch<__nv_bfloat16>(*a, p, mode, st)
+                    : a->dtype == TT_FP16 ? dispatch<__half>(*a, p, mode, st) : dispatch<float>(*a, p, mode, st);
+    if (rc2 != TT_OK) return rc2;
     TT_CHECK_LAUNCH();
     if (mode == kNormBwd) {
         const dim3 grid((a->head_dim + kFinCols - 1) / kFinCols, (a->q_heads > 0) + (a->k_heads > 0));
