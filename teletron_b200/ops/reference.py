@@ -156,25 +156,26 @@ def masked_attention(q, k, v, ranges, scale: Optional[float] = None, softcap: Op
     B, h, S, D = q.shape
     n, group = k.shape[2], h // k.shape[1]
     calc = torch.promote_types(q.dtype, torch.float32)
-    kf, vf = (t.to(calc).repeat_interleave(group, dim=1) for t in (k, v))
-    s = (q.to(calc) @ kf.transpose(-1, -2)) * (D ** -0.5 if scale is None else scale)
+    j = torch.arange(n, device=q.device)
+    see = (j >= ranges.first[..., None]) & (j < ranges.behind[..., None])              # [B, S, n]
+    # what no run reaches may hold anything, in the gradients too: 0 times a NaN is a NaN
+    live, used = see.any(dim=2)[:, None, :, None], see.any(dim=1)[:, None, :, None]
+    qf = q.to(calc).masked_fill(~live, 0.0)
+    kf, vf = (t.to(calc).masked_fill(~used, 0.0).repeat_interleave(group, dim=1) for t in (k, v))
+    s = (qf @ kf.transpose(-1, -2)) * (D ** -0.5 if scale is None else scale)
     if softcap is not None:
         s = softcap * torch.tanh(s / softcap)
-    j = torch.arange(n, device=q.device)
     if distance_bias is not None:
         R = (distance_bias.shape[1] - 1) // 2
         i = torch.arange(S, device=q.device)[None] + (0 if ranges.query_start is None else ranges.query_start.long()[:, None])
         far = (j - i[..., None]).clamp(-R, R) + R                                      # [1 or B, S, n]
         s = s + distance_bias.to(calc)[:, far].transpose(0, 1)
-    see = (j >= ranges.first[..., None]) & (j < ranges.behind[..., None])              # [B, S, n]
     s = s.masked_fill(~see[:, None], float("-inf"))
     top = s.amax(dim=-1, keepdim=True).detach() if n else s.new_zeros(B, h, S, 1)
     p = torch.exp(s - top.masked_fill(top == float("-inf"), 0.0))
     total = p.sum(dim=-1, keepdim=True)
     p = p / total.masked_fill(total == 0, 1.0)
-    # values that no query sees may hold anything: 0 times a NaN is a NaN
-    used = see.any(dim=1)[:, None, :, None]
-    o = p @ vf.masked_fill(~used, 0.0)
+    o = (p @ vf).masked_fill(~live, 0.0)
     return o.to(q.dtype).transpose(1, 2).reshape(B, S, h * D)
 
 

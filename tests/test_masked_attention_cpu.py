@@ -78,6 +78,11 @@ def test_rows_and_keys_without_a_run_are_left_out():
         t[:, :, [0, 6, 7]] = float("nan")
     got = ops.masked_attention(q, k, v, r)
     assert torch.equal(got, want) and not bool(got[:, [0, 6, 7]].any())
+    # nor do they reach a gradient, or the other way
+    dout = torch.randn(1, 8, 8, dtype=torch.float64)
+    dout[:, [0, 6, 7]] = float("inf")
+    for g in torch.autograd.grad(ops.masked_attention(*[t.requires_grad_() for t in (q, k, v)], r, softcap=3.0), (q, k, v), dout):
+        assert bool(torch.isfinite(g).all()) and not bool(g[:, :, [0, 6, 7]].any())
 
 
 def test_gradients_against_differences():
