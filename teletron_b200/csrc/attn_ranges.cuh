@@ -185,6 +185,8 @@ inline Cap make_cap(float scale, float softcap) {
     k.out = softcap * kLog2e;
     k.inv_out = 1.f / k.out;
     k.small = scale != 0.f ? (float)fmin(0.3 / fabs(u), 3e38) : 3e38f;
+    for (float c : k.c)
+        if (!isfinite(c)) k.small = -1.f;           // a cap so far below the scale that the series has no coefficients in 32 bits
     return k;
 }
 __device__ __forceinline__ float2 cap_small(const Cap& k, float2 z) {

@@ -137,6 +137,20 @@ def test_large_scores_and_infinite_biases():
     assert not bool(ops.masked_attention(q.detach(), k.detach(), v.detach(), ops.key_ranges(200, device="cuda"), distance_bias=bias).any())
 
 
+@pytest.mark.parametrize("softcap", [1e-2, 1e-6, 1e-9])
+def test_caps_far_below_the_scores(softcap):
+    """All weights of a row nearly or wholly the same: behind the cap no score is more than it from another."""
+    torch.manual_seed(7)
+    q, k, v = heads(1, 140, (2, 1, 1), 64, BF16, False)
+    q[:, :, 3] = 0
+    out = ops.masked_attention(q, k, v, ops.key_ranges(140, causal=True, device="cuda"), softcap=softcap)
+    mean = v.double().cumsum(2) / torch.arange(1, 141, device="cuda")[:, None]
+    got = out.view(1, 140, 2, 64).transpose(1, 2).double()
+    size = v.double().abs().cumsum(2) / torch.arange(1, 141, device="cuda")[:, None]
+    # weights off by e^(2 cap), P and the output rounded to 2^-8 each
+    assert bool(((got - mean).abs() <= (2.5 * softcap + 2 * 2.0 ** -8) * size + 2.0 ** -8 * mean.abs()).all())
+
+
 def test_strides_that_copies_cannot_address():
     torch.manual_seed(2)
     base = torch.randn(1, 2, 130, 65, device="cuda").to(BF16)
