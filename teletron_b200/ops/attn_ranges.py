@@ -251,6 +251,7 @@ def _backward(ctx, dout):
         delta = lse.new_empty(lse.shape)
         dbias = partials = None
         if ctx.wide:
+            _lib.LAUNCHES += 1          # the sum of the bias's gradients
             dbias = bias.new_empty(bias.shape)
             partials = lse.new_empty((B * hq * (lse.shape[2] // TILE) * bias.shape[1],))
         call("tt_attn_ranges_bwd", _pack(q, k, v, ctx.ranges, out, out if ctx.wide else None, lse, ctx.scale, ctx.softcap, bias)
