@@ -457,7 +457,8 @@ __global__ void __launch_bounds__(kThreads, MODE == kRotate ? 3 : MODE == kNorm 
                         add_product<V>(sq, f1[i], f1[i]);
                     }
                     const float ss = total<V>(sq);
-                    const float r = rsqrtf(group_sum(ss) * a.inv_D + a.eps);
+                    float r = rsqrtf(group_sum(ss) * a.inv_D + a.eps);
+                    if (MODE == kNormBwd && h0 >= h_end) r = 0.f;         // a row behind the last head; without eps it would be NaN
                     float g0[NV][V], g1[NV][V], dots[V];
 #pragma unroll
                     for (int e = 0; e < V; ++e) dots[e] = 0.f;

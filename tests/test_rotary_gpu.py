@@ -163,6 +163,19 @@ def test_empty_operands(tokens, heads_q, heads_k):
         assert bool(torch.isfinite(dq).all()) and bool(torch.isfinite(dk).all())
 
 
+def test_norm_without_eps_at_heads_that_do_not_fill_a_warp():
+    torch.manual_seed(5)
+    q, k = (torch.randn(2, h, 9, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for h in (3, 1))
+    wq, wk = (torch.ones(64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(2))
+    freqs, pos = ops.rotary_frequencies(64, device="cuda"), torch.arange(9, device="cuda")
+    grads = []
+    for eps in (0.0, 1e-12):        # which is nothing to squares of about 1
+        out = ops.qk_norm_rotary(q, k, wq, wk, pos, freqs, eps=eps)
+        grads.append(torch.autograd.grad(out, (q, k, wq, wk), [torch.ones_like(t) for t in out]))
+    for a, b in zip(*grads):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
 def test_only_what_needs_a_gradient_gets_one():
     freqs = ops.rotary_frequencies(64, device="cuda")
     pos = torch.arange(5, device="cuda")
