@@ -23,6 +23,8 @@ from .gemm_tcgen05 import status_tensor
 
 TILE = 128
 MAX_DISTANCE = 1024
+MAX_BATCH = MAX_HEADS = 65535
+MAX_LEN = 1 << 30           # of queries and of keys
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
@@ -55,7 +57,12 @@ def _lengths(value, name: str, batch: int, device, per_document: Optional[int] =
     shapes = [(batch,)] + ([(batch, per_document)] if per_document is not None else [])
     if tuple(t.shape) not in shapes:
         raise ValueError(f"{name}: expected an int or one of the shapes {shapes}, got {tuple(t.shape)}")
-    return None, t.to(device=device, dtype=torch.int32).contiguous()
+    return None, _int32(t.to(device))
+
+
+def _int32(t):
+    """Lengths, offsets and positions in 32 bits; what lies beyond them is beyond every length too."""
+    return (t if t.dtype is torch.int32 else t.clamp(-MAX_LEN, MAX_LEN).to(torch.int32)).contiguous()
 
 
 def _runs(q_len, kv_len, batch, causal, documents, prefix_len, prefix, kv_valid_len, query_start, device):
@@ -100,6 +107,8 @@ def key_ranges(q_len: int, kv_len: Optional[int] = None, *, batch: int = 1, caus
     q_len, kv_len, batch = int(q_len), int(q_len if kv_len is None else kv_len), int(batch)
     if q_len < 0 or kv_len < 0 or batch < 0:
         raise ValueError(f"key_ranges: negative sizes ({q_len} queries, {kv_len} keys, {batch} samples)")
+    if max(q_len, kv_len) > MAX_LEN:
+        raise ValueError(f"key_ranges: {q_len} queries and {kv_len} keys, at most {MAX_LEN} of each")
     for v in (documents, prefix_len, kv_valid_len, query_start):
         if device is None and isinstance(v, torch.Tensor):
             device = v.device
@@ -118,19 +127,21 @@ def key_ranges(q_len: int, kv_len: Optional[int] = None, *, batch: int = 1, caus
         if documents.dtype not in (torch.int32, torch.int64) or documents.dim() not in (1, 2) or documents.shape[-1] < 2 \
                 or (documents.dim() == 2 and documents.shape[0] != batch):
             raise ValueError(f"documents: expected integer offsets [n + 1] or [{batch}, n + 1], got {documents.dtype} {tuple(documents.shape)}")
-        documents = documents.to(device=device, dtype=torch.int32).contiguous()
+        documents = _int32(documents.to(device))
         documents = documents[None] if documents.dim() == 1 else documents
         n = documents.shape[1] - 1
     prefix_len, prefix = _lengths(prefix_len, "prefix_len", batch, device, n)
     kv_valid_int, kv_valid = _lengths(kv_valid_len, "kv_valid_len", batch, device)
     start_int, start = _lengths(query_start, "query_start", batch, device)
-    if prefix_len is not None and prefix_len < 0:
-        raise ValueError(f"prefix_len: {prefix_len} is negative")
+    if prefix_len is not None:
+        if prefix_len < 0:
+            raise ValueError(f"prefix_len: {prefix_len} is negative")
+        prefix_len = min(prefix_len, kv_len)
     if kv_valid_int is not None:
         kv_valid = torch.full((batch,), min(max(kv_valid_int, 0), kv_len), dtype=torch.int32, device=device)
     if start_int:
-        start = torch.full((batch,), start_int, dtype=torch.int32, device=device)
-    if device.type != "cuda" or not _lib.available() or min(q_len, kv_len, batch) == 0:
+        start = torch.full((batch,), max(-MAX_LEN, min(MAX_LEN, start_int)), dtype=torch.int32, device=device)
+    if device.type != "cuda" or not _lib.available() or min(q_len, kv_len, batch) == 0 or batch > MAX_BATCH:
         first, behind = _runs(q_len, kv_len, batch, causal, documents, prefix_len, prefix, kv_valid, start, device)
         return KeyRanges(batch, q_len, kv_len, first, behind, start, None, bool(causal))
     at = _layout(batch, q_len, kv_len)
@@ -185,7 +196,7 @@ def check_arguments(q, k, v, ranges, scale, softcap, distance_bias) -> None:
 
 def supported(q, k, v, ranges, distance_bias) -> bool:
     return (_lib.available() and q.is_cuda and q.dtype in _DTYPES and q.shape[3] in (64, 128) and ranges.plan is not None
-            and q.numel() > 0 and k.numel() > 0 and q.shape[0] <= 65535 and q.shape[1] <= 65535
+            and q.numel() > 0 and k.numel() > 0 and q.shape[1] <= MAX_HEADS
             and (distance_bias is None or distance_bias.shape[1] <= 2 * MAX_DISTANCE + 1))
 
 

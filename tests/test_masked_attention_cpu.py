@@ -42,6 +42,19 @@ def test_key_ranges_refuses(kw):
         ops.key_ranges(**kw)
 
 
+def test_lengths_beyond_32_bits():
+    huge, n = 2 ** 32 + 1, 6
+    want = ops.key_ranges(n, batch=2, causal=True, prefix_len=n, kv_valid_len=n)
+    for kw in (dict(prefix_len=huge), dict(prefix_len=[huge, huge]), dict(query_start=huge), dict(query_start=torch.tensor([huge, huge])),
+               dict(prefix_len=n, kv_valid_len=huge), dict(prefix_len=n, kv_valid_len=[huge, huge]), dict(prefix_len=n, documents=[0, huge])):
+        got = ops.key_ranges(n, batch=2, causal=True, **kw)
+        assert torch.equal(got.first, want.first) and torch.equal(got.behind, want.behind), kw
+    none = ops.key_ranges(n, batch=2, causal=True, query_start=-huge)
+    assert not bool(none.behind.any())
+    with pytest.raises(ValueError):
+        ops.key_ranges(huge)
+
+
 def _operands(**change):
     a = dict(q=torch.randn(2, 4, 6, 8), k=torch.randn(2, 2, 6, 8), v=torch.randn(2, 2, 6, 8), ranges=ops.key_ranges(6, batch=2))
     a.update(change)

@@ -122,6 +122,23 @@ def test_runs_on_the_device_are_the_definitions():
         assert got.plan is not None
 
 
+def test_lengths_beyond_32_bits_and_batches_beyond_a_grid():
+    huge = 2 ** 32 + 1
+    for kw in (dict(prefix_len=huge), dict(query_start=huge), dict(query_start=-huge), dict(kv_valid_len=torch.tensor([huge, 3])),
+               dict(documents=[2, huge]), dict(prefix_len=[huge, 1])):
+        for a, b in zip(*[(r.first.cpu(), r.behind.cpu()) for r in (ops.key_ranges(150, batch=2, causal=True, device=d, **kw) for d in ("cuda", "cpu"))]):
+            assert torch.equal(a, b), kw
+    from teletron_b200.ops import fallback
+    q = torch.randn(65537, 1, 2, 64, device="cuda").to(BF16)
+    was = fallback.strict()
+    try:
+        fallback.set_strict(False)
+        got = ops.masked_attention(q, q, q, ops.key_ranges(2, batch=65537, causal=True, device="cuda"))
+    finally:
+        fallback.set_strict(was)
+    assert torch.equal(got[:, 0], q[:, 0, 0])
+
+
 def test_large_scores_and_infinite_biases():
     torch.manual_seed(1)
     q, k, v = heads(1, 200, (2, 2, 2), 64, BF16, False)
