@@ -24,6 +24,7 @@ from .gemm_tcgen05 import status_tensor
 TILE = 128
 MAX_DISTANCE = 1024
 MAX_BATCH = MAX_HEADS = 65535
+_LARGEST = 1e30
 MAX_LEN = 1 << 30           # of queries and of keys
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -183,10 +184,11 @@ def check_arguments(q, k, v, ranges, scale, softcap, distance_bias) -> None:
         raise ValueError(f"runs of {ranges.batch} x {ranges.q_len} queries and {ranges.kv_len} keys for {B} x {n} queries and {m} keys")
     if ranges.first.get_device() != device:
         raise ValueError(f"runs on {ranges.device}, queries on {q.device}")
-    if scale is not None and not math.isfinite(scale):
-        raise ValueError(f"scale: {scale} is not finite")
-    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
-        raise ValueError(f"softcap: expected a positive number or None, got {softcap}")
+    if scale is not None and not abs(scale) <= _LARGEST:
+        raise ValueError(f"scale: {scale} is not finite, or beyond {_LARGEST}")
+    # the kernels hold the cap, its inverse and scale / cap in 32 bits
+    if softcap is not None and not (1 / _LARGEST <= softcap <= _LARGEST and (1.0 if scale is None else abs(scale)) <= _LARGEST * softcap):
+        raise ValueError(f"softcap: expected a positive number or None, neither it nor the scale ({scale}) over it beyond {_LARGEST}, got {softcap}")
     if distance_bias is not None:
         if distance_bias.dim() != 2 or distance_bias.shape[0] != hq or distance_bias.shape[1] % 2 == 0:
             raise ValueError(f"distance_bias: expected [{hq}, 2 R + 1], got {tuple(distance_bias.shape)}")

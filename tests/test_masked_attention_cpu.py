@@ -63,7 +63,8 @@ def _operands(**change):
 
 @pytest.mark.parametrize("change", [dict(q=torch.randn(2, 4, 8)), dict(k=torch.randn(2, 3, 6, 8), v=torch.randn(2, 3, 6, 8)), dict(k=torch.randn(2, 2, 5, 8)),
                                     dict(v=torch.randn(2, 2, 6, 8).half()), dict(q=torch.randn(1, 4, 6, 8)), dict(ranges=None), dict(ranges=ops.key_ranges(6)),
-                                    dict(ranges=ops.key_ranges(5, 6, batch=2)), dict(scale=float("nan")), dict(softcap=0.0), dict(softcap=-1.0),
+                                    dict(ranges=ops.key_ranges(5, 6, batch=2)), dict(scale=float("nan")), dict(scale=1e300), dict(softcap=1e-300),
+                                    dict(softcap=1e38), dict(softcap=float("nan")), dict(scale=1e20, softcap=1e-20), dict(softcap=0.0), dict(softcap=-1.0),
                                     dict(softcap=float("inf")), dict(distance_bias=torch.zeros(4, 4)), dict(distance_bias=torch.zeros(2, 5)),
                                     dict(distance_bias=torch.zeros(4, 5).double()), dict(distance_bias=torch.zeros(5)),
                                     dict(q=torch.zeros(2, 4, 6, 8, dtype=torch.int32), k=torch.zeros(2, 2, 6, 8, dtype=torch.int32), v=torch.zeros(2, 2, 6, 8, dtype=torch.int32))])
