@@ -157,7 +157,7 @@ def rotary(q, k, positions, freqs):
 def qk_norm_rotary(q, k, q_weight, k_weight, positions, freqs, eps: float = 1e-6):
     """RMS norm of every head of ``q`` and ``k`` (weights ``[head_dim]``, statistics in fp32), then :func:`rotary`, rounded once."""
     stride = rope.check_arguments(q, k, positions, freqs)
-    rope.check_weights(q, k, q_weight, k_weight)
+    rope.check_norm(q, k, q_weight, k_weight, eps)
     if _rotary_kernel_ok(q):
         return rope.qk_norm_rotary(q, k, q_weight, k_weight, positions, stride, freqs, eps)
     return reference.qk_norm_rotary(q, k, q_weight, k_weight, rope.by_axis(positions, freqs.num_axes), freqs, eps)

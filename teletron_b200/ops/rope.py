@@ -40,7 +40,11 @@ class Rotary:
     dim: int = dataclasses.field(init=False)        # elements of a head that are rotated
 
     def __post_init__(self):
-        object.__setattr__(self, "dim", 2 * self.inv_freq.shape[0])
+        w, h, a = self.inv_freq, self.half_turns, self.axis
+        if w.dim() != 1 or h.shape != w.shape or h.dtype is not torch.float64 or h.device != w.device or not h.is_contiguous() \
+                or (a is not None and (a.shape != w.shape or a.dtype is not torch.int32 or a.device != w.device or not a.is_contiguous())):
+            raise ValueError("rotary: expected frequencies as rotary_frequencies makes them")
+        object.__setattr__(self, "dim", 2 * w.shape[0])
 
     def to(self, device) -> "Rotary":
         move = lambda t: None if t is None else t.to(device)
@@ -160,7 +164,11 @@ def by_axis(positions, num_axes: int):
     return positions[None, None] if positions.dim() == 1 else positions[:, None]
 
 
-def check_weights(q, k, q_weight, k_weight) -> None:
+def check_norm(q, k, q_weight, k_weight, eps) -> None:
+    if k is None:
+        raise ValueError("qk_norm_rotary: expected queries and keys")
+    if not 0 <= eps < math.inf:
+        raise ValueError(f"eps: expected a number of 0 or more, got {eps}")
     for x, w, n in ((q, q_weight, "q_weight"), (k, k_weight, "k_weight")):
         if w.dim() != 1 or w.shape[0] != x.shape[3] or w.dtype is not x.dtype or w.get_device() != x.get_device():
             raise ValueError(f"{n}: expected [{x.shape[3]}] {x.dtype} on {x.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")

@@ -123,6 +123,24 @@ def test_norm_weights_are_checked(shape, dtype):
         ops.qk_norm_rotary(a["q"], a["k"], good, torch.ones(shape, dtype=dtype), a["positions"], a["freqs"])
 
 
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+def test_eps_is_checked(eps):
+    a, w = _operands(), torch.ones(8)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rotary(a["q"], a["k"], w, w, a["positions"], a["freqs"], eps=eps)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rotary(a["q"], None, w, w, a["positions"], a["freqs"])
+
+
+@pytest.mark.parametrize("change", [dict(half_turns=torch.ones(3, dtype=torch.float64)), dict(half_turns=torch.ones(4)),
+                                    dict(axis=torch.zeros(4, dtype=torch.int64)), dict(axis=torch.zeros(8, dtype=torch.int32)[::2]),
+                                    dict(half_turns=torch.ones(8, dtype=torch.float64)[::2])])
+def test_frequencies_of_other_shapes_are_refused(change):
+    import dataclasses
+    with pytest.raises(ValueError):
+        dataclasses.replace(ops.rotary_frequencies(8), **change)
+
+
 def test_native_arguments_have_the_layout_that_the_library_expects():
     """The packed arguments are read as the C structure; sizes that disagree are refused before anything is launched."""
     from teletron_b200.ops import _lib, rope
