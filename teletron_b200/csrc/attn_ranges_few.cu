@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const FewParams p) {
     const bool whole = p.ctas == 0;
     long at_step = 0, end_step = 1;
     if (!whole) {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");        // the join: it waits for this grid's end before it reads a result
         shares.count(p.plan, p.batch, p.k_heads, p.ctas);
         if ((int)blockIdx.x >= shares.ctas) return;
         at_step = shares.first_of(blockIdx.x);
@@ -386,6 +387,7 @@ __global__ void __launch_bounds__(kJoinThreads) few_join_kernel(const FewParams 
     shares.count(p.plan, p.batch, p.k_heads, p.ctas);
     const long steps = (shares.before[b + 1] - shares.before[b]) / p.k_heads, first = shares.before[b] + kv_head * steps;
     const int c0 = steps > 0 ? shares.share_of(first) : 0, n = steps > 0 ? shares.share_of(first + steps - 1) - c0 + 1 : 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // the kernel ahead has ended and its results are in memory
     const float* part = p.partials + ((long)(unit + c0) * rows + r) * (D + 2);
     const long next = (long)rows * (D + 2);         // of the next piece
     float top = -INFINITY;
@@ -465,8 +467,18 @@ int launch(const tt_ranges_args& a, const FewParams& p, int dev, cudaStream_t st
     kern<<<p.ctas ? p.ctas : (int)units, kThreads, Few<D, MT>::kSmem, st>>>(p);
     TT_CHECK_LAUNCH();
     if (p.ctas) {
-        few_join_kernel<D, BF16><<<(int)(units * rows), kJoinThreads, 0, st>>>(p);
-        TT_CHECK_LAUNCH();
+        // started while the pieces are still computed, so that neither its launch nor the counting of the shares is waited for
+        cudaLaunchAttribute early = {};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(units * rows));
+        cfg.blockDim = dim3(kJoinThreads);
+        cfg.stream = st;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, few_join_kernel<D, BF16>, p);
+        if (e != cudaSuccess) return tt_record_cuda(e);
     }
     return TT_OK;
 }

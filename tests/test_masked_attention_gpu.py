@@ -337,3 +337,47 @@ def test_few_queries_past_32_bits_of_elements():
     q = torch.randn(2, 4, 300, 64, device="cuda").to(BF16)
     r = ops.key_ranges(300, batch=2, causal=True, device="cuda")
     assert torch.equal(ops.masked_attention(q, k, k, r), ops.masked_attention(q, k.contiguous(), k.contiguous(), r))
+
+
+def test_new_tokens_in_a_captured_graph_and_on_two_streams():
+    torch.manual_seed(11)
+    B, hq, hk, n, D = 3, 8, 2, 5000, 128
+    q = torch.randn(B, hq, 1, D, device="cuda").to(BF16)
+    k, v = (torch.randn(B, hk, n, D, device="cuda").to(BF16) for _ in range(2))
+    lengths = torch.tensor([5000, 40, 1300], device="cuda")
+
+    def step(x):            # a layer after the other: each reads what the one ahead wrote
+        r = ops.key_ranges(1, n, batch=B, causal=True, kv_valid_len=lengths, query_start=lengths - 1)
+        for _ in range(4):
+            x = ops.masked_attention(x, k, v, r, scale=1.0).view(B, 1, hq, D).transpose(1, 2)
+        return x
+
+    want = step(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(q)
+    for _ in range(3):
+        graph.replay()
+    assert torch.equal(held, want)
+    lengths.copy_(torch.tensor([0, 5000, 4999], device="cuda"))
+    q.neg_()
+    for _ in range(3):
+        graph.replay()
+    want = step(q)
+    assert torch.equal(held, want) and not bool(want[0].any())
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step(q))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("batch", [128, 129])
+def test_few_queries_of_many_samples(batch):
+    """Both sides of the largest batch whose steps are dealt out."""
+    lengths = torch.arange(batch, device="cuda") * 5
+    check(batch, 1, 600, 2, 1, 64, BF16, train=False, causal=True, kv_valid_len=lengths, query_start=lengths - 1)
