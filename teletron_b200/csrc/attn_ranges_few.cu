@@ -56,6 +56,9 @@ template <int D> __device__ __forceinline__ uint32_t place(uint32_t base, int ro
     return base + row * (D * 2) + ((piece ^ (row & 7)) << 4);
 }
 
+constexpr int kMaxBatch = 128;          // of shared steps; more samples are many CTAs by themselves
+static_assert(kMaxBatch <= kThreads, "a thread a sample");
+
 template <int D, int MT> struct Few {
     static constexpr int kTileBytes = kStep * D * 2;                        // 16 keys
     static constexpr int kRing = kStages * 2 * kTileBytes;                  // of one warp
@@ -64,7 +67,6 @@ template <int D, int MT> struct Few {
     static_assert(kRing >= MT * 16 * D * 4, "a warp's outputs are joined in its ring");
 };
 
-constexpr int kMaxBatch = 128;          // of shared steps; more samples are many CTAs by themselves
 constexpr int kMinSteps = 2 * kWarps;   // of a share
 
 // The keys that any of a sample's queries sees, from a multiple of a step on
@@ -79,18 +81,32 @@ __device__ __forceinline__ void run_of(const PlanPtr& plan, int b, int* lo, int*
 // numbered u + c.
 struct Shares {
     long before[kMaxBatch + 1];         // steps of the samples ahead
+    long warps[kMaxBatch / 32];         // of 32 samples
     int ctas;
-    __device__ void count(const PlanPtr& plan, int batch, int k_heads, int most) {       // whole CTA
-        for (int b = threadIdx.x; b < batch; b += blockDim.x) {
+    __device__ void count(const PlanPtr& plan, int batch, int k_heads, int most) {       // whole CTA, of kMaxBatch threads or more
+        const int b = threadIdx.x, lane = b & 31, warp = b >> 5;
+        long sum = 0;
+        if (b < batch) {
             int lo, hi;
             run_of(plan, b, &lo, &hi);
-            before[b + 1] = (long)((hi - lo + kStep - 1) / kStep) * k_heads;
+            sum = (long)((hi - lo + kStep - 1) / kStep) * k_heads;
         }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        if (lane == 31 && warp < kMaxBatch / 32) warps[warp] = sum;
         __syncthreads();
-        if (threadIdx.x == 0) {
+        long total = 0;
+#pragma unroll
+        for (int w = 0; w < kMaxBatch / 32; ++w) {
+            if (w < warp) sum += warps[w];
+            total += warps[w];
+        }
+        if (b < batch) before[b + 1] = sum;
+        if (b == 0) {
             before[0] = 0;
-            for (int b = 0; b < batch; ++b) before[b + 1] += before[b];
-            const long total = before[batch];
             const long wanted = (total + kMinSteps - 1) / kMinSteps;
             ctas = (int)(wanted < most ? wanted : most);
             samples = batch;
@@ -375,82 +391,110 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const FewParams p) {
     }
 }
 
-// One CTA a row: eight warps add the pieces' results, each its own in their order, then the warps' sums in theirs.
-constexpr int kMaxShares = 512, kJoinThreads = 256;
-template <int D, bool BF16>
+// W warps a row, 8 / W rows a CTA: every warp adds its share of the row's pieces in their order, then the warps' sums are added in theirs.
+constexpr int kJoinThreads = 256;
+template <int D, bool BF16, int W>
 __global__ void __launch_bounds__(kJoinThreads) few_join_kernel(const FewParams p) {
     __shared__ Shares shares;
-    __shared__ float weight[kMaxShares], red[kJoinThreads / 32], sums[kJoinThreads / 32][D + 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = p.group * p.q_len, r = blockIdx.x % rows, unit = blockIdx.x / rows;
-    const int b = unit / p.k_heads, kv_head = unit - b * p.k_heads, head = kv_head * p.group + r % p.group, i = r / p.group;
+    __shared__ float sums[W > 1 ? W : 1][D + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_piece = W > 1 ? warp : 0;
+    const int rows = p.group * p.q_len;
+    const long row = (long)blockIdx.x * (8 / W) + (W > 1 ? 0 : warp);
     shares.count(p.plan, p.batch, p.k_heads, p.ctas);
+    if (row >= (long)p.batch * p.k_heads * rows) return;        // (W == 1: whole warps, with no barrier to come)
+    const int unit = (int)(row / rows), r = (int)(row - (long)unit * rows);
+    const int b = unit / p.k_heads, kv_head = unit - b * p.k_heads, head = kv_head * p.group + r % p.group, i = r / p.group;
     const long steps = (shares.before[b + 1] - shares.before[b]) / p.k_heads, first = shares.before[b] + kv_head * steps;
     const int c0 = steps > 0 ? shares.share_of(first) : 0, n = steps > 0 ? shares.share_of(first + steps - 1) - c0 + 1 : 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");          // the kernel ahead has ended and its results are in memory
     const float* part = p.partials + ((long)(unit + c0) * rows + r) * (D + 2);
     const long next = (long)rows * (D + 2);         // of the next piece
-    float top = -INFINITY;
-    for (int s = threadIdx.x; s < n; s += kJoinThreads) {
-        weight[s] = part[s * next + D];
-        top = fmaxf(top, weight[s]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-    top = red[0];
-#pragma unroll
-    for (int k = 1; k < kJoinThreads / 32; ++k) top = fmaxf(top, red[k]);
-    for (int s = threadIdx.x; s < n; s += kJoinThreads) weight[s] = weight[s] == -INFINITY ? 0.f : exp2f(weight[s] - top);
-    __syncthreads();
-    float sum = 0.f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");          // the kernel ahead has ended and its results are in memory
+    // the first piece, often a warp's only one, is read with the maxima
+    float m1 = -INFINITY, l1 = 0.f;
     float2 acc[D / 64];
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+    if (first_piece < n) {
+        const float* q = part + first_piece * next;
+        m1 = q[D];
+        l1 = q[D + 1];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) acc[c] = *reinterpret_cast<const float2*>(q + c * 64 + lane * 2);
+    }
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, part[s * next + D]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float a1 = m1 == -INFINITY ? 0.f : exp2f(m1 - top);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(a1 * acc[c].x, a1 * acc[c].y);
+    float sum = lane == 0 ? a1 * l1 : 0.f;
+    for (int s0 = first_piece + W; s0 < n; s0 += 32 * W) {
+        const int mine = s0 + lane * W, count = min(32, (n - s0 + W - 1) / W);
+        float weight = 0.f;
+        if (mine < n) {
+            const float m = part[mine * next + D];
+            weight = m == -INFINITY ? 0.f : exp2f(m - top);
+            sum += weight * part[mine * next + D + 1];
+        }
 #pragma unroll 8
-    for (int s = warp; s < n; s += kJoinThreads / 32) {
-        const float* q = part + s * next;
-        const float a = weight[s];
-        sum += a * q[D + 1];
+        for (int k = 0; k < count; ++k) {
+            const float* q = part + (s0 + k * W) * next;
+            const float a = __shfl_sync(0xffffffffu, weight, k);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const float2 x = *reinterpret_cast<const float2*>(q + c * 64 + lane * 2);
+                acc[c].x += a * x.x;
+                acc[c].y += a * x.y;
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (W > 1) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
-            const float2 x = *reinterpret_cast<const float2*>(q + c * 64 + lane * 2);
-            acc[c].x += a * x.x;
-            acc[c].y += a * x.y;
+            sums[warp][c * 64 + lane * 2] = acc[c].x;
+            sums[warp][c * 64 + lane * 2 + 1] = acc[c].y;
         }
-    }
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-        sums[warp][c * 64 + lane * 2] = acc[c].x;
-        sums[warp][c * 64 + lane * 2 + 1] = acc[c].y;
-    }
-    if (lane == 0) sums[warp][D] = sum;
-    __syncthreads();
-    const int d = threadIdx.x * 2;
-    if (d < D) {
-        float2 o2 = make_float2(0.f, 0.f);
+        if (lane == 0) sums[warp][D] = sum;
+        __syncthreads();
+        if (warp > 0) return;
         sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kJoinThreads / 32; ++k) {
-            o2.x += sums[k][d];
-            o2.y += sums[k][d + 1];
+        for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
             sum += sums[k][D];
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                acc[c].x += sums[k][c * 64 + lane * 2];
+                acc[c].y += sums[k][c * 64 + lane * 2 + 1];
+            }
         }
-        const bool none = sum == 0.f;
-        const float inv = none ? 0.f : 1.f / sum;
-        *reinterpret_cast<uint32_t*>(p.out + (((long)b * p.q_len + i) * p.q_heads + head) * D + d) = none ? 0u : pack2<BF16>(o2.x * inv, o2.y * inv);
-        if (d == 0) p.lse[((long)b * p.q_heads + head) * kTile + i] = none ? INFINITY : top + log2f(sum);
     }
-    if (i == 0) write_padding(p.lse, b, p.q_heads, head, 1, p.q_len);
+    const bool none = sum == 0.f;
+    const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+        *reinterpret_cast<uint32_t*>(p.out + (((long)b * p.q_len + i) * p.q_heads + head) * D + c * 64 + lane * 2) =
+            none ? 0u : pack2<BF16>(acc[c].x * inv, acc[c].y * inv);
+    float* const lse = p.lse + ((long)b * p.q_heads + head) * kTile;
+    if (lane == 0) lse[i] = none ? INFINITY : top + log2f(sum);
+    if (i == 0)         // the rest of the statistics' tile says "no such query" to the backward
+        for (int c = p.q_len + lane; c < kTile; c += 32) lse[c] = INFINITY;
 }
 
-// CTAs of equal shares: two fit an SM.  0 (a CTA for each sample and key head, which needs no join) where those fill the device four times over,
-// where there are few keys (up to 256: two rounds of the warps' steps, against 4 us for the join), and for batches beyond the shares' table.
+// CTAs of equal shares, two of which fit an SM; 0: a CTA for each sample and key head, which needs no join.  Those leave a share of the device idle
+// in their last round, for as long as a sample's keys take; shares cost a second kernel and a few more loads, ~6 us and more with
+// many rows.  Measured, one CTA each against shares, in us (heads of 128, 4 rows): 8 units of 512 keys 8.4 / 10.0, of 1024 12.4 / 11.2, of
+// 2048 19.3 / 12.0; 64 units of 512 11.4 / 14.5, of 1024 17.1 / 17.4, of 4096 50.7 / 29.5; 256 units of 1024 25.4 / 30.4, of 8192 139 / 135;
+// 304 units of 4096 110 / 87; 512 units of 2048 75 / 77.  With 32 rows: 64 units of 1024 28.4 / 31.4, of 4096 77 / 46; 512 of 2048 108 / 118.
 int few_ctas(const tt_ranges_args& a, int sms) {
-    const long units = (long)a.batch * a.k_heads, slots = 2L * sms;
-    if (units >= 4 * slots || a.kv_len <= 256 || a.batch > kMaxBatch) return 0;
-    return (int)(slots < kMaxShares ? slots : kMaxShares);
+    const long units = (long)a.batch * a.k_heads, slots = 2L * sms, rounds = (units + slots - 1) / slots;
+    const long idle_keys = a.kv_len * (rounds * slots - units) / (rounds * slots);
+    if (idle_keys < 768 + units * (a.q_heads / a.k_heads) * a.q_len / 24 || a.batch > kMaxBatch) return 0;
+    return (int)slots;
 }
 
 template <int D, bool BF16, bool GEN, int MT>
@@ -468,16 +512,17 @@ int launch(const tt_ranges_args& a, const FewParams& p, int dev, cudaStream_t st
     TT_CHECK_LAUNCH();
     if (p.ctas) {
         // started while the pieces are still computed, so that neither its launch nor the counting of the shares is waited for
+        const bool wide = units * rows <= 4L * tt_device().sms;
         cudaLaunchAttribute early = {};
         early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         early.val.programmaticStreamSerializationAllowed = 1;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(units * rows));
+        cfg.gridDim = dim3((unsigned)(wide ? units * rows : (units * rows + 7) / 8));
         cfg.blockDim = dim3(kJoinThreads);
         cfg.stream = st;
         cfg.attrs = &early;
         cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, few_join_kernel<D, BF16>, p);
+        const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, few_join_kernel<D, BF16, 8>, p) : cudaLaunchKernelEx(&cfg, few_join_kernel<D, BF16, 1>, p);
         if (e != cudaSuccess) return tt_record_cuda(e);
     }
     return TT_OK;
@@ -491,7 +536,14 @@ int pick(const tt_ranges_args& a, const FewParams& p, bool gen, int dev, cudaStr
 
 }  // namespace
 
-bool tt_ranges_few_rows(const tt_ranges_args& a) { return a.out32 == nullptr && (long)(a.q_heads / a.k_heads) * a.q_len <= kMaxRows; }
+// At most 32 rows of a group (beyond them, and from 17 on over few short caches, the kernel for tiles is the faster one).  In us, tiles against
+// this: 64 units of 8192 keys, heads of 128, 32 rows 106 / 76, 4 rows 106 / 46; 8 units of 1024 keys, 16 rows 14.5 / 13.5, 32 rows 14.5 / 20.2; 64 units of 1024, 32
+// rows 20.7 / 28.4, of 4096 57 / 46; 256 units of 256, 32 rows 29 / 21.  Heads of 64, 32 rows: 64 units of 1024 19.0 / 18.2.
+bool tt_ranges_few_rows(const tt_ranges_args& a) {
+    const long rows = (long)(a.q_heads / a.k_heads) * a.q_len, units = (long)a.batch * a.k_heads;
+    const bool short_caches = rows > 16 && a.head_dim == 128 && a.kv_len <= 1536 && 2 * units <= tt_device().sms;
+    return a.out32 == nullptr && rows <= kMaxRows && !short_caches;
+}
 
 extern "C" long tt_attn_ranges_fwd_floats(const tt_ranges_args* a) {
     if (tt_ranges_check(a) != TT_OK || !tt_ranges_few_rows(*a)) return 0;

@@ -381,3 +381,14 @@ def test_few_queries_of_many_samples(batch):
     """Both sides of the largest batch whose steps are dealt out."""
     lengths = torch.arange(batch, device="cuda") * 5
     check(batch, 1, 600, 2, 1, 64, BF16, train=False, causal=True, kv_valid_len=lengths, query_start=lengths - 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("batch,hk,group,n,m", [(1, 2, 8, 4, 1700), (2, 3, 20, 1, 2500), (40, 8, 4, 1, 2500), (70, 8, 2, 9, 300), (37, 8, 32, 1, 700),
+                                                (1, 1, 17, 1, 1536), (1, 1, 17, 1, 1537), (75, 1, 32, 1, 600)])
+def test_few_queries_by_shares_and_by_heads(batch, hk, group, n, m, D):
+    """Few and many samples and key heads, on either side of what makes shares of them, with one and with two tiles of rows."""
+    torch.manual_seed(batch + m)
+    lengths = torch.randint(n, m + 1, (batch,), device="cuda")
+    lengths[0] = m
+    check(batch, n, m, hk * group, hk, D, BF16, train=False, causal=True, kv_valid_len=lengths, query_start=lengths - n)
