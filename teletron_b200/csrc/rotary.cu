@@ -609,11 +609,13 @@ Plan plan(const tt_rotary_args& a, int sms, int mode) {
     while ((1 << p.log_l) < chunks && p.log_l < 5) ++p.log_l;
     const int rows = 32 >> p.log_l;
     const long tokens = a.batch * a.tokens;
-    // All heads of a token in one unit share its angles.  With few tokens a unit takes fewer heads, so that the units cover the device.
-    p.whole = tokens >= (long)sms * kWarps;
+    // All heads of a token in one unit share its angles.  With fewer tokens than three quarters of the device's warps at a CTA an SM a unit takes
+    // fewer heads, so that the units cover the device (32 + 8 heads of 128, parts against whole tokens: 256 tokens 4.0 / 6.0 us, 600
+    // 5.4 / 6.1, 1100 7.9 / 6.8, 2000 9.8 / 8.8).
+    p.whole = tokens >= (long)sms * (kWarps * 3 / 4);
     auto heads_per_unit = [&](int heads) {
         int per = (heads + rows - 1) / rows;
-        while (per > 1 && tokens * ((heads + rows * per - 1) / (rows * per)) < (long)sms * kWarps) per = (per + 1) / 2;
+        while (!p.whole && per > 1 && tokens * ((heads + rows * per - 1) / (rows * per)) < (long)sms * kWarps) per = (per + 1) / 2;
         return rows * (per > 0 ? per : 1);
     };
     p.hpu_q = heads_per_unit(a.q_heads);

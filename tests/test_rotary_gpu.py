@@ -163,6 +163,24 @@ def test_empty_operands(tokens, heads_q, heads_k):
         assert bool(torch.isfinite(dq).all()) and bool(torch.isfinite(dk).all())
 
 
+@pytest.mark.parametrize("tokens", [887, 888, 1184])
+def test_tokens_on_either_side_of_whole_units(tokens):
+    """A unit of work takes some heads of a token or all of them: the same results, and the same as of the tokens one by one."""
+    torch.manual_seed(6)
+    q, k = (torch.randn(1, tokens, h, 64, device="cuda", dtype=torch.bfloat16).transpose(1, 2).requires_grad_() for h in (20, 3))
+    wq, wk = (torch.randn(64, device="cuda", dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    freqs, pos = ops.rotary_frequencies(64, device="cuda"), torch.arange(tokens, device="cuda")
+    for op in (lambda a, b, p: ops.rotary(a, b, p, freqs), lambda a, b, p: ops.qk_norm_rotary(a, b, wq, wk, p, freqs)):
+        out = op(q, k, pos)
+        dout = [torch.randn_like(t) for t in out]
+        grads = torch.autograd.grad(out, (q, k), dout)
+        for i in range(0, tokens, 300):
+            part = op(q[:, :, i:i + 300], k[:, :, i:i + 300], pos[i:i + 300])
+            assert all(torch.equal(a, b[:, :, i:i + 300]) for a, b in zip(part, out))
+            for a, b in zip(torch.autograd.grad(part, (q, k), [g[:, :, i:i + 300] for g in dout]), grads):
+                assert torch.equal(a[:, :, i:i + 300], b[:, :, i:i + 300])
+
+
 def test_norm_without_eps_at_heads_that_do_not_fill_a_warp():
     torch.manual_seed(5)
     q, k = (torch.randn(2, h, 9, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for h in (3, 1))
