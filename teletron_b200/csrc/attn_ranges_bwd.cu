@@ -14,9 +14,10 @@
 // dP (in a second buffer) are formed behind this chunk's dS.  Warp
 // 0 loads, warp 1 issues, sixteen warps turn T1, T2 into P and dS (a thread: one stationary row, 32 streamed ones).
 //
-// Measured (bf16, heads of 128), dK dV and dQ: five clips packed into 32656 tokens x 24 heads 4.4 - 4.7 and 2.9 - 3.0 ms (1.1 - 1.3 PFLOP/s of the products
-// executed; the power cap holds long runs to 1.38); 2 x 4095 tokens x 32 heads, causal behind a prefix, capped 590 - 640 and 470 - 510 us; 4 x 512 tokens x 64 heads of 64 with
-// a bias 90 us, with its gradient 111, where every item has four chunks and its first loads, sums and output are half of it.
+// Measured (bf16, heads of 128), dK dV and dQ: five clips packed into 32656 tokens x 24 heads 4.4 - 4.7 and 2.9 - 3.0 ms (1.1 - 1.3 PFLOP/s of the
+// products executed; the power cap holds long runs to 1.38); 2 x 4095 tokens x 32 heads, causal behind a prefix, capped 590 - 640 and 470 - 510 us; 4
+// x 512 tokens x 64 heads of 64 with a bias 90 us, with its gradient 111, where every item has four chunks and its first loads, sums and output are
+// half of it.
 #include <limits.h>
 
 #include <type_traits>

@@ -1,13 +1,14 @@
 // The attention of attn_ranges_fwd.cu for few queries over long keys (new tokens over a cache): at most 32 rows of a key head's group.
 //
-// What bounds it is reading keys and values once, so the steps of 16 keys of all samples and key heads, counted as the samples' runs have
-// them, are dealt to the CTAs in equal shares, and a share's steps to its four warps.  Every warp streams its keys and values through a ring of its own in shared memory (16-byte asynchronous copies, three steps
-// deep: 96 KB in flight per CTA at heads of 128) and keeps running maxima, sums and outputs of its 16 or 32 rows (the queries of all heads of the
-// group, so that shared keys are read once) in registers; the products are mma.sync of 16 x 8 x 16, which a tile of 128 queries on
-// tcgen05 would leave seven eighths empty.  Warps are joined through shared memory, CTAs by a second kernel in a fixed order.
+// What bounds it is reading keys and values once, so the steps of 16 keys of all samples and key heads, counted as the samples' runs have them, are
+// dealt to the CTAs in equal shares, and a share's steps to its four warps.  Every warp streams its keys and values through a ring of its own in
+// shared memory (16-byte asynchronous copies, three steps deep: 96 KB in flight per CTA at heads of 128) and keeps running maxima, sums and outputs
+// of its 16 or 32 rows (the queries of all heads of the group, so that shared keys are read once) in registers; the products are mma.sync of 16 x 8 x
+// 16, which a tile of 128 queries on tcgen05 would leave seven eighths empty.  Warps are joined through shared memory, CTAs by a second kernel in a
+// fixed order.
 //
-// Measured: one token each of eight samples over up to 8192 keys (32 heads of 128 on 8) 43.7 us, 4.7 TB/s; of 76 samples over up to 8192 keys 305 us (6.7 TB/s).  The rest is the first
-// loads of every share, the border of heads inside some of them, and the join.
+// Measured: one token each of eight samples over up to 8192 keys (32 heads of 128 on 8) 43.7 us, 4.7 TB/s; of 76 samples over up to 8192 keys 305 us
+// (6.7 TB/s).  The rest is the first loads of every share, the border of heads inside some of them, and the join.
 #include <limits.h>
 
 #include "attn_ranges.cuh"
@@ -539,9 +540,9 @@ int pick(const tt_ranges_args& a, const FewParams& p, bool gen, int dev, cudaStr
 
 }  // namespace
 
-// At most 32 rows of a group (beyond them, and from 17 on over few short caches, the kernel for tiles is the faster one).  In us, tiles against
-// this: 64 units of 8192 keys, heads of 128, 32 rows 106 / 76, 4 rows 106 / 46; 8 units of 1024 keys, 16 rows 14.5 / 13.5, 32 rows 14.5 / 20.2; 64 units of 1024, 32
-// rows 20.7 / 28.4, of 4096 57 / 46; 256 units of 256, 32 rows 29 / 21.  Heads of 64, 32 rows: 64 units of 1024 19.0 / 18.2.
+// At most 32 rows of a group (beyond them, and from 17 on over few short caches, the kernel for tiles is the faster one).  In us, tiles against this:
+// 64 units of 8192 keys, heads of 128, 32 rows 106 / 76, 4 rows 106 / 46; 8 units of 1024 keys, 16 rows 14.5 / 13.5, 32 rows 14.5 / 20.2; 64 units of
+// 1024, 32 rows 20.7 / 28.4, of 4096 57 / 46; 256 units of 256, 32 rows 29 / 21.  Heads of 64, 32 rows: 64 units of 1024 19.0 / 18.2.
 bool tt_ranges_few_rows(const tt_ranges_args& a) {
     const long rows = (long)(a.q_heads / a.k_heads) * a.q_len, units = (long)a.batch * a.k_heads;
     const bool short_caches = rows > 16 && a.head_dim == 128 && a.kv_len <= 1536 && 2 * units <= tt_device().sms;

@@ -4,17 +4,18 @@
 //   s = scale q . k;   s = cap tanh(s / cap);   s += bias[h, clamp(key position - query position, -R, R) + R]
 //   out = softmax over the query's run of keys (s) v;   0 where the run is empty
 //
-// One CTA owns two tiles of 128 queries that ping-pong through the tensor core and share the loaded keys and values: the same queries
-// of two heads of a group where groups are even (both tiles then have the same runs, and keys and values are read once for both), else two
-// neighbouring tiles of one head.  TMEM columns [0, 256): scores of both tiles, overwritten in place by P; from 256 on: both outputs.
-// Warp 0 loads (and clears values that no query sees), warp 1 issues every product, warps 2-5 and 6-9 are the softmax of the tiles, one query
-// per thread.  A CTA goes on with items of the grid that have not been launched, each role at its own pace, so that the loads and first products
-// of one item run behind the softmax and output of the one before.  Tiles of keys that no query of a tile sees are not touched; whole tiles are not masked; between them a warp masks by the
-// bits of its rows' runs.
+// One CTA owns two tiles of 128 queries that ping-pong through the tensor core and share the loaded keys and values: the same queries of two heads of
+// a group where groups are even (both tiles then have the same runs, and keys and values are read once for both), else two neighbouring tiles of one
+// head.  TMEM columns [0, 256): scores of both tiles, overwritten in place by P; from 256 on: both outputs.  Warp 0 loads (and clears values that no
+// query sees), warp 1 issues every product, warps 2-5 and 6-9 are the softmax of the tiles, one query per thread.  A CTA goes on with items of the
+// grid that have not been launched, each role at its own pace, so that the loads and first products of one item run behind the softmax and output of
+// the one before.  Tiles of keys that no query of a tile sees are not touched; whole tiles are not masked; between them a warp masks by the bits of
+// its rows' runs.
 //
-// What bounds it is the chain of a tile (scores, softmax, P V), of which two ping-pong.  Measured (bf16, heads of 128): five clips packed into 32656 tokens x 24 heads
-// 2.2 - 2.3 ms (1.12 - 1.18 PFLOP/s of the visible pairs); 2 x 4095 tokens x 32 heads, causal behind a prefix, capped 355 - 385 us (0.73 - 0.79).  With few tiles a CTA latencies count: 8
-// prompts of 256 tokens 21.5 us; 4 x 512 tokens x 64 heads of 64 with a bias that is trained 74 us, of which the output in both types is a sixth.
+// What bounds it is the chain of a tile (scores, softmax, P V), of which two ping-pong.  Measured (bf16, heads of 128): five clips packed into 32656
+// tokens x 24 heads 2.2 - 2.3 ms (1.12 - 1.18 PFLOP/s of the visible pairs); 2 x 4095 tokens x 32 heads, causal behind a prefix, capped 355 - 385 us
+// (0.73 - 0.79).  With few tiles a CTA latencies count: 8 prompts of 256 tokens 21.5 us; 4 x 512 tokens x 64 heads of 64 with a bias that is trained
+// 74 us, of which the output in both types is a sixth.
 #include <limits.h>
 
 #include "attn_ranges.cuh"

@@ -7,12 +7,12 @@
 // With the norm x is replaced by x^ w, x^ = r x, r = rsqrt(mean x^2 + eps); backward, with g' the rotated-back gradient:
 // dw = sum over rows of g' x^, dx = r (g' w - x^ mean(g' w x^)).
 //
-// No table is read: the angle of a (token, pair) is shared by all heads, so a warp forms it once per token, in 64 bits (a
-// position of 10^5 times a frequency near 1 leaves 2^-7 of a turn's fraction in 32 bits), reduced to a part of a turn and spread over
-// the lanes while the first heads' elements are being loaded.  The kernels are bound by memory: 2 passes over q and k forward, 3 for the norm's
-// backward.  Measured (bf16, heads of 128): 24 + 24 heads of 32400 tokens, rotation there and back 252 us (6.3 TB/s), norm and rotation forward 138 (5.8),
-// backward 199 (6.0) and 4 for the weights' gradients; 4 x 8192 tokens of 32 + 8 heads (fp16) 107 (6.3); eight tokens 3.4, most of it the launch.  fp32 heads of 80 with
-// 20 rotated elements go two elements a lane (142 MB there and back in 56 us, 2.5 TB/s).
+// No table is read: the angle of a (token, pair) is shared by all heads, so a warp forms it once per token, in 64 bits (in 32 a position of 10^5 times a
+// frequency near 1 is off by up to 2^-8 of a radian), reduced to a part of a turn and spread over the lanes while the first heads'
+// elements are being loaded.  The kernels are bound by memory: 2 passes over q and k forward, 3 for the norm's backward.  Measured (bf16, heads of
+// 128): 24 + 24 heads of 32400 tokens, rotation there and back 252 us (6.3 TB/s), norm and rotation forward 138 (5.8), backward 199 (6.0) and 4 for
+// the weights' gradients; 4 x 8192 tokens of 32 + 8 heads (fp16) 107 (6.3); eight tokens 3.4, most of it the launch.  fp32 heads of 80 with 20
+// rotated elements go two elements a lane (142 MB there and back in 56 us, 2.5 TB/s).
 #include <cuda_fp16.h>
 #include <limits.h>
 

@@ -147,6 +147,7 @@ def key_ranges(q_len: int, kv_len: Optional[int] = None, *, batch: int = 1, caus
         return KeyRanges(batch, q_len, kv_len, first, behind, start, None, bool(causal))
     at = _layout(batch, q_len, kv_len)
     with torch.cuda.device(device):
+        status_tensor(device)           # here, since in a captured attention it would be cleared by replays only
         plan = torch.empty(at.ints, dtype=torch.int32, device=device)
         call("tt_key_ranges", ptr(plan), c_int(batch), c_int(q_len), c_int(kv_len), c_int(causal), ptr(documents), c_int(n or 0),
              c_long(0 if documents is None or documents.shape[0] == 1 else documents.shape[1]), ptr(prefix),

@@ -392,3 +392,74 @@ def test_few_queries_by_shares_and_by_heads(batch, hk, group, n, m, D):
     lengths = torch.randint(n, m + 1, (batch,), device="cuda")
     lengths[0] = m
     check(batch, n, m, hk * group, hk, D, BF16, train=False, causal=True, kv_valid_len=lengths, query_start=lengths - n)
+
+
+def test_broadcast_inputs_and_inputs_given_twice():
+    torch.manual_seed(12)
+    freqs, pos = ops.rotary_frequencies(64, device="cuda"), torch.arange(150, device="cuda")
+    r = ops.key_ranges(150, batch=2, causal=True, device="cuda")
+    x = torch.randn(2, 2, 150, 64, device="cuda").to(BF16).requires_grad_()
+    one = torch.randn(1, 1, 150, 64, device="cuda").to(BF16).requires_grad_()
+    dout = torch.randn(2, 150, 128, device="cuda").to(BF16)
+
+    def run(q, k, v):
+        q, k = ops.rotary(q, k, pos, freqs)
+        return ops.masked_attention(q, k, v, r)
+
+    shared = run(x, one.expand(2, 2, -1, -1), one.expand(2, 1, -1, -1).expand(2, 2, -1, -1))
+    got = torch.autograd.grad(shared, (x, one), dout)
+    k, v = (one.detach().repeat(2, 2, 1, 1).requires_grad_() for _ in range(2))
+    own = run(x, k, v)
+    dx, dk, dv = torch.autograd.grad(own, (x, k, v), dout)
+    assert torch.equal(shared, own) and torch.equal(got[0], dx)
+    # autograd adds the four copies' gradients, and those of both operands, in bf16
+    want, size = (f(dk.double()) + f(dv.double()) for f in (lambda t: t.sum((0, 1), keepdim=True), lambda t: t.abs().sum((0, 1), keepdim=True)))
+    assert bool(((got[1].double() - want).abs() <= 6 * 2.0 ** -8 * size).all())
+    same, = torch.autograd.grad(run(x, x, x), x, dout)
+    q, k, v = (x.detach().clone().requires_grad_() for _ in range(3))
+    parts = [g.double() for g in torch.autograd.grad(run(q, k, v), (q, k, v), dout)]
+    assert bool(((same.double() - sum(parts)).abs() <= 2 * 2.0 ** -8 * sum(g.abs() for g in parts)).all())
+
+
+def test_a_captured_backward_while_an_eager_graph_of_the_same_leaves_lives():
+    torch.manual_seed(13)
+    freqs, pos = ops.rotary_frequencies(64, device="cuda"), torch.arange(150, device="cuda")
+    r = ops.key_ranges(150, causal=True, device="cuda")
+    leaves = [torch.randn(1, 2, 150, 64, device="cuda").to(BF16).requires_grad_() for _ in range(3)]
+    leaves += [torch.randn(64, device="cuda").to(BF16).requires_grad_() for _ in range(2)] + [torch.randn(2, 41, device="cuda").requires_grad_()]
+    dout = torch.randn(1, 150, 128, device="cuda").to(BF16)
+
+    def forward():
+        q, k = ops.qk_norm_rotary(*leaves[:2], *leaves[3:5], pos, freqs)
+        return ops.masked_attention(q, k, leaves[2], r, distance_bias=leaves[5])
+
+    # on the stream that is captured: the eager graph's accumulation nodes belong to the stream that they were made on, and the engine
+    # makes that one wait for what is captured, whatever the operator is
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = torch.autograd.grad(forward(), leaves, dout)
+        alive = forward()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        held = torch.autograd.grad(forward(), leaves, dout)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(held, want))
+    with torch.cuda.stream(side):
+        again = torch.autograd.grad(alive, leaves, dout)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_a_first_call_in_a_captured_graph(monkeypatch):
+    from teletron_b200.ops import gemm_tcgen05
+    monkeypatch.setattr(gemm_tcgen05, "_STATUS", {})
+    q = torch.randn(1, 2, 150, 64, device="cuda").to(BF16)
+    r = ops.key_ranges(150, causal=True, device="cuda")
+    word, = gemm_tcgen05._STATUS.values()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.masked_attention(q, q, q, r)
+    assert list(gemm_tcgen05._STATUS.values())[0] is word and not bool(word.any())
+    graph.replay()
+    assert torch.equal(held, ops.masked_attention(q, q, q, r))
