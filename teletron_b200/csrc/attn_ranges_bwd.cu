@@ -415,12 +415,17 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 const Chunk ch = chunk_at(w, c);
                 const int col0 = ch.t * kTile + part * kCols;         // first streamed row of this thread's 32
                 uint32_t see = 0xffffffffu;
+                bool one = false;           // the query (KVS: of column `lane`) sees one key
                 if (KVS) {
                     const int4 r = plan.q_tiles[ch.t];
-                    if (r.z > r0 || r.w < min(r0 + kTile, p.kv_len)) {         // some query does not see all of these keys
+                    if (r.z > r0 || r.w < min(r0 + kTile, p.kv_len) || p.kv_len - r0 == 1) {        // some query does not see all of these keys, or it is one
                         const int q = col0 + lane, k0 = r0 + quad * 32;
                         uint32_t mine = 0u;                                    // keys of this warp that query `lane` sees
-                        if (q < p.q_len) mine = bits_between(plan.first[q] - k0, plan.behind[q] - k0);
+                        if (q < p.q_len) {
+                            const int first = plan.first[q], behind = plan.behind[q];
+                            mine = bits_between(first - k0, behind - k0);
+                            one = behind - first == 1;
+                        }
                         see = 0u;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) see |= (__shfl_sync(0xffffffffu, mine, e) >> lane & 1u) << e;
@@ -524,6 +529,9 @@ ranges_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready);
+                // a query that sees one key weighs it 1 whatever its score: dP - delta is nothing but rounding
+                if (KVS) see &= ~__ballot_sync(0xffffffffu, one);
+                else if (v.behind - v.first == 1) see = 0u;
 
                 // beyond the largest distance the bias's gradient takes sums only
                 const int corner = ch.t * kTile - (start + r0);         // distance of the tile's first key from its first query

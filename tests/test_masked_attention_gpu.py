@@ -463,3 +463,21 @@ def test_a_first_call_in_a_captured_graph(monkeypatch):
     assert list(gemm_tcgen05._STATUS.values())[0] is word and not bool(word.any())
     graph.replay()
     assert torch.equal(held, ops.masked_attention(q, q, q, r))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,mask", [(1, {}), (129, dict(documents=[0, 128, 129])), (300, dict(documents=list(range(301)))), (130, dict(causal=True, documents=[0, 1, 2, 130])),
+                                    (257, dict(causal=True, kv_valid_len=1))])
+def test_queries_that_see_one_key_have_no_gradient_of_their_scores(n, mask, D):
+    torch.manual_seed(14)
+    r = ops.key_ranges(n, batch=2, device="cuda", **mask)
+    for softcap, R in ((None, None), (3.0, None), (None, 9)):
+        q, k, v = (t.requires_grad_() for t in heads(2, n, (4, 2, 2), D, BF16, True))
+        bias = None if R is None else torch.randn(4, 2 * R + 1, device="cuda").requires_grad_()
+        out = ops.masked_attention(q, k, v, r, softcap=softcap, distance_bias=bias)
+        dout = torch.randn_like(out)
+        one = r.behind - r.first == 1
+        grads = torch.autograd.grad(out, (q, k, v) + (() if bias is None else (bias,)), dout)
+        assert not bool(grads[0].transpose(1, 2)[one].any()) and bool(grads[2].any())
+        if bool((one | (r.behind == r.first)).all()):
+            assert not bool(grads[1].any()) and (bias is None or not bool(grads[3].any()))
