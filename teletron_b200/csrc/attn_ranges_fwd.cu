@@ -61,7 +61,7 @@ static_assert(Layout<128>::smem(TT_RANGES_MAX_DISTANCE) <= 232448, "shared memor
 enum { kPlain = 0, kGeneral = 1, kGeneralWide = 2 };
 
 // kGeneral: scores are scaled (by any factor), capped and biased ahead of the softmax; kPlain: the positive scale is part of its exponent.
-// kGeneralWide, for a bias that is trained, also writes the output before rounding, to 2^-16 instead of P's 2^-8: P is split into two 16-bit
+// kGeneralWide, for a bias that is trained and for trained calls of few keys, also writes the output before rounding, to 2^-16 instead of P's 2^-8: P is split into two 16-bit
 // parts (the second one takes the 64 columns that the scores leave free) and multiplied twice.  The bias's gradient sums P (dP - delta)
 // over whole diagonals in 32 bits; with delta from a product with rounded P it was good to 1e-3 only.
 template <int D, bool BF16, int MODE>

@@ -481,3 +481,20 @@ def test_queries_that_see_one_key_have_no_gradient_of_their_scores(n, mask, D):
         assert not bool(grads[0].transpose(1, 2)[one].any()) and bool(grads[2].any())
         if bool((one | (r.behind == r.first)).all()):
             assert not bool(grads[1].any()) and (bias is None or not bool(grads[3].any()))
+
+
+@pytest.mark.parametrize("n", [2, 3, 16, 128, 129])
+def test_gradients_of_few_keys(n):
+    """dP - delta of few keys is small against both: the gradients are no further off than their own rounding and that of dS."""
+    torch.manual_seed(15)
+    q, k, v = (t.requires_grad_() for t in heads(4, n, (8, 8, 8), 128, BF16, True))
+    r = ops.key_ranges(n, batch=4, causal=True, device="cuda")
+    out = ops.masked_attention(q, k, v, r)
+    dout = torch.randn_like(out)
+    got = torch.autograd.grad(out, (q, k, v), dout)
+    x = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    with ops.impl("torch"):
+        want = torch.autograd.grad(ops.masked_attention(*x, r), x, dout.double())
+    for a, b in zip(got, want):
+        # two roundings, each off by at most 2^-8 and uniformly spread below that (by 3^-1/2 of it), and for 129 keys delta's
+        assert float((a.double() - b).norm() / b.norm()) < (2 if n <= 128 else 3) ** 0.5 * 2.0 ** -8 / 3 ** 0.5
