@@ -164,7 +164,7 @@ int tt_attn_bwd_uses_pairs(int heads, int S, int sms);
 /* ---- attention in which every query sees one run of the keys (attn_ranges*.cu) ---- */
 #define TT_RANGES_TILE 128          /* rows of a tile of queries and of a tile of keys */
 #define TT_RANGES_MAX_DISTANCE 1024
-/* Offsets, in ints, of the parts of a plan for `batch` samples; the whole takes tt_key_ranges_ints. */
+/* Offsets, in ints, of the parts of a plan for `batch` samples; the whole takes `ints`. */
 typedef struct {
     long q_tiles;       /* [batch, tiles of queries, 4]: first key any of them sees, behind the last, first key all see, behind the last */
     long dead;          /* [batch, tiles of keys, 4]: bit j: key j of the tile is seen by no query */
