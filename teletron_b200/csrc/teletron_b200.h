@@ -85,7 +85,8 @@ typedef struct {
     float* partials;                    /* scratch of the backward: partial_floats >= tt_rotary_partial_floats */
     long partial_floats;
 } tt_rotary_args;
-long tt_rotary_partial_floats(const tt_rotary_args* args);     /* of the norm's backward; touches no device memory */
+/* of the norm's backward with these arguments (the alignment of every operand counts, the gradients' among them); touches no device memory */
+long tt_rotary_partial_floats(const tt_rotary_args* args);
 int tt_rotary(const tt_rotary_args* args, void* stream);
 int tt_norm_rotary_fwd(const tt_rotary_args* args, void* stream);
 int tt_norm_rotary_bwd(const tt_rotary_args* args, void* stream);

@@ -295,10 +295,10 @@ def _norm_backward(ctx, gq, gk):
                 dw.zero_()
         if some_q or some_k:
             head = _pack(q if some_q else None, k if some_k else None, dq, dk, positions, ctx.pos_stride, ctx.freqs, False, ctx.eps, q_weight, k_weight)
-            size = _lib.lib().tt_rotary_partial_floats(head + _NO_BACKWARD)
+            grads = (gq.data_ptr(), gk.data_ptr(), *gq.stride()[:3], *gk.stride()[:3], dqw.data_ptr(), dkw.data_ptr())
+            size = _lib.lib().tt_rotary_partial_floats(head + _TAIL.pack(*grads, 0, 0))         # by the gradients' alignment too
             partials = q.new_empty((max(size, 1),), dtype=torch.float32)
-            call("tt_norm_rotary_bwd", head + _TAIL.pack(gq.data_ptr(), gk.data_ptr(), *gq.stride()[:3], *gk.stride()[:3], dqw.data_ptr(), dkw.data_ptr(),
-                                                         partials.data_ptr(), size), stream())
+            call("tt_norm_rotary_bwd", head + _TAIL.pack(*grads, partials.data_ptr(), size), stream())
     a, b, c, d = ctx.needs_input_grad[:4]
     return dq if a else None, dk if b else None, dqw if c else None, dkw if d else None, None, None, None, None
 

@@ -153,3 +153,32 @@ def test_native_arguments_have_the_layout_that_the_library_expects():
     wide = rope._ARGS.pack(rope._ARGS.size, 1, 4, 2, 1, 258, 4, 2, 0, 0, 0, 16, 16, *[0] * 6, 16, 16, *[0] * 6, 16, 0, 0, 1, 16, 0, 1.0, 0.0,
                            16, 16, 16, 16, *[0] * 6, 16, 16, 0, 0)
     assert _lib.lib().tt_norm_rotary_fwd(wide, None) == 4
+
+
+def _recorded(monkeypatch):
+    """The native calls of the op layer, noted instead of made, on tensors of the host."""
+    import contextlib
+    from teletron_b200.ops import rope
+    calls = []
+    monkeypatch.setattr(rope, "call", lambda name, args, stream: calls.append((name, args)))
+    monkeypatch.setattr(rope, "stream", lambda: None)
+    monkeypatch.setattr(rope, "on_device", lambda t: contextlib.nullcontext())
+    return calls
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 100, 887, 2000])
+@pytest.mark.parametrize("behind", [0, 1, 2])
+def test_the_scratch_of_the_norms_backward_is_sized_for_its_gradients(monkeypatch, tokens, behind):
+    """Gradients at other alignments than the inputs (views into wider rows) change how the work is shared out."""
+    from teletron_b200.ops import _lib, rope
+    if not _lib.available():
+        pytest.skip("native library not built")
+    calls = _recorded(monkeypatch)
+    q, k = (torch.randn(1, h, tokens, 128).bfloat16().requires_grad_() for h in (32, 8))
+    w = torch.ones(128, dtype=torch.bfloat16, requires_grad=True)
+    outs = rope.qk_norm_rotary(q, k, w, w, torch.arange(tokens), (0, 0, 1), ops.rotary_frequencies(128), 1e-6)
+    torch.autograd.grad(outs, (q, k), [torch.randn(1, h, tokens, 128 + behind).bfloat16()[..., behind:] for h in (32, 8)])
+    (name, args), = calls[1:]
+    assert name == "tt_norm_rotary_bwd"
+    given, = rope.struct.unpack_from("@l", args, len(args) - 8)
+    assert given == _lib.lib().tt_rotary_partial_floats(args) > 0

@@ -257,3 +257,30 @@ def test_wide_heads_take_the_plain_path_with_a_note():
             ops.rotary(x, None, pos, freqs)
     finally:
         fallback.set_strict(was)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("behind", [1, 2])
+@pytest.mark.parametrize("tokens", [1, 8, 100])
+def test_gradients_at_other_alignments_than_the_inputs(tokens, behind, dtype):
+    """What a concatenation's backward hands on: views into wider rows."""
+    torch.manual_seed(7)
+    q, k = (torch.randn(1, h, tokens, 128, device="cuda").to(dtype).requires_grad_() for h in (32, 8))
+    w = [(1 + 0.2 * torch.randn(128, device="cuda")).to(dtype).requires_grad_() for _ in range(2)]
+    freqs, pos = ops.rotary_frequencies(128, device="cuda"), torch.arange(tokens, device="cuda")
+    a = angles(pos[None, None], inverse_frequencies(128, 10000.0))
+    outs = ops.qk_norm_rotary(q, k, *w, pos, freqs)
+    grads = [torch.randn(*o.shape[:3], 128 + behind, device="cuda").to(dtype)[..., behind:] for o in outs]
+    got = torch.autograd.grad(outs, (q, k, *w), grads)
+    rel = norm_error(128)
+    for i, (x, g) in enumerate(zip((q, k), grads)):
+        xd, wd, gd = x.detach().double(), w[i].detach().double(), g.double()
+        r = torch.rsqrt(xd.square().mean(-1, keepdim=True) + 1e-6)
+        hat = xd * r
+        back, back_size = turn(gd, -a, 1.0, False), pair_size(gd, 64, 1.0, False)
+        dw = (back * hat).sum((0, 1, 2))
+        close(got[2 + i], dw, rounding(dtype, dw) + (back_size * hat.abs()).sum((0, 1, 2)) * (x[..., 0].numel() * U32 + ROTATION + rel), "dw")
+        gw = back * wd
+        dx = r * (gw - hat * (gw * hat).mean(-1, keepdim=True))
+        spread = r * (back_size * wd.abs() + hat.abs() * (back_size * wd.abs() * hat.abs()).mean(-1, keepdim=True))
+        close(got[i], dx, rounding(dtype, dx) + spread * (ROTATION + 3 * rel + 128 * U32), "dx")
