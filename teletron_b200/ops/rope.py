@@ -51,17 +51,59 @@ class Rotary:
         return dataclasses.replace(self, inv_freq=move(self.inv_freq), half_turns=move(self.half_turns), axis=move(self.axis))
 
 
-def _need(scaling: dict, name: str, kind: str) -> float:
-    if name not in scaling:
-        raise ValueError(f"rotary scaling {kind!r} needs {name!r}")
+_LARGEST = 1e30          # of an amplitude, which the kernels hold in 32 bits
+# What a dictionary may hold: the kind, what belongs to the caller's other arguments or says nothing about angles, and the keys of any kind (a kind passes
+# over those of the others, as configurations carry them along).  A key that is not here might change angles in a way that is not followed.
+_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "max_position_embeddings", "finetuned", "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor",
+         "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"}
+
+
+def _positive(scaling: dict, name: str) -> Optional[float]:
+    """The number under ``name``, or None where there is none."""
+    if scaling.get(name) is None:
+        return None
     value = float(scaling[name])
     if not (math.isfinite(value) and value > 0):
         raise ValueError(f"rotary scaling: {name} must be positive, got {scaling[name]}")
     return value
 
 
+def _need(scaling: dict, name: str, kind: str) -> float:
+    value = _positive(scaling, name)
+    if value is None:
+        raise ValueError(f"rotary scaling {kind!r} needs {name!r}")
+    return value
+
+
+def _check_scaling(scaling: dict, theta: float) -> str:
+    """The kind of scaling; raises ``ValueError`` for what would be passed over."""
+    unknown = [k for k, v in scaling.items() if k not in _KEYS and v is not None]
+    if unknown:
+        raise ValueError(f"rotary scaling: unknown keys {unknown}")
+    kind = scaling.get("rope_type", scaling.get("type"))
+    if kind is None:
+        if scaling.get("factor") is not None:
+            raise ValueError("rotary scaling: a factor needs a 'rope_type'")
+        kind = "default"
+    if scaling.get("rope_theta") is not None and float(scaling["rope_theta"]) != theta:
+        raise ValueError(f"rotary scaling: rope_theta {scaling['rope_theta']} is not theta {theta}")
+    return kind
+
+
+def _yarn_amplitude(scaling: dict, factor: float) -> float:
+    amplitude = scaling.get("attention_factor")
+    if amplitude is None:
+        over, under = (_positive(scaling, name) if scaling.get(name) else None for name in ("mscale", "mscale_all_dim"))     # 0: not given
+        log = math.log(factor) if factor > 1 else 0.0
+        amplitude = 0.1 * log + 1.0 if over is None or under is None else (0.1 * over * log + 1.0) / (0.1 * under * log + 1.0)
+    amplitude = float(amplitude)
+    if not abs(amplitude) <= _LARGEST:
+        raise ValueError(f"rotary scaling: amplitude {amplitude} is not finite, or beyond {_LARGEST}")
+    return amplitude
+
+
 def _axis_frequencies(dim: int, theta: float, scaling: dict) -> Tuple[torch.Tensor, float]:
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    kind = _check_scaling(scaling, theta)
     j = torch.arange(0, dim, 2, dtype=torch.float64)
     inv = theta ** (-j / dim)
     if kind in ("default", "none"):
@@ -84,17 +126,17 @@ def _axis_frequencies(dim: int, theta: float, scaling: dict) -> Tuple[torch.Tens
         return keep * inv + (1.0 - keep) * inv / factor, 1.0
     if theta <= 1.0:
         raise ValueError("rotary scaling 'yarn' needs a theta above 1")
-    fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+    fast, slow = (_positive(scaling, name) if scaling.get(name) else turns for name, turns in (("beta_fast", 32.0), ("beta_slow", 1.0)))     # 0: not given
 
     def pair_with(turns: float) -> float:
         return dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-    low, high = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), dim - 1)
+    low, high = pair_with(fast), pair_with(slow)
+    if scaling.get("truncate", True):           # the ramp from whole pair to whole pair
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, dim - 1)
     ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
-    amplitude = scaling.get("attention_factor")
-    if amplitude is None:
-        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
-    return (1.0 - ramp) * inv + ramp * inv / factor, float(amplitude)
+    return (1.0 - ramp) * inv + ramp * inv / factor, _yarn_amplitude(scaling, factor)
 
 
 def rotary_frequencies(dim: int, theta: float = 10000.0, *, axes: Optional[Sequence[int]] = None, scaling: Optional[dict] = None,
@@ -105,7 +147,8 @@ def rotary_frequencies(dim: int, theta: float = 10000.0, *, axes: Optional[Seque
     ``dim`` and every axis starts with its fastest pair).  ``scaling``: a model configuration's dictionary, ``rope_type`` one of
     ``linear`` and ``ntk`` (``factor``), ``llama3`` (``factor``, ``low_freq_factor``, ``high_freq_factor``,
     ``original_max_position_embeddings``), ``yarn`` (``factor``, ``original_max_position_embeddings``; optionally ``beta_fast``, ``beta_slow``,
-    ``attention_factor``); it applies to every axis."""
+    ``truncate``, ``mscale`` with ``mscale_all_dim``, ``attention_factor``); it applies to every axis.  Keys that no kind knows, a factor without a kind
+    and a ``rope_theta`` other than ``theta`` are refused."""
     dims = [int(dim)] if axes is None else [int(a) for a in axes]
     if not dims or any(d <= 0 or d % 2 for d in dims) or sum(dims) != dim:
         raise ValueError(f"rotary dims must be positive, even and sum to {dim}, got {dims}")

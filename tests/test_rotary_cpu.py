@@ -182,3 +182,52 @@ def test_the_scratch_of_the_norms_backward_is_sized_for_its_gradients(monkeypatc
     assert name == "tt_norm_rotary_bwd"
     given, = rope.struct.unpack_from("@l", args, len(args) - 8)
     assert given == _lib.lib().tt_rotary_partial_floats(args) > 0
+
+
+@pytest.mark.parametrize("extra", [dict(truncate=False), dict(truncate=True), dict(truncate=False, beta_fast=20.0, beta_slow=2.0),
+                                   dict(mscale=0.707, mscale_all_dim=0.707), dict(mscale=1.0, mscale_all_dim=0.707), dict(mscale=1.0, mscale_all_dim=0.5),
+                                   dict(mscale=0.5), dict(mscale_all_dim=0.5), dict(mscale=1.0, mscale_all_dim=0.0), dict(mscale=1.0, mscale_all_dim=0.5, attention_factor=1.25),
+                                   dict(attention_factor=None, mscale=None, mscale_all_dim=None, beta_fast=None, truncate=True)])
+@pytest.mark.parametrize("factor", [4.0, 40.0, 1.0])
+def test_yarn_follows_all_of_its_keys(extra, factor):
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    scaling = dict(rope_type="yarn", factor=factor, rope_theta=500000.0, original_max_position_embeddings=2048, **extra)
+    cfg = LlamaConfig(hidden_size=512, num_attention_heads=4, max_position_embeddings=8192, rope_parameters=dict(scaling))
+    inv, amplitude = ROPE_INIT_FUNCTIONS["yarn"](cfg, "cpu")
+    mine = ops.rotary_frequencies(128, 500000.0, scaling=scaling)
+    assert torch.allclose(mine.inv_freq.float(), inv.float(), rtol=1e-5, atol=0)
+    assert math.isclose(mine.amplitude, amplitude, rel_tol=1e-6)
+
+
+def test_yarn_without_truncation_and_with_two_scales_by_its_formulas():
+    dim, theta, factor, context = 64, 10000.0, 8.0, 4096
+    got = ops.rotary_frequencies(dim, theta, scaling=dict(rope_type="yarn", factor=factor, original_max_position_embeddings=context, truncate=False,
+                                                          mscale=1.2, mscale_all_dim=0.4))
+    assert math.isclose(got.amplitude, (0.12 * math.log(factor) + 1) / (0.04 * math.log(factor) + 1), rel_tol=1e-12)
+    low, high = (dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(theta)) for turns in (32, 1))
+    for j, (have, base) in enumerate(zip(got.inv_freq.tolist(), inverse_frequencies(dim, theta))):
+        stretched = min(max((j - low) / (high - low), 0.0), 1.0)
+        assert math.isclose(have, base * (1 - stretched) + base / factor * stretched, rel_tol=1e-12)
+
+
+@pytest.mark.parametrize("scaling", [dict(rope_type="linear", factor=2.0, short_factor=[1.0]), dict(rope_type="default", alpha=3.0), dict(factor=4.0),
+                                     dict(rope_type="linear", factor=None), dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64, mscal=1.0),
+                                     dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64, attention_factor=float("nan")),
+                                     dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64, attention_factor=1e300),
+                                     dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64, mscale=float("inf"), mscale_all_dim=1.0),
+                                     dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64, mscale=1.0, mscale_all_dim=-10 / math.log(4.0)),
+                                     dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=64, beta_fast=-1.0),
+                                     dict(rope_type="linear", factor=4.0, rope_theta=500000.0)])
+def test_scalings_that_would_not_be_followed_are_refused(scaling):
+    with pytest.raises(ValueError):
+        ops.rotary_frequencies(128, 10000.0, scaling=scaling)
+
+
+def test_what_configurations_hold_beside_the_scaling_is_taken():
+    plain = ops.rotary_frequencies(128, 500000.0)
+    for scaling in ({}, dict(rope_type="default", rope_theta=500000.0), dict(type="default", partial_rotary_factor=0.5), dict(rope_type="default", factor=None),
+                    dict(rope_type="default", factor=1.0, original_max_position_embeddings=8192), dict(rope_theta=500000.0),
+                    dict(rope_type="linear", factor=1.0, finetuned=True, max_position_embeddings=8192)):
+        got = ops.rotary_frequencies(128, 500000.0, scaling=scaling)
+        assert torch.equal(got.inv_freq, plain.inv_freq) and got.amplitude == 1.0
