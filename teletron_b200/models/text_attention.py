@@ -83,13 +83,33 @@ class T5SelfAttention(nn.Module):
         return self.o(o.to(self.o.weight.dtype)), None
 
 
+def rotary_of(cfg) -> ops.Rotary:
+    """Frequencies of a model configuration.  Releases ahead of 5 of the encoders' package keep the scaling in ``rope_scaling`` and the rest beside it."""
+    rope = getattr(cfg, "rope_parameters", None)
+    rope = dict((getattr(cfg, "rope_scaling", None) if rope is None else rope) or {})
+    head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    part = rope.get("partial_rotary_factor") or getattr(cfg, "partial_rotary_factor", None) or 1.0
+    theta = rope.get("rope_theta") or getattr(cfg, "rope_theta", None) or 10000.0
+    return ops.rotary_frequencies(int(head_dim * part), float(theta), scaling=rope)
+
+
+def _check_rotary(model, freqs: ops.Rotary) -> None:
+    """Raises ``ValueError`` where the model's own table says otherwise (16-bit models hold it in 16 bits)."""
+    own = getattr(model, "rotary_emb", None)
+    inv = getattr(own, "inv_freq", None)
+    if inv is None or inv.is_meta:
+        return
+    amplitude = getattr(own, "attention_scaling", freqs.amplitude)
+    if inv.shape != freqs.inv_freq.shape or not torch.allclose(inv.double().cpu(), freqs.inv_freq, rtol=2 ** -7, atol=2 ** -24) \
+            or not math.isclose(amplitude, freqs.amplitude, rel_tol=2 ** -7):
+        raise ValueError("native attention: the model rotates by other frequencies than its configuration says")
+
+
 class _NativeLlama:
     def __init__(self, model):
-        self.shared, cfg = _Shared(), model.config
-        rope = dict(getattr(cfg, "rope_parameters", None) or {})
-        head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
-        freqs = ops.rotary_frequencies(int(head_dim * rope.get("partial_rotary_factor", 1.0)), float(rope.get("rope_theta", getattr(cfg, "rope_theta", 10000.0))),
-                                       scaling=rope, device=model.embed_tokens.weight.device)
+        self.shared, freqs = _Shared(), rotary_of(model.config)
+        _check_rotary(model, freqs)
+        freqs = freqs.to(model.embed_tokens.weight.device)
         for layer in model.layers:
             layer.self_attn = LlamaSelfAttention(layer.self_attn, freqs, self.shared)
 

@@ -83,6 +83,41 @@ def test_refusals_and_flag():
     assert clip_text_config() is not None
 
 
+class _Config:
+    """A configuration as the encoders' package had it ahead of its release 5: the scaling apart from the base."""
+
+    def __init__(self, rope_scaling, rope_theta=500000.0, **kw):
+        self.hidden_size, self.num_attention_heads, self.rope_scaling, self.rope_theta = 64, 4, rope_scaling, rope_theta
+        self.__dict__.update(kw)
+
+
+@pytest.mark.parametrize("scaling", [None, dict(rope_type="llama3", factor=4.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=16),
+                                     dict(type="linear", factor=3.0)])
+def test_scalings_of_older_configurations_are_followed(scaling):
+    from teletron_b200 import ops
+    from teletron_b200.models.text_attention import rotary_of
+    for kw, dim in ((dict(), 16), (dict(partial_rotary_factor=0.5), 8), (dict(head_dim=32), 32)):
+        got, want = rotary_of(_Config(scaling, **kw)), ops.rotary_frequencies(dim, 500000.0, scaling=scaling)
+        assert torch.equal(got.inv_freq, want.inv_freq) and got.amplitude == want.amplitude
+    now = rotary_of(_Config(dict(rope_type="linear", factor=3.0), rope_parameters=dict(rope_type="linear", factor=5.0, rope_theta=10000.0)))
+    assert torch.equal(now.inv_freq, ops.rotary_frequencies(16, 10000.0, scaling=dict(rope_type="linear", factor=5.0)).inv_freq)
+
+
+def test_a_model_that_rotates_otherwise_than_its_configuration_says_is_refused():
+    """Frequencies from the configuration are compared with the model's own, whatever names a release keeps them under."""
+    enc = _llama()[1]
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        use_native_attention(copy.deepcopy(enc.model).to(dtype))
+    enc.model.rotary_emb.inv_freq.div_(4.0)
+    with pytest.raises(ValueError):
+        use_native_attention(enc.model)
+    enc = _llama()[1]
+    enc.model.rotary_emb.attention_scaling = 1.2
+    with pytest.raises(ValueError):
+        use_native_attention(enc.model)
+    assert type(enc.model.layers[0].self_attn).__name__ == "LlamaAttention"         # as it was
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_llama_on_the_kernels(dtype):
