@@ -15,6 +15,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -306,7 +307,8 @@ def masked_attention(q, k, v, ranges, scale, softcap, distance_bias):
     scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)
     with on_device(q):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, distance_bias)):
+        # under a forward-mode level operands may have tangents, which the autograd function refuses and a kernel alone would lose
+        if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, distance_bias))):
             return _MaskedAttention.apply(q, k, v, distance_bias, ranges, scale, softcap)
         bias = None if distance_bias is None else distance_bias.contiguous()
         return _forward(_rows(q), _rows(k), _rows(v), ranges, scale, softcap, bias, False)[0]

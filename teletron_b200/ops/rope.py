@@ -15,6 +15,7 @@ import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -308,7 +309,8 @@ class _Rotary(torch.autograd.Function):
 
 def rotary(q, k, positions, pos_stride, freqs):
     with on_device(q):
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        # (under a forward-mode level operands may have tangents, which the autograd function refuses and a kernel alone would lose)
+        if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
             out = _Rotary.apply(q, k, positions, pos_stride, freqs)
             return (out, None) if k is None else out
         return _forward(q, k, positions, pos_stride, freqs)
@@ -364,6 +366,7 @@ class _NormRotary(torch.autograd.Function):
 def qk_norm_rotary(q, k, q_weight, k_weight, positions, pos_stride, freqs, eps):
     with on_device(q):
         q, k, q_weight, k_weight = _rows(q), _rows(k), q_weight.contiguous(), k_weight.contiguous()
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+        if forward_ad._current_level >= 0 or \
+                (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad)):
             return _NormRotary.apply(q, k, q_weight, k_weight, positions, pos_stride, freqs, float(eps))
         return _norm_forward(q, k, q_weight, k_weight, positions, pos_stride, freqs, float(eps))

@@ -159,3 +159,33 @@ def test_plan_parts_do_not_overlap():
             place += size
         assert at.ints == place and at.dead % 4 == 0 and at.k_tiles % 2 == 0
     assert isinstance(ctypes.sizeof(A._Layout), int)
+
+
+def test_forward_mode_derivatives_are_refused_not_lost(monkeypatch):
+    """Dual tensors need no ``requires_grad``; a kernel reads their primals alone."""
+    import contextlib
+    import torch.autograd.forward_ad as fwd
+    from teletron_b200.ops import _lib, attn_ranges
+    if not _lib.available():
+        pytest.skip("native library not built")
+    calls = []
+    monkeypatch.setattr(attn_ranges, "call", lambda name, *args: calls.append(name))
+    monkeypatch.setattr(attn_ranges, "stream", lambda: None)
+    monkeypatch.setattr(attn_ranges, "on_device", lambda t: contextlib.nullcontext())
+    n, m = 40, 200
+    ranges = ops.key_ranges(n, m, batch=2)
+    object.__setattr__(ranges, "plan", torch.zeros(16, dtype=torch.int32))
+    q, k, v = (torch.randn(2, h, s, 64).bfloat16() for h, s in ((4, n), (2, m), (2, m)))
+    bias = torch.randn(4, 5)
+    with fwd.dual_level():
+        for grad in (True, False):
+            for which in range(4):
+                args = [q, k, v, bias]
+                args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    attn_ranges.masked_attention(*args[:3], ranges, None, None, args[3])
+        before = len(calls)
+        attn_ranges.masked_attention(q, k, v, ranges, None, None, bias)         # no tangents: as ever
+        assert len(calls) == before + 1
+    with pytest.raises(RuntimeError):           # the same by transformation
+        torch.func.jvp(lambda x: attn_ranges.masked_attention(x, k, v, ranges, None, None, None), (q,), (q,))

@@ -498,3 +498,20 @@ def test_gradients_of_few_keys(n):
     for a, b in zip(got, want):
         # two roundings, each off by at most 2^-8 and uniformly spread below that (by 3^-1/2 of it), and for 129 keys delta's
         assert float((a.double() - b).norm() / b.norm()) < (2 if n <= 128 else 3) ** 0.5 * 2.0 ** -8 / 3 ** 0.5
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    freqs, pos, w = ops.rotary_frequencies(64, device="cuda"), torch.arange(9, device="cuda"), torch.ones(64, device="cuda", dtype=BF16)
+    q = torch.randn(1, 2, 9, 64, device="cuda").to(BF16)
+    runs_ = ops.key_ranges(9, causal=True, device="cuda")
+    want = ops.masked_attention(q, q, q, runs_), ops.rotary(q, q, pos, freqs)[0], ops.qk_norm_rotary(q, q, w, w, pos, freqs)[0]
+    with fwd.dual_level():
+        x = fwd.make_dual(q, torch.ones_like(q))
+        for f in (lambda: ops.masked_attention(q, x, q, runs_), lambda: ops.rotary(q, x, pos, freqs), lambda: ops.qk_norm_rotary(x, q, w, w, pos, freqs)):
+            with pytest.raises(RuntimeError):
+                f()
+        got = ops.masked_attention(q, q, q, runs_), ops.rotary(q, q, pos, freqs)[0], ops.qk_norm_rotary(q, q, w, w, pos, freqs)[0]
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    # few rows by themselves and in a tile: P is rounded to bf16 against another maximum, and the output once, in each
+    assert torch.allclose(got[0].float(), want[0].float(), atol=4 * 2.0 ** -8 * float(q.float().abs().max()), rtol=0)

@@ -231,3 +231,36 @@ def test_what_configurations_hold_beside_the_scaling_is_taken():
                     dict(rope_type="linear", factor=1.0, finetuned=True, max_position_embeddings=8192)):
         got = ops.rotary_frequencies(128, 500000.0, scaling=scaling)
         assert torch.equal(got.inv_freq, plain.inv_freq) and got.amplitude == 1.0
+
+
+def test_forward_mode_derivatives_are_refused_not_lost(monkeypatch):
+    """Dual tensors need no ``requires_grad``; a kernel reads their primals alone."""
+    import torch.autograd.forward_ad as fwd
+    from teletron_b200.ops import _lib, rope
+    if not _lib.available():
+        pytest.skip("native library not built")
+    calls = _recorded(monkeypatch)
+    freqs, pos, w = ops.rotary_frequencies(64), torch.arange(3), torch.ones(64)
+    q, k = torch.randn(1, 2, 3, 64), torch.randn(1, 1, 3, 64)
+    with fwd.dual_level():
+        for grad in (True, False):
+            for which in range(4):
+                args = [q, k, w, w]
+                args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+                with torch.set_grad_enabled(grad):
+                    with pytest.raises(RuntimeError):
+                        rope.qk_norm_rotary(*args, pos, (0, 0, 1), freqs, 1e-6)
+                    if which < 2:
+                        with pytest.raises(RuntimeError):
+                            rope.rotary(*args[:2], pos, (0, 0, 1), freqs)
+        with pytest.raises(RuntimeError):
+            rope.rotary(fwd.make_dual(q, q), None, pos, (0, 0, 1), freqs)
+        n = len(calls)
+        rope.rotary(q, k, pos, (0, 0, 1), freqs)            # no tangents: as ever
+        rope.qk_norm_rotary(q, k, w, w, pos, (0, 0, 1), freqs, 1e-6)
+        assert len(calls) == n + 2
+        # the plain path carries them
+        out, _ = ops.rotary(fwd.make_dual(q, q), None, pos, freqs)
+        assert torch.allclose(fwd.unpack_dual(out).tangent, ops.rotary(q, None, pos, freqs)[0], atol=1e-5)
+    with pytest.raises(RuntimeError):           # the same by transformation
+        torch.func.jvp(lambda x: rope.rotary(x, k, pos, (0, 0, 1), freqs)[0], (q,), (q,))
