@@ -9,7 +9,8 @@ library (``teletron/models/hunyuanvideo/text_encoder.py:125-238``).
 from __future__ import annotations
 
 import math
-from typing import Optional
+import threading
+from typing import NamedTuple, Optional
 
 import torch
 from torch import nn
@@ -47,11 +48,33 @@ def prompt_ranges(mask: Optional[torch.Tensor], batch: int, length: int, causal:
     raise ValueError("native attention takes prompts that are padded on one side")
 
 
-class _Shared:
+class _Prepared(NamedTuple):
     """What the layers of one call share."""
-    ranges: Optional[ops.KeyRanges] = None
+    ranges: ops.KeyRanges
     positions: Optional[torch.Tensor] = None
     bias: Optional[torch.Tensor] = None
+
+
+class _Shared:
+    """The prepared call of every thread, so that threads on one model do not see one another's masks."""
+
+    def __init__(self):
+        self._mine, self._last, self._threads = threading.local(), None, set()
+
+    def prepare(self, **call) -> None:
+        self._mine.call = self._last = _Prepared(**call)
+        self._threads.add(threading.get_ident())
+
+    def call(self) -> _Prepared:
+        call = getattr(self._mine, "call", None)
+        if call is None and len(self._threads) == 1:        # another thread goes on with it: autograd's, which computes checkpointed layers again
+            call = self._last
+        if call is None:
+            raise ValueError("native attention: prepare(...) has to be called ahead of the model, by the same thread")
+        return call
+
+    def __reduce__(self):       # a copy begins unprepared
+        return _Shared, ()
 
 
 class LlamaSelfAttention(nn.Module):
@@ -64,8 +87,9 @@ class LlamaSelfAttention(nn.Module):
     def forward(self, hidden_states, **_):
         B, L, _ = hidden_states.shape
         q, k, v = (p(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
-        q, k = ops.rotary(q, k, self.shared.positions, self.freqs)
-        return self.o_proj(ops.masked_attention(q, k, v, self.shared.ranges, scale=self.scaling)), None
+        call = self.shared.call()
+        q, k = ops.rotary(q, k, call.positions, self.freqs)
+        return self.o_proj(ops.masked_attention(q, k, v, call.ranges, scale=self.scaling)), None
 
 
 class T5SelfAttention(nn.Module):
@@ -79,7 +103,8 @@ class T5SelfAttention(nn.Module):
     def forward(self, hidden_states, **_):
         B, L, _ = hidden_states.shape
         q, k, v = (p(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2) for p in (self.q, self.k, self.v))
-        o = ops.masked_attention(q, k, v, self.shared.ranges, scale=1.0, distance_bias=self.shared.bias)
+        call = self.shared.call()
+        o = ops.masked_attention(q, k, v, call.ranges, scale=1.0, distance_bias=call.bias)
         return self.o(o.to(self.o.weight.dtype)), None
 
 
@@ -114,8 +139,7 @@ class _NativeLlama:
             layer.self_attn = LlamaSelfAttention(layer.self_attn, freqs, self.shared)
 
     def prepare(self, mask, batch, length, device):
-        self.shared.positions = torch.arange(length, device=device, dtype=torch.int32)
-        self.shared.ranges = prompt_ranges(mask, batch, length, True, device)
+        self.shared.prepare(ranges=prompt_ranges(mask, batch, length, True, device), positions=torch.arange(length, device=device, dtype=torch.int32))
 
 
 class _NativeT5:
@@ -127,13 +151,13 @@ class _NativeT5:
         self.buckets = distance_buckets(cfg.relative_attention_max_distance, cfg.relative_attention_num_buckets, device=self.table.weight.device)
 
     def prepare(self, mask, batch, length, device):
-        self.shared.ranges = prompt_ranges(mask, batch, length, False, device)
-        self.shared.bias = self.table.weight[self.buckets].t().float().contiguous()
+        self.shared.prepare(ranges=prompt_ranges(mask, batch, length, False, device), bias=self.table.weight[self.buckets].t().float().contiguous())
 
 
 def use_native_attention(model):
     """Exchanges the attention modules of a ``LlamaModel`` or ``T5EncoderModel`` in place.  Returns an object whose
-    ``prepare(mask, batch, length, device)`` has to be called ahead of each call of the model, with the tokenizer's mask or None."""
+    ``prepare(mask, batch, length, device)`` has to be called ahead of each call of the model, by the same thread, with the tokenizer's mask or
+    None."""
     kind = type(model).__name__
     if kind == "LlamaModel":
         return _NativeLlama(model)

@@ -118,6 +118,62 @@ def test_a_model_that_rotates_otherwise_than_its_configuration_says_is_refused()
     assert type(enc.model.layers[0].self_attn).__name__ == "LlamaAttention"         # as it was
 
 
+@pytest.mark.parametrize("kind", ["llama", "t5"])
+def test_two_threads_on_one_encoder_keep_their_own_masks(kind):
+    import threading
+    if kind == "llama":
+        enc = _llama(native_attention=True)[1]
+        model, call = enc.model, lambda prompts: enc(prompts)[0]
+    else:
+        enc = PromptEncoder("t5", max_length=24, dtype=torch.float32, configs=[t5_config(2, 32, 4, 64, 300)], native_attention=True)
+        enc.load_model()
+        model, call = enc.encoders[0].model, lambda prompts: enc(prompts, with_attention_mask=True)[0]
+    sets = [PROMPTS, PROMPTS[::-1]]
+    want = [call(p) for p in sets]
+    both, got, errors = threading.Barrier(2, timeout=60), [None, None], []
+    first = model.layers[0] if kind == "llama" else model.encoder.block[0]
+
+    def wait(*_):           # neither begins ahead of the other's preparation
+        both.wait()
+
+    hook = first.register_forward_pre_hook(wait)
+
+    def work(i):
+        try:
+            got[i] = call(sets[i])
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    hook.remove()
+    assert not errors
+    # the same sums in the same order, but for the products' own threads
+    assert all(torch.allclose(a, b, atol=1e-5, rtol=0) for a, b in zip(want, got)) and not torch.allclose(want[0], want[1], atol=1e-2)
+
+
+def test_a_model_that_was_not_prepared_says_so():
+    import threading
+    enc = _llama(native_attention=True)[1]
+    ids = torch.ones(1, 5, dtype=torch.long)
+    with pytest.raises(ValueError, match="prepare"):
+        enc.model(input_ids=ids, use_cache=False)
+    enc.native.prepare(None, 1, 5, "cpu")
+    want = enc.model(input_ids=ids, use_cache=False).last_hidden_state
+    got = []
+    t = threading.Thread(target=lambda: got.append(enc.model(input_ids=ids, use_cache=False).last_hidden_state))       # one has prepared: its call goes on here
+    t.start(), t.join()
+    assert torch.allclose(got[0], want, atol=1e-5, rtol=0)
+    import pickle
+    copied = copy.deepcopy(enc)
+    assert torch.equal(copied(PROMPTS)[0], enc(PROMPTS)[0])
+    with pytest.raises(ValueError, match="prepare"):
+        pickle.loads(pickle.dumps(enc.model))(input_ids=ids, use_cache=False)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_llama_on_the_kernels(dtype):
