@@ -52,6 +52,7 @@ class _Prepared(NamedTuple):
     """What the layers of one call share."""
     ranges: ops.KeyRanges
     positions: Optional[torch.Tensor] = None
+    freqs: Optional[ops.Rotary] = None
     bias: Optional[torch.Tensor] = None
 
 
@@ -78,17 +79,17 @@ class _Shared:
 
 
 class LlamaSelfAttention(nn.Module):
-    def __init__(self, inner: nn.Module, freqs: ops.Rotary, shared: _Shared):
+    def __init__(self, inner: nn.Module, shared: _Shared):
         super().__init__()
         self.q_proj, self.k_proj, self.v_proj, self.o_proj = inner.q_proj, inner.k_proj, inner.v_proj, inner.o_proj
         self.head_dim, self.scaling = inner.head_dim, inner.scaling
-        self.freqs, self.shared = freqs, shared
+        self.shared = shared
 
     def forward(self, hidden_states, **_):
         B, L, _ = hidden_states.shape
         q, k, v = (p(hidden_states).view(B, L, -1, self.head_dim).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
         call = self.shared.call()
-        q, k = ops.rotary(q, k, call.positions, self.freqs)
+        q, k = ops.rotary(q, k, call.positions, call.freqs)
         return self.o_proj(ops.masked_attention(q, k, v, call.ranges, scale=self.scaling)), None
 
 
@@ -132,14 +133,16 @@ def _check_rotary(model, freqs: ops.Rotary) -> None:
 
 class _NativeLlama:
     def __init__(self, model):
-        self.shared, freqs = _Shared(), rotary_of(model.config)
-        _check_rotary(model, freqs)
-        freqs = freqs.to(model.embed_tokens.weight.device)
+        self.shared, self.freqs = _Shared(), rotary_of(model.config)
+        _check_rotary(model, self.freqs)
+        self.freqs = self.freqs.to(model.embed_tokens.weight.device)
         for layer in model.layers:
-            layer.self_attn = LlamaSelfAttention(layer.self_attn, freqs, self.shared)
+            layer.self_attn = LlamaSelfAttention(layer.self_attn, self.shared)
 
     def prepare(self, mask, batch, length, device):
-        self.shared.prepare(ranges=prompt_ranges(mask, batch, length, True, device), positions=torch.arange(length, device=device, dtype=torch.int32))
+        self.freqs = freqs = self.freqs.to(device)          # the model may have moved
+        self.shared.prepare(ranges=prompt_ranges(mask, batch, length, True, device), freqs=freqs,
+                            positions=torch.arange(length, device=device, dtype=torch.int32))
 
 
 class _NativeT5:

@@ -175,6 +175,22 @@ def test_a_model_that_was_not_prepared_says_so():
 
 
 @pytest.mark.gpu
+def test_models_that_move_to_the_device_after_the_exchange():
+    torch.manual_seed(4)
+    cfg = llama_config(2, 256, 4, 2, 512, 1000)
+    llama = LlamaTextEncoder(max_length=64, dtype=torch.float32, config=cfg, native_attention=True)
+    t5 = PromptEncoder("t5", max_length=64, dtype=torch.float32, configs=[t5_config(2, 64, 2, 64, 300)], native_attention=True)
+    t5.load_model()
+    want = llama(PROMPTS)[0], t5(PROMPTS, with_attention_mask=True)[0]
+    llama.model.to("cuda"), t5.encoders[0].model.to("cuda")
+    got = llama(PROMPTS)[0], t5(PROMPTS, with_attention_mask=True)[0]
+    # fp32 in the library's products on either side, states of the order of 1
+    assert all(g.is_cuda and torch.allclose(g.cpu(), w, atol=2e-3, rtol=0) for g, w in zip(got, want))
+    llama.model.to("cpu")
+    assert torch.allclose(llama(PROMPTS)[0], want[0], atol=2e-4, rtol=0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_llama_on_the_kernels(dtype):
     """Heads of 128, shared, padded prompts; nearer to the fp32 states than a fiftieth, as the library's own are."""
