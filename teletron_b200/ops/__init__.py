@@ -200,8 +200,9 @@ def masked_attention(q, k, v, ranges, scale=None, softcap=None, distance_bias=No
     if _use_cuda(q, dtypes=(torch.bfloat16, torch.float16)):
         if attn_ranges.supported(q, k, v, ranges, distance_bias):
             return attn_ranges.masked_attention(q, k, v, ranges, scale, softcap, distance_bias)
-        from . import fallback
-        fallback.note("masked_attention", f"q {tuple(q.shape)} {q.dtype}")
+        if q.numel() and k.numel():             # nothing to compute is no fallback
+            from . import fallback
+            fallback.note("masked_attention", f"q {tuple(q.shape)} {q.dtype}")
     return reference.masked_attention(q, k, v, ranges, scale, softcap, distance_bias)
 
 

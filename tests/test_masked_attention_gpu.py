@@ -515,3 +515,18 @@ def test_forward_mode_derivatives_are_refused():
     assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
     # few rows by themselves and in a tile: P is rounded to bf16 against another maximum, and the output once, in each
     assert torch.allclose(got[0].float(), want[0].float(), atol=4 * 2.0 ** -8 * float(q.float().abs().max()), rtol=0)
+
+
+@pytest.mark.parametrize("B,n,m", [(0, 3, 3), (2, 0, 3), (2, 3, 0)])
+def test_empty_operands_are_no_fallback(B, n, m):
+    """No samples, no queries, a cache that holds nothing yet: what a training run with its strict kernels calls too."""
+    from teletron_b200.ops import fallback
+    q, k, v = (torch.randn(B, h, s, 64, device="cuda").to(BF16).requires_grad_() for h, s in ((4, n), (2, m), (2, m)))
+    was = fallback.strict()
+    try:
+        fallback.set_strict(True)
+        out = ops.masked_attention(q, k, v, ops.key_ranges(n, m, batch=B, device="cuda"))
+        grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    finally:
+        fallback.set_strict(was)
+    assert out.shape == (B, n, 256) and not bool(out.any()) and all(not bool(g.any()) for g in grads)
