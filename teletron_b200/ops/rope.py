@@ -52,7 +52,7 @@ class Rotary:
         return dataclasses.replace(self, inv_freq=move(self.inv_freq), half_turns=move(self.half_turns), axis=move(self.axis))
 
 
-_LARGEST = 1e30          # of an amplitude and of eps, which the kernels hold in 32 bits
+_LARGEST = 1e30          # of an amplitude, which the kernels hold in 32 bits
 # What a dictionary may hold: the kind, what belongs to the caller's other arguments or says nothing about angles, and the keys of any kind (a kind passes
 # over those of the others, as configurations carry them along).  A key that is not here might change angles in a way that is not followed.
 _KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "max_position_embeddings", "finetuned", "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor",
@@ -211,8 +211,8 @@ def by_axis(positions, num_axes: int):
 def check_norm(q, k, q_weight, k_weight, eps) -> None:
     if k is None:
         raise ValueError("qk_norm_rotary: expected queries and keys")
-    if not 0 <= eps <= _LARGEST:            # held in 32 bits
-        raise ValueError(f"eps: expected a number from 0 to {_LARGEST}, got {eps}")
+    if not 0 <= eps < math.inf:
+        raise ValueError(f"eps: expected a number of 0 or more, got {eps}")
     for x, w, n in ((q, q_weight, "q_weight"), (k, k_weight, "k_weight")):
         if w.dim() != 1 or w.shape[0] != x.shape[3] or w.dtype is not x.dtype or w.get_device() != x.get_device():
             raise ValueError(f"{n}: expected [{x.shape[3]}] {x.dtype} on {x.device}, got {tuple(w.shape)} {w.dtype} on {w.device}")

@@ -264,16 +264,3 @@ def test_forward_mode_derivatives_are_refused_not_lost(monkeypatch):
         assert torch.allclose(fwd.unpack_dual(out).tangent, ops.rotary(q, None, pos, freqs)[0], atol=1e-5)
     with pytest.raises(RuntimeError):           # the same by transformation
         torch.func.jvp(lambda x: rope.rotary(x, k, pos, (0, 0, 1), freqs)[0], (q,), (q,))
-
-
-@pytest.mark.parametrize("eps", [1e39, 1e300])
-def test_eps_beyond_32_bits_is_refused(eps):
-    """By the operator, not by the packing of the native call's arguments."""
-    import struct
-    a, w = _operands(), torch.ones(8)
-    with pytest.raises((OverflowError, struct.error)):
-        struct.pack("f", eps)
-    with pytest.raises(ValueError):
-        ops.qk_norm_rotary(a["q"], a["k"], w, w, a["positions"], a["freqs"], eps=eps)
-    for good in (0.0, 1e30):
-        ops.qk_norm_rotary(a["q"], a["k"], w, w, a["positions"], a["freqs"], eps=good)
