@@ -2,7 +2,8 @@
 //
 // What bounds it is reading keys and values once, so the steps of 16 keys of all samples and key heads, counted as the samples' runs have them, are
 // dealt to the CTAs in equal shares, and a share's steps to its four warps.  Every warp streams its keys and values through a ring of its own in
-// shared memory (16-byte asynchronous copies, three steps deep: 96 KB in flight per CTA at heads of 128) and keeps running maxima, sums and outputs
+// shared memory (16-byte asynchronous copies; three steps of 8 KB a warp at heads of 128, 96 KB a CTA, of which two steps are under way while the third is
+// worked on: 64 KB) and keeps running maxima, sums and outputs
 // of its 16 or 32 rows (the queries of all heads of the group, so that shared keys are read once) in registers; the products are mma.sync of 16 x 8 x
 // 16, which a tile of 128 queries on tcgen05 would leave seven eighths empty.  Warps are joined through shared memory, CTAs by a second kernel in a
 // fixed order.
@@ -60,7 +61,9 @@ template <int D> __device__ __forceinline__ uint32_t place(uint32_t base, int ro
     return base + row * (D * 2) + ((piece ^ (row & 7)) << 4);
 }
 
-constexpr int kMaxBatch = 128;          // of shared steps; more samples are many CTAs by themselves
+// of shared steps; more samples are many CTAs by themselves (one key head, 4 rows, us: 128 samples in shares against 129 without, 1024 keys 24.6 / 24.6, 4096
+// 65.5 / 65.5, 8192 114.7 / 110.6)
+constexpr int kMaxBatch = 128;
 static_assert(kMaxBatch <= kThreads, "a thread a sample");
 
 template <int D, int MT> struct Few {
@@ -543,6 +546,8 @@ int pick(const tt_ranges_args& a, const FewParams& p, bool gen, int dev, cudaStr
 // At most 32 rows of a group (beyond them, and from 17 on over few short caches, the kernel for tiles is the faster one).  In us, tiles against this:
 // 64 units of 8192 keys, heads of 128, 32 rows 106 / 76, 4 rows 106 / 46; 8 units of 1024 keys, 16 rows 14.5 / 13.5, 32 rows 14.5 / 20.2; 64 units of
 // 1024, 32 rows 20.7 / 28.4, of 4096 57 / 46; 256 units of 256, 32 rows 29 / 21.  Heads of 64, 32 rows: 64 units of 1024 19.0 / 18.2.
+// Beyond them long caches are far from their floor, as the kernel for tiles gives one CTA two heads' tiles and all keys: eight heads on one key head over 65536
+// keys, 4 new tokens 43 us, 5 776; 32 heads on 8 key heads over as many, 8 new tokens 72, 9 778, 128 789.
 bool tt_ranges_few_rows(const tt_ranges_args& a) {
     const long rows = (long)(a.q_heads / a.k_heads) * a.q_len, units = (long)a.batch * a.k_heads;
     const bool short_caches = rows > 16 && a.head_dim == 128 && a.kv_len <= 1536 && 2 * units <= tt_device().sms;

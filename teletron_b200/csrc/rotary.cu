@@ -12,7 +12,7 @@
 // elements are being loaded.  The kernels are bound by memory: 2 passes over q and k forward, 3 for the norm's backward.  Measured (bf16, heads of
 // 128): 24 + 24 heads of 32400 tokens, rotation there and back 252 us (6.3 TB/s), norm and rotation forward 138 (5.8), backward 199 (6.0) and 4 for
 // the weights' gradients; 4 x 8192 tokens of 32 + 8 heads (fp16) 107 (6.3); eight tokens 3.4, most of it the launch.  fp32 heads of 80 with 20
-// rotated elements go two elements a lane (142 MB there and back in 56 us, 2.5 TB/s).
+// rotated elements go two elements a lane, as do all pairs in the half layout that 16 bytes do not divide (142 MB there and back in 56 us, 2.5 TB/s).
 #include <cuda_fp16.h>
 #include <limits.h>
 
@@ -231,6 +231,9 @@ struct Params {
     float amplitude, sin_amplitude, eps, inv_D;
 };
 
+// Three CTAs an SM leave 80 registers a thread, of which the norm's forward on eight 16-bit elements a lane spills 72 - 84 bytes.  Two CTAs without spills: 24 + 24
+// heads of 32400 tokens 148.5 us against 146.5, 8 x 256 tokens of 32 + 8 heads 15.5 - 16.4 against 17.4, 3 x 1001 of 12 + 4 heads of 64 level.
+//
 // A group of 2^log_l lanes holds one head of one token; a warp's groups take consecutive heads.  A unit is a token with all heads of q and k
 // (`whole`), or with `hpu` heads of one of them; consecutive warps take consecutive tokens, whose rows are neighbours in the head-major
 // output.  The norm's backward keeps q and k apart, since a CTA sums one weight's gradient: CTAs below ctas_q work on q, the others on k.

@@ -213,7 +213,8 @@ _NO_BACKWARD = bytes(_TAIL.size - 16)
 _SCRATCH = struct.Struct("@PP")
 # Up to so many keys a trained call keeps the output before rounding: dP - delta of few keys is small against either.  Relative errors of dQ and dK without
 # and with it: 2 keys 3.9e-3 / 2.4e-3, 16 causal ones 2.8e-3 / 2.3e-3, 128 2.6e-3 / 2.4e-3, 512 2.5e-3 / 2.3e-3 (rounding the results alone: 1.7e-3); forward and
-# backward of 8 x 128 tokens, 32 + 8 heads of 128, 40 / 45 us, of 8 x 256 67 / 83.
+# backward of 8 x 128 tokens, 32 + 8 heads of 128, 40 / 45 us, of 8 x 256 67 / 83.  It goes by the length of the keys, which the host knows, not by what a query
+# sees: documents of a few tokens within longer sequences keep the larger error.
 WIDE_KEYS = 128
 FEW_ROWS = 32           # queries of a group that the kernels for few queries take
 
