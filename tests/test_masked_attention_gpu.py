@@ -530,3 +530,44 @@ def test_empty_operands_are_no_fallback(B, n, m):
     finally:
         fallback.set_strict(was)
     assert out.shape == (B, n, 256) and not bool(out.any()) and all(not bool(g.any()) for g in grads)
+
+
+def test_two_threads_at_once():
+    """Rotation and attention, forward and backward, by two threads on streams of their own: the bits of one alone."""
+    import threading
+    freqs = ops.rotary_frequencies(64, device="cuda")
+
+    def work(seed, n, hk):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        q, k, v = (torch.randn(2, h, n, 64, device="cuda", generator=g).to(BF16).requires_grad_() for h in (4, hk, hk))
+        dout = torch.randn(2, n, 256, device="cuda", generator=g).to(BF16)
+        new = torch.randn(2, 4, 1, 64, device="cuda", generator=g).to(BF16)
+        out = []
+        for _ in range(20):
+            a, b = ops.rotary(q, k, torch.arange(n, device="cuda"), freqs)
+            y = ops.masked_attention(a, b, v, ops.key_ranges(n, batch=2, causal=True, documents=[0, n // 3, n], device="cuda"))
+            one = ops.masked_attention(new, b.detach(), v.detach(), ops.key_ranges(1, n, batch=2, device="cuda"))
+            out = [y.detach(), one, *torch.autograd.grad(y, (q, k, v), dout)]
+        return out
+
+    jobs = [(1, 300, 2), (2, 513, 4)]
+    want = [work(*job) for job in jobs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = work(*jobs[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    status.check_all(what="test")
+    assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
