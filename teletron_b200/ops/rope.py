@@ -81,7 +81,7 @@ def _check_scaling(scaling: dict, theta: float) -> str:
     unknown = [k for k, v in scaling.items() if k not in _KEYS and v is not None]
     if unknown:
         raise ValueError(f"rotary scaling: unknown keys {unknown}")
-    kind = scaling.get("rope_type", scaling.get("type"))
+    kind = scaling.get("rope_type") or scaling.get("type")
     if kind is None:
         if scaling.get("factor") is not None:
             raise ValueError("rotary scaling: a factor needs a 'rope_type'")

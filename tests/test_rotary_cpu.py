@@ -228,7 +228,7 @@ def test_what_configurations_hold_beside_the_scaling_is_taken():
     plain = ops.rotary_frequencies(128, 500000.0)
     for scaling in ({}, dict(rope_type="default", rope_theta=500000.0), dict(type="default", partial_rotary_factor=0.5), dict(rope_type="default", factor=None),
                     dict(rope_type="default", factor=1.0, original_max_position_embeddings=8192), dict(rope_theta=500000.0),
-                    dict(rope_type="linear", factor=1.0, finetuned=True, max_position_embeddings=8192)):
+                    dict(rope_type="linear", factor=1.0, finetuned=True, max_position_embeddings=8192), dict(rope_type=None, type="linear", factor=1.0)):
         got = ops.rotary_frequencies(128, 500000.0, scaling=scaling)
         assert torch.equal(got.inv_freq, plain.inv_freq) and got.amplitude == 1.0
 
